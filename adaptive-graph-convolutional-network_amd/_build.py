@@ -11,8 +11,11 @@ ARCH = "gfx950"
 # -Wno-pass-failed: "loop not unrolled" remarks for unroll hints on runtime-bounded loops of the per-graph kernels
 # -fno-slp-vectorize: keeps adjacent scalar fp32 adds / fmas as v_add_f32 / v_fma_f32; the packed v_pk_*_f32 forms the
 # SLP vectoriser would build issue several times slower on gfx950 (measured in the pairwise-distance loop)
+# -packed-fp32-ops (a feature of the device target; the host pass warns that it does not know it): no v_pk_*_f32 from ext_vector
+# arithmetic either -- some of their forms have given wrong results on this hardware
 # -fvisibility=hidden: the dynamic symbol table is the functions of include/agcn.h (AGCN_API) and nothing else
 FLAGS = ["-O3", "-ffp-contract=off", "-fno-slp-vectorize", "-fPIC", "-shared", "-std=c++17", "-Wall",
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
          "-Wno-unused-function", "-Wno-pass-failed", "-fvisibility=hidden", "-fvisibility-inlines-hidden"]
 
 
