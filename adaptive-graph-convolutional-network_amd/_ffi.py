@@ -55,6 +55,22 @@ class DenseDesc(C.Structure):
                 ("ldx", C.c_int32), ("ldy", C.c_int32), ("ldadd", C.c_int32), ("flags", C.c_uint32)]
 
 
+class NormDesc(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("F", C.c_int32), ("norm", C.c_int32), ("gate", C.c_int32), ("gate_activation", C.c_int32),
+                ("x_dtype", C.c_int32), ("z_dtype", C.c_int32), ("ldx", C.c_int32), ("ldz", C.c_int32), ("ldg", C.c_int32),
+                ("eps", C.c_float)]
+
+
+class NormInputs(C.Structure):
+    _fields_ = [("z", C.c_void_p), ("x", C.c_void_p), ("gate", C.c_void_p), ("scale", C.c_void_p), ("post_weight", C.c_void_p),
+                ("post_bias", C.c_void_p), ("pre_weight", C.c_void_p), ("pre_bias", C.c_void_p)]
+
+
+class NormGrads(C.Structure):
+    _fields_ = [("dz", C.c_void_p), ("dx", C.c_void_p), ("dgate", C.c_void_p), ("dscale", C.c_void_p),
+                ("dpost_weight", C.c_void_p), ("dpost_bias", C.c_void_p), ("dpre_weight", C.c_void_p), ("dpre_bias", C.c_void_p)]
+
+
 class GraphStoreC(C.Structure):
     _fields_ = [("n_graphs", C.c_int64), ("F", C.c_int32), ("reserved", C.c_int32), ("n", C.c_void_p),
                 ("row_off", C.c_void_p), ("X", C.c_void_p), ("rowptr", C.c_void_p), ("col", C.c_void_p),
@@ -108,6 +124,9 @@ def dispatch_flags(base=0, **knobs):
 MODE = {"reference": 0, "paper": 1}
 VARIANT = {"SGC_LL": 0, "SGC_LL_Reslap": 1}
 ACT = {None: 0, "linear": 0, "relu": 1, "tanh": 2}
+GATE_ACT = {None: 0, "linear": 0, "tanh": 2, "sigmoid": 3}          # agcn_norm_gate_residual_*
+FFN_ACT = {"relu": 1, "sigmoid": 3, "silu": 4, "gelu": 5}           # agcn_gated_ffn_*
+NORM = {"rms": 0, "layer": 1}
 RESERVE_HEADER_BYTES = 65536      # include/agcn.h: AGCN_RESERVE_HEADER_BYTES (what must be zero when a reserve is first used)
 
 # every symbol include/agcn.h declares (tests/test_abi.py checks the two lists agree)
@@ -122,6 +141,8 @@ SYMBOLS = [
     "agcn_rows_dense_scaled_forward_ws",
     "agcn_multitask_ce_workspace_bytes", "agcn_multitask_ce_forward", "agcn_multitask_ce_backward",
     "agcn_graph_pool_forward", "agcn_graph_pool_backward",
+    "agcn_norm_gate_residual_forward", "agcn_norm_gate_residual_backward_workspace_bytes", "agcn_norm_gate_residual_backward",
+    "agcn_clip_workspace_bytes", "agcn_clip_by_global_norm",
     "agcn_store_batch_sizes", "agcn_store_pack_batch", "agcn_store_stage_bytes", "agcn_store_stage_batch",
     "agcn_cast_rows", "agcn_rows_pack", "agcn_rows_unpack",
     "agcn_version", "agcn_last_error", "agcn_get_lds_limit", "agcn_set_lds_limit",
@@ -183,6 +204,17 @@ def _declare(lib):
     lib.agcn_multitask_ce_forward.argtypes = [I32, I32, I32, P, I32, P, P, P, P, C.c_float, P, P, P, SZ, P]
     lib.agcn_multitask_ce_backward.restype = C.c_int
     lib.agcn_multitask_ce_backward.argtypes = [I32, I32, I32, P, I32, P, P, P, P, C.c_float, P, P, P, P, P, SZ, P]
+    lib.agcn_norm_gate_residual_forward.restype = C.c_int
+    lib.agcn_norm_gate_residual_forward.argtypes = [C.POINTER(NormDesc), P, P, C.POINTER(NormInputs), P, P, P, P]
+    lib.agcn_norm_gate_residual_backward_workspace_bytes.restype = SZ
+    lib.agcn_norm_gate_residual_backward_workspace_bytes.argtypes = [C.POINTER(NormDesc), P]
+    lib.agcn_norm_gate_residual_backward.restype = C.c_int
+    lib.agcn_norm_gate_residual_backward.argtypes = [C.POINTER(NormDesc), P, P, C.POINTER(NormInputs), P, P, P,
+                                                     C.POINTER(NormGrads), P, SZ, P]
+    lib.agcn_clip_workspace_bytes.restype = SZ
+    lib.agcn_clip_workspace_bytes.argtypes = [I32, P, P]
+    lib.agcn_clip_by_global_norm.restype = C.c_int
+    lib.agcn_clip_by_global_norm.argtypes = [I32, P, P, P, P, C.c_float, P, P, SZ, P]
     lib.agcn_rows_pack.restype = C.c_int
     lib.agcn_rows_pack.argtypes = [P, P, P, I32, I32, I32, P, I32, P]
     lib.agcn_rows_unpack.restype = C.c_int

@@ -1,0 +1,643 @@
+// The frame of a residual block in one pass over the rows: the norm behind the block, its gate and residual scale, the residual
+// sum, and the norm in front of the next block (beside BlockEnd, models/layers/blockend.py:67-86, whose sum has neither):
+//     u = N(z; w, b)          N: rms  v / sqrt(mean v^2 + eps) * w   |   layer  (v - mean v) / sqrt(var v + eps) * w + b
+//     y = x + s (.) a(g) (.) u
+//     h = N(y; w', b')
+// Backward, with D = dy + N'(dh; y):
+//     dx = D;  dg = D s u a'(g);  dz = N'(D s a(g); z);  N'(d; v) = r (d w - vh mean(d w vh) [- mean(d w)]),  vh = (v [- mean]) r
+//     with q1 = sum D a zh and q2 = sum D a over the rows:  dw = s q1, db = s q2, ds = w q1 + b q2;
+//     dw' = sum dh yh, db' = sum dh;  a gate per graph:  dg = a'(g) s (w sum D zh + b sum D) over the graph's rows.
+// Bound by memory: every operand is read once and every result written once (the row stays in registers between the two norms
+// and through all reductions).  L lanes share a row (8 consecutive elements per lane and vector, so that a lane keeps the
+// parameters and the column sums of ITS columns in registers over all rows it meets).  Sums, means and column sums are fp32
+// (a column sum's partials, one per workgroup, are added in a fixed order: no atomics); rounding happens where a result is
+// stored, and h is taken from the unrounded y.  Pad rows give zeros and take part in no sum.
+#include <hip/hip_bf16.h>
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "agcn_device.h"
+#include "sgc_kernels.h"
+
+namespace agcn {
+namespace {
+constexpr int V = 8;                    // elements per vector
+constexpr int kGraphRows = 64;          // per-graph gates: rows of a graph that one workgroup adds up
+
+struct NormArgs {
+  AgcnNormDesc d;
+  // plan (nullable: no pad rows, no graphs)
+  const int32_t *n, *row_off, *row_graph;
+  int32_t B, splits;
+  const void *z, *x, *gate, *dy, *dh;
+  const float *scale, *w, *b, *w2, *b2;
+  void *y, *h, *dz, *dx, *dgate;
+  float* stats;                         // [rows][4]: mean z, 1 / deviation of z, mean y, 1 / deviation of y
+  float* part;                          // [units][4][F]
+  int32_t units, pads;
+};
+
+typedef uint32_t u4f __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u4h __attribute__((ext_vector_type(4), aligned(2)));
+
+// eight elements, columns c .. c + 7 of a row of F (0 beyond), as floats.  Vectors are read at the alignment of an element: the
+// target runs in unaligned access mode, and odd widths start every row elsewhere.
+__device__ __forceinline__ void load8(const float* p, int c, int F, float* v) {
+  if (c + V <= F) {
+    const u4f a = *reinterpret_cast<const u4f*>(p + c), b = *reinterpret_cast<const u4f*>(p + c + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { v[i] = __uint_as_float(a[i]); v[4 + i] = __uint_as_float(b[i]); }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = c + i < F ? p[c + i] : 0.f;
+  }
+}
+__device__ __forceinline__ void load8(const __hip_bfloat16* p_, int c, int F, float* v) {
+  const uint16_t* p = reinterpret_cast<const uint16_t*>(p_);
+  if (c + V <= F) {
+    const u4h a = *reinterpret_cast<const u4h*>(p + c);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(a[i] << 16); v[2 * i + 1] = __uint_as_float(a[i] & 0xffff0000u); }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = c + i < F ? __uint_as_float((uint32_t)p[c + i] << 16) : 0.f;
+  }
+}
+__device__ __forceinline__ void store8(float* p, int c, int F, const float* v) {
+  if (c + V <= F) {
+    u4f a, b;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { a[i] = __float_as_uint(v[i]); b[i] = __float_as_uint(v[4 + i]); }
+    *reinterpret_cast<u4f*>(p + c) = a;
+    *reinterpret_cast<u4f*>(p + c + 4) = b;
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) if (c + i < F) p[c + i] = v[i];
+  }
+}
+__device__ __forceinline__ uint32_t pk_bf(float a, float b) {
+  typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, (b2){(__bf16)a, (__bf16)b});
+}
+__device__ __forceinline__ void store8(__hip_bfloat16* p_, int c, int F, const float* v) {
+  uint16_t* p = reinterpret_cast<uint16_t*>(p_);
+  if (c + V <= F) {
+    u4h a;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] = pk_bf(v[2 * i], v[2 * i + 1]);
+    *reinterpret_cast<u4h*>(p + c) = a;
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) if (c + i < F) p[c + i] = (uint16_t)pk_bf(v[i], 0.f);
+  }
+}
+
+__device__ __forceinline__ float gate_act(int act, float g) {
+  if (act == AGCN_ACT_TANH) return tanhf(g);
+  if (act == AGCN_ACT_SIGMOID) return 1.f / (1.f + expf(-g));
+  return g;
+}
+// a'(g), from g: 1 - a^2 and a (1 - a) lose their digits where the activation is flat (e^-2|g| and e^-|g| do not)
+__device__ __forceinline__ float gate_slope(int act, float g) {
+  if (act == AGCN_ACT_LINEAR) return 1.f;
+  const float e = expf(act == AGCN_ACT_TANH ? -2.f * fabsf(g) : -fabsf(g)), d = 1.f / (1.f + e);
+  return (act == AGCN_ACT_TANH ? 4.f : 1.f) * e * d * d;
+}
+
+// Sums of N values over the L lanes of a row; every lane gets them.  L > 64: over the whole workgroup through `red`
+// (two areas used in turn, so that one barrier per call is enough).
+template <int L, int N>
+__device__ __forceinline__ void row_sums(float (&v)[N], float* red, int& turn) {
+#pragma unroll
+  for (int o = (L < 64 ? L : 64) >> 1; o; o >>= 1)
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], o);
+  if (L > 64) {
+    constexpr int W = L > 64 ? L / 64 : 1;
+    float* r = red + turn * (2 * W);
+    turn ^= 1;
+    if ((threadIdx.x & 63) == 0)
+#pragma unroll
+      for (int i = 0; i < N; ++i) r[(threadIdx.x >> 6) * 2 + i] = v[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      float s = 0.f;
+#pragma unroll
+      for (int w = 0; w < W; ++w) s += r[w * 2 + i];
+      v[i] = s;
+    }
+  }
+}
+
+template <int L> constexpr int threads_of() { return L < 256 ? 256 : L; }
+
+// Normalises the row in place: v -> vh; returns mean and 1 / deviation.  Two passes over the registers: the sum of squares is
+// taken around the mean, not as a difference of two large sums.
+template <int L, int NV>
+__device__ __forceinline__ void normalise(float (&v)[NV][V], const NormArgs& a, int lane, float& mean, float& r, float* red, int& turn) {
+  const float inv = 1.f / (float)a.d.F;
+  mean = 0.f;
+  if (a.d.norm == AGCN_NORM_LAYER) {
+    float s[1] = {0.f};
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int i = 0; i < V; ++i) s[0] += v[k][i];          // (columns beyond F hold 0)
+    row_sums<L, 1>(s, red, turn);
+    mean = s[0] * inv;
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[k][i] = (k * L + lane) * V + i < a.d.F ? v[k][i] - mean : 0.f;
+  }
+  float q[1] = {0.f};
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+#pragma unroll
+    for (int i = 0; i < V; ++i) q[0] = fmaf(v[k][i], v[k][i], q[0]);
+  row_sums<L, 1>(q, red, turn);
+  r = 1.f / sqrtf(fmaf(q[0], inv, a.d.eps));
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[k][i] *= r;
+}
+
+__device__ __forceinline__ void load_params(const NormArgs& a, int c, int F, float* s, float* w, float* b) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) { s[i] = 1.f; w[i] = 1.f; b[i] = 0.f; }
+  if (a.scale) load8(a.scale, c, F, s);
+  if (a.w) load8(a.w, c, F, w);
+  if (a.b) load8(a.b, c, F, b);
+}
+
+__device__ __forceinline__ bool is_pad(const NormArgs& a, int64_t row) {
+  if (!a.pads) return false;
+  const int g = a.row_graph[row];
+  return (int)row - a.row_off[g] >= a.n[g];
+}
+
+template <typename TX, typename TZ, int L, int NV>
+__global__ __launch_bounds__(threads_of<L>()) void norm_forward_kernel(NormArgs a) {
+  constexpr int R = threads_of<L>() / L;                    // rows side by side
+  __shared__ float red[4 * (L > 64 ? L / 64 : 1)];
+  const int lane = threadIdx.x % L, F = a.d.F;
+  int turn = 0;
+  float w[NV][V], b[NV][V], w2[NV][V], b2[NV][V], s[NV][V];
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int c = (k * L + lane) * V;
+#pragma unroll
+    for (int i = 0; i < V; ++i) { w2[k][i] = 1.f; b2[k][i] = 0.f; }
+    load_params(a, c, F, s[k], w[k], b[k]);
+    if (a.w2) load8(a.w2, c, F, w2[k]);
+    if (a.b2) load8(a.b2, c, F, b2[k]);
+  }
+  const int64_t step = (int64_t)gridDim.x * R;
+  // (the loop runs on the workgroup's first row: all its lanes meet at the barriers of row_sums)
+  for (int64_t r0 = (int64_t)blockIdx.x * R; r0 < a.d.rows; r0 += step) {
+    const int64_t row = r0 + threadIdx.x / L;
+    const bool live = row < a.d.rows, pad = live && is_pad(a, row);
+    float y[NV][V], zz[NV][V];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int c = (k * L + lane) * V;
+#pragma unroll
+      for (int i = 0; i < V; ++i) { y[k][i] = 0.f; zz[k][i] = 0.f; }
+      if (live && !pad) {
+        load8(static_cast<const TX*>(a.x) + row * a.d.ldx, c, F, y[k]);
+        if (a.z) load8(static_cast<const TZ*>(a.z) + row * a.d.ldz, c, F, zz[k]);
+      }
+    }
+    float mz = 0.f, rz = 1.f, my = 0.f, ry = 1.f;
+    if (a.z) {
+      if (a.w) normalise<L, NV>(zz, a, lane, mz, rz, red, turn);
+      const int64_t grow = a.d.gate == AGCN_GATE_GRAPH ? (live ? a.row_graph[row] : 0) : row;
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int c = (k * L + lane) * V;
+        float g[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) g[i] = 1.f;
+        if (a.gate && live && !pad) {
+          load8(static_cast<const TZ*>(a.gate) + grow * a.d.ldg, c, F, g);
+#pragma unroll
+          for (int i = 0; i < V; ++i) g[i] = gate_act(a.d.gate_activation, g[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) y[k][i] = fmaf(s[k][i] * g[i], fmaf(zz[k][i], w[k][i], b[k][i]), y[k][i]);
+        if (c + V > F)
+#pragma unroll
+          for (int i = 0; i < V; ++i) if (c + i >= F) y[k][i] = 0.f;
+        if (live) {
+          if (pad)
+#pragma unroll
+            for (int i = 0; i < V; ++i) y[k][i] = 0.f;
+          store8(static_cast<TX*>(a.y) + row * F, c, F, y[k]);
+        }
+      }
+    }
+    if (a.h) {
+      normalise<L, NV>(y, a, lane, my, ry, red, turn);
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int c = (k * L + lane) * V;
+        float o[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) o[i] = pad ? 0.f : fmaf(y[k][i], w2[k][i], b2[k][i]);
+        if (live) store8(static_cast<TZ*>(a.h) + row * F, c, F, o);
+      }
+    }
+    if (a.stats && live && lane == 0) *reinterpret_cast<f32x4*>(a.stats + row * 4) = (f32x4){mz, rz, my, ry};
+  }
+}
+
+// One workgroup walks a strip of rows (no gate per graph: rows block, block + grid, ..; with one: up to kGraphRows rows of one
+// graph) and leaves the partial sums of its columns: q1, q2 (per graph: sum D zh, sum D), q3 = sum dh yh, q4 = sum dh.
+// y is formed again from x, z and the gate, which have to be read anyway (x in y's place): the stored y may be rounded to
+// bf16, and a row whose features differ by less than that rounding would get a wrong yh.
+template <typename TX, typename TZ, int L, int NV>
+__global__ __launch_bounds__(threads_of<L>(), 2) void norm_backward_kernel(NormArgs a) {
+  constexpr int T = threads_of<L>(), R = T / L;
+  __shared__ float red[4 * (L > 64 ? L / 64 : 1)];
+  __shared__ float cols[R > 1 ? T * V : 1];
+  const int lane = threadIdx.x % L, rl = threadIdx.x / L, F = a.d.F;
+  int turn = 0;
+  const float inv = 1.f / (float)F;
+  const bool per_graph = a.d.gate == AGCN_GATE_GRAPH, layer = a.d.norm == AGCN_NORM_LAYER;
+  int64_t row_begin, row_end, step;
+  if (per_graph) {
+    const int g = blockIdx.x / a.splits, sp = blockIdx.x - g * a.splits;
+    const int lo = sp * kGraphRows, all = a.row_off[g + 1] - a.row_off[g];   // pad rows too: their gradients are written (0)
+    if (lo >= all) return;
+    row_begin = a.row_off[g] + lo;
+    row_end = a.row_off[g] + (all < lo + kGraphRows ? all : lo + kGraphRows);
+    step = R;
+  } else {
+    row_begin = (int64_t)blockIdx.x * R;
+    row_end = a.d.rows;
+    step = (int64_t)gridDim.x * R;
+  }
+  float q1[NV][V], q2[NV][V], q3[NV][V], q4[NV][V];
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+#pragma unroll
+    for (int i = 0; i < V; ++i) { q1[k][i] = 0.f; q2[k][i] = 0.f; q3[k][i] = 0.f; q4[k][i] = 0.f; }
+  for (int64_t r0 = row_begin; r0 < row_end; r0 += step) {
+    const int64_t row = r0 + rl;
+    const bool live = row < row_end, pad = live && is_pad(a, row), use = live && !pad;
+    f32x4 st = {0.f, 1.f, 0.f, 1.f};
+    if (use) st = *reinterpret_cast<const f32x4*>(a.stats + row * 4);
+    // D: the gradient of y (dx); yh: y, then normalised; zh; g: the gate before its activation
+    float D[NV][V], yh[NV][V], zh[NV][V], g[NV][V];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int c = (k * L + lane) * V;
+#pragma unroll
+      for (int i = 0; i < V; ++i) { D[k][i] = 0.f; yh[k][i] = 0.f; zh[k][i] = 0.f; g[k][i] = 0.f; }
+      if (use) {
+        load8(static_cast<const TX*>(a.x) + row * a.d.ldx, c, F, yh[k]);
+        if (a.z) load8(static_cast<const TZ*>(a.z) + row * a.d.ldz, c, F, zh[k]);
+        if (a.dy) load8(static_cast<const TX*>(a.dy) + row * F, c, F, D[k]);
+        if (a.gate) {
+          load8(static_cast<const TZ*>(a.gate) + (per_graph ? (int64_t)a.row_graph[row] : row) * a.d.ldg, c, F, g[k]);
+        }
+      }
+      if (a.z) {
+        float s[V], w[V], b[V];
+        load_params(a, c, F, s, w, b);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          zh[k][i] = c + i < F && use ? (zh[k][i] - st.x) * st.y : 0.f;   // (no post norm: mean 0, deviation 1)
+          const float ga = a.gate ? gate_act(a.d.gate_activation, g[k][i]) : 1.f;
+          yh[k][i] = fmaf(s[i] * ga, fmaf(zh[k][i], w[i], b[i]), yh[k][i]);
+        }
+      }
+    }
+    if (a.dh) {
+      float e[NV][V], m[2] = {0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int c = (k * L + lane) * V;
+        float w2[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) e[k][i] = 0.f;
+        if (use) load8(static_cast<const TZ*>(a.dh) + row * F, c, F, e[k]);
+        load8(a.w2, c, F, w2);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          yh[k][i] = c + i < F && use ? (yh[k][i] - st.z) * st.w : 0.f;
+          q3[k][i] = fmaf(e[k][i], yh[k][i], q3[k][i]);
+          q4[k][i] += e[k][i];
+          e[k][i] *= w2[i];
+          m[0] = fmaf(e[k][i], yh[k][i], m[0]);
+          m[1] += e[k][i];
+        }
+      }
+      row_sums<L, 2>(m, red, turn);
+      const float m0 = m[0] * inv, m1 = layer ? m[1] * inv : 0.f;
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i) D[k][i] = fmaf(st.w, e[k][i] - fmaf(yh[k][i], m0, m1), D[k][i]);
+    }
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int c = (k * L + lane) * V;
+#pragma unroll
+      for (int i = 0; i < V; ++i) D[k][i] = c + i < F && use ? D[k][i] : 0.f;
+      if (live) store8(static_cast<TX*>(a.dx) + row * F, c, F, D[k]);
+    }
+    if (a.z) {
+      float m[2] = {0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int c = (k * L + lane) * V;
+        float s[V], w[V], b[V], dg[V];
+        load_params(a, c, F, s, w, b);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float ga = a.gate ? gate_act(a.d.gate_activation, g[k][i]) : 1.f;
+          const float Dq = per_graph ? D[k][i] : D[k][i] * ga;
+          q1[k][i] = fmaf(Dq, zh[k][i], q1[k][i]);
+          q2[k][i] += Dq;
+          dg[i] = a.gate ? D[k][i] * s[i] * fmaf(zh[k][i], w[i], b[i]) * gate_slope(a.d.gate_activation, g[k][i]) : 0.f;
+          D[k][i] *= s[i] * ga * w[i];                           // gradient of zh
+          m[0] = fmaf(D[k][i], zh[k][i], m[0]);
+          m[1] += D[k][i];
+        }
+        if (a.d.gate == AGCN_GATE_ROW && live) store8(static_cast<TZ*>(a.dgate) + row * F, c, F, dg);
+      }
+      float m0 = 0.f, m1 = 0.f;
+      if (a.w) {
+        row_sums<L, 2>(m, red, turn);
+        m0 = m[0] * inv;
+        m1 = layer ? m[1] * inv : 0.f;
+      }
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int c = (k * L + lane) * V;
+        float o[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) o[i] = st.y * (D[k][i] - fmaf(zh[k][i], m0, m1));
+        if (live) store8(static_cast<TZ*>(a.dz) + row * F, c, F, o);
+      }
+    }
+  }
+  // partial column sums of the workgroup: the R row lanes of a column through LDS, in order
+  float* part = a.part + (int64_t)blockIdx.x * 4 * F;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if ((j < 2 && !a.z) || (j >= 2 && !a.dh)) continue;
+    float(&q)[NV][V] = j == 0 ? q1 : j == 1 ? q2 : j == 2 ? q3 : q4;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      if (R > 1) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < V; ++i) cols[(rl * L + lane) * V + i] = q[k][i];
+        __syncthreads();
+        for (int e = threadIdx.x; e < L * V; e += T) {
+          float sum = 0.f;
+          for (int r = 0; r < R; ++r) sum += cols[r * L * V + e];
+          if (k * L * V + e < F) part[(int64_t)j * F + k * L * V + e] = sum;
+        }
+      } else {
+        store8(part + (int64_t)j * F, (k * L + lane) * V, F, q[k]);
+      }
+    }
+  }
+}
+
+struct ReduceArgs {
+  NormArgs a;
+  float *dscale, *dw, *db, *dw2, *db2;
+};
+
+// Adds the workgroups' partial column sums (64 columns per workgroup, 16 row lanes, then those in order) and forms the
+// parameters' gradients.
+__global__ __launch_bounds__(1024) void norm_params_kernel(ReduceArgs p) {
+  __shared__ float s[4][16][64];
+  const NormArgs& a = p.a;
+  const int F = a.d.F, cl = threadIdx.x & 63, rl = threadIdx.x >> 6, c = blockIdx.x * 64 + cl;
+  float q[4] = {0.f, 0.f, 0.f, 0.f};
+  if (c < F) {
+    const bool per_graph = a.d.gate == AGCN_GATE_GRAPH;
+    for (int u = rl; u < a.units; u += 16) {
+      float f = 1.f;
+      if (per_graph) {
+        const int g = u / a.splits, sp = u - g * a.splits;
+        if (sp * kGraphRows >= a.row_off[g + 1] - a.row_off[g]) continue;
+        const int64_t at = (int64_t)g * a.d.ldg + c;
+        const float gv = a.d.z_dtype == AGCN_DTYPE_BF16
+                             ? __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(a.gate)[at] << 16)
+                             : static_cast<const float*>(a.gate)[at];
+        f = gate_act(a.d.gate_activation, gv);
+      }
+      const float* t = a.part + (int64_t)u * 4 * F + c;
+      if (a.z) { q[0] = fmaf(f, t[0], q[0]); q[1] = fmaf(f, t[F], q[1]); }
+      if (a.dh) { q[2] += t[2 * (int64_t)F]; q[3] += t[3 * (int64_t)F]; }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) s[j][rl][cl] = q[j];
+  __syncthreads();
+  if (rl || c >= F) return;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    q[j] = 0.f;
+    for (int r = 0; r < 16; ++r) q[j] += s[j][r][cl];
+  }
+  const float sc = a.scale ? a.scale[c] : 1.f, w = a.w ? a.w[c] : 1.f, b = a.b ? a.b[c] : 0.f;
+  if (p.dscale) p.dscale[c] = fmaf(w, q[0], b * q[1]);
+  if (p.dw) p.dw[c] = sc * q[0];
+  if (p.db) p.db[c] = sc * q[1];
+  if (p.dw2) p.dw2[c] = q[2];
+  if (p.db2) p.db2[c] = q[3];
+}
+
+// dg[graph] = a'(g) s (w sum D zh + b sum D): one thread per graph and column
+__global__ __launch_bounds__(256) void norm_graph_gate_kernel(NormArgs a) {
+  const int F = a.d.F, g = blockIdx.x, c = blockIdx.y * 256 + threadIdx.x;
+  if (c >= F) return;
+  const int all = a.row_off[g + 1] - a.row_off[g];
+  float q1 = 0.f, q2 = 0.f;
+  for (int sp = 0; sp * kGraphRows < all; ++sp) {
+    const float* t = a.part + ((int64_t)g * a.splits + sp) * 4 * F + c;
+    q1 += t[0];
+    q2 += t[F];
+  }
+  const bool bf = a.d.z_dtype == AGCN_DTYPE_BF16;
+  const int64_t at = (int64_t)g * a.d.ldg + c;
+  const float gv = bf ? __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(a.gate)[at] << 16) : static_cast<const float*>(a.gate)[at];
+  const float da = gate_slope(a.d.gate_activation, gv);
+  const float sc = a.scale ? a.scale[c] : 1.f, w = a.w ? a.w[c] : 1.f, b = a.b ? a.b[c] : 0.f;
+  const float o = da * sc * fmaf(w, q1, b * q2);
+  if (bf) reinterpret_cast<uint16_t*>(a.dgate)[(int64_t)g * F + c] = (uint16_t)pk_bf(o, 0.f);
+  else static_cast<float*>(a.dgate)[(int64_t)g * F + c] = o;
+}
+
+// ---- host side ---------------------------------------------------------------------------------------------------
+
+// lanes per row and vectors per lane for a width: the fewest lanes that hold the row in one vector each, then two
+struct Shape { int L, NV; };
+Shape shape_for(int F) {
+  const int vecs = (F + V - 1) / V;
+  if (vecs <= 8) return {8, 1};
+  if (vecs <= 16) return {16, 1};
+  if (vecs <= 32) return {32, 1};
+  if (vecs <= 64) return {64, 1};
+  if (vecs <= 128) return {64, 2};
+  if (vecs <= 256) return {256, 1};
+  if (vecs <= 512) return {256, 2};
+  if (vecs <= 1024) return {512, 2};
+  return {1024, 2};
+}
+
+template <typename TX, typename TZ, int L, int NV>
+void launch_one(bool back, const NormArgs& a, int grid, hipStream_t s) {
+  if (back) hipLaunchKernelGGL((norm_backward_kernel<TX, TZ, L, NV>), dim3(grid), dim3(threads_of<L>()), 0, s, a);
+  else hipLaunchKernelGGL((norm_forward_kernel<TX, TZ, L, NV>), dim3(grid), dim3(threads_of<L>()), 0, s, a);
+}
+template <typename TX, typename TZ>
+void launch_shape(bool back, const NormArgs& a, Shape sh, int grid, hipStream_t s) {
+  if (sh.L == 8) launch_one<TX, TZ, 8, 1>(back, a, grid, s);
+  else if (sh.L == 16) launch_one<TX, TZ, 16, 1>(back, a, grid, s);
+  else if (sh.L == 32) launch_one<TX, TZ, 32, 1>(back, a, grid, s);
+  else if (sh.L == 64 && sh.NV == 1) launch_one<TX, TZ, 64, 1>(back, a, grid, s);
+  else if (sh.L == 64) launch_one<TX, TZ, 64, 2>(back, a, grid, s);
+  else if (sh.L == 256 && sh.NV == 1) launch_one<TX, TZ, 256, 1>(back, a, grid, s);
+  else if (sh.L == 256) launch_one<TX, TZ, 256, 2>(back, a, grid, s);
+  else if (sh.L == 512) launch_one<TX, TZ, 512, 2>(back, a, grid, s);
+  else launch_one<TX, TZ, 1024, 2>(back, a, grid, s);
+}
+void launch(bool back, const NormArgs& a, Shape sh, int grid, hipStream_t s) {
+  if (a.d.x_dtype == AGCN_DTYPE_F32 && a.d.z_dtype == AGCN_DTYPE_F32) launch_shape<float, float>(back, a, sh, grid, s);
+  else if (a.d.x_dtype == AGCN_DTYPE_F32) launch_shape<float, __hip_bfloat16>(back, a, sh, grid, s);
+  else launch_shape<__hip_bfloat16, __hip_bfloat16>(back, a, sh, grid, s);
+}
+
+// workgroups that walk the rows: as many as the rows ask for, up to four (forward) / two (backward) of 256 threads per CU
+int row_grid(const AgcnNormDesc& d, Shape sh, bool back) {
+  const int T = sh.L < 256 ? 256 : sh.L, R = T / sh.L;
+  const int64_t want = (d.rows + R - 1) / R, cap = (int64_t)256 * (T > 256 ? 1024 / T : (back ? 2 : 4));
+  return (int)std::max<int64_t>(1, std::min(want, cap));
+}
+
+int check_norm(const AgcnNormDesc* d, const void* plan_host, const void* plan_dev, NormArgs* a, const char* who) {
+  std::memset(a, 0, sizeof(*a));
+  if (!d) return fail(AGCN_EINVAL, "%s: null descriptor", who);
+  a->d = *d;
+  if (d->rows < 0 || d->rows > 0x7fffffff || d->F < 1 || d->F > 16384)
+    return fail(AGCN_EINVAL, "%s: rows must be in 0..2^31-1 and F in 1..16384 (%lld, %d)", who, (long long)d->rows, d->F);
+  if (d->norm != AGCN_NORM_RMS && d->norm != AGCN_NORM_LAYER) return fail(AGCN_EINVAL, "%s: unknown norm %d", who, d->norm);
+  if (!(d->eps > 0.f)) return fail(AGCN_EINVAL, "%s: eps must be positive", who);
+  if (d->gate < AGCN_GATE_NONE || d->gate > AGCN_GATE_GRAPH) return fail(AGCN_EINVAL, "%s: unknown gate %d", who, d->gate);
+  if (d->gate_activation != AGCN_ACT_LINEAR && d->gate_activation != AGCN_ACT_TANH && d->gate_activation != AGCN_ACT_SIGMOID)
+    return fail(AGCN_EINVAL, "%s: the gate's activation is linear, tanh or sigmoid", who);
+  const bool xf = d->x_dtype == AGCN_DTYPE_F32, zf = d->z_dtype == AGCN_DTYPE_F32;
+  if ((!xf && d->x_dtype != AGCN_DTYPE_BF16) || (!zf && d->z_dtype != AGCN_DTYPE_BF16) || (!xf && zf))
+    return fail(AGCN_EINVAL, "%s: types are f32 / f32, bf16 / bf16, or an f32 residual with a bf16 block", who);
+  if (plan_host) {
+    PlanView host, dev;
+    int rc = plan_view(plan_host, plan_host, &host);
+    if (rc != AGCN_OK) return rc;
+    if (!plan_dev) return fail(AGCN_EINVAL, "%s: null device plan", who);
+    plan_view(plan_host, plan_dev, &dev);
+    if (host.info.rows != d->rows) return fail(AGCN_EINVAL, "%s: %lld rows, but the plan has %d", who, (long long)d->rows, host.info.rows);
+    a->n = dev.n; a->row_off = dev.row_off; a->row_graph = dev.row_graph;
+    a->B = host.info.B;
+    a->pads = host.info.rows != host.info.N1;
+    int32_t most = 0;                       // rows of the largest graph, its pad rows counted
+    for (int32_t g = 0; g < host.info.B; ++g) most = std::max(most, host.row_off[g + 1] - host.row_off[g]);
+    a->splits = (most + kGraphRows - 1) / kGraphRows;
+  } else if (d->gate == AGCN_GATE_GRAPH) {
+    return fail(AGCN_EINVAL, "%s: a gate per graph needs a plan", who);
+  }
+  return AGCN_OK;
+}
+
+int check_inputs(NormArgs* a, const AgcnNormInputs* in, const char* who) {
+  const AgcnNormDesc& d = a->d;
+  if (!in || !in->x) return fail(AGCN_EINVAL, "%s: null tensor", who);
+  if (!in->z && (in->gate || in->scale || in->post_weight || in->post_bias))
+    return fail(AGCN_EINVAL, "%s: gate, scale and post norm need a block output z", who);
+  if (!in->z && !in->pre_weight) return fail(AGCN_EINVAL, "%s: neither a block output z nor a pre norm: nothing to compute", who);
+  if ((in->post_bias && !in->post_weight) || (in->pre_bias && !in->pre_weight)) return fail(AGCN_EINVAL, "%s: a bias without its weight", who);
+  if (d.norm == AGCN_NORM_RMS && (in->post_bias || in->pre_bias)) return fail(AGCN_EINVAL, "%s: the rms norm has no bias", who);
+  if ((d.gate != AGCN_GATE_NONE) != (in->gate != nullptr)) return fail(AGCN_EINVAL, "%s: gate tensor and gate kind do not agree", who);
+  if (d.ldx < d.F || (in->z && d.ldz < d.F) || (in->gate && d.ldg < d.F)) return fail(AGCN_EINVAL, "%s: a leading dimension is smaller than F", who);
+  a->z = in->z; a->x = in->x; a->gate = in->gate; a->scale = in->scale;
+  a->w = in->post_weight; a->b = in->post_bias; a->w2 = in->pre_weight; a->b2 = in->pre_bias;
+  return AGCN_OK;
+}
+
+int back_units(const NormArgs& a) {
+  return a.d.gate == AGCN_GATE_GRAPH ? a.B * a.splits : row_grid(a.d, shape_for(a.d.F), true);
+}
+}  // namespace
+}  // namespace agcn
+
+using namespace agcn;
+
+extern "C" int agcn_norm_gate_residual_forward(const AgcnNormDesc* desc, const void* plan_host, const void* plan_dev,
+                                               const AgcnNormInputs* in, void* y, void* h, float* stats, void* hip_stream) {
+  const char* who = "agcn_norm_gate_residual_forward";
+  NormArgs a;
+  int rc = check_norm(desc, plan_host, plan_dev, &a, who);
+  if (rc != AGCN_OK) return rc;
+  if ((rc = check_inputs(&a, in, who)) != AGCN_OK) return rc;
+  if ((a.z != nullptr) != (y != nullptr) || (a.w2 != nullptr) != (h != nullptr))
+    return fail(AGCN_EINVAL, "%s: y goes with z, h with the pre norm", who);
+  if (a.d.rows == 0) return AGCN_OK;
+  a.y = y; a.h = h; a.stats = stats;
+  hipStream_t s = static_cast<hipStream_t>(hip_stream);
+  const Shape sh = shape_for(a.d.F);
+  launch(false, a, sh, row_grid(a.d, sh, false), s);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return fail(AGCN_EDEVICE, "%s: %s", who, hipGetErrorString(e));
+  return AGCN_OK;
+}
+
+extern "C" size_t agcn_norm_gate_residual_backward_workspace_bytes(const AgcnNormDesc* desc, const void* plan_host) {
+  NormArgs a;
+  if (check_norm(desc, plan_host, plan_host, &a, "agcn_norm_gate_residual_backward_workspace_bytes") != AGCN_OK) return 0;
+  return align256((size_t)back_units(a) * 4 * a.d.F * sizeof(float));
+}
+
+extern "C" int agcn_norm_gate_residual_backward(const AgcnNormDesc* desc, const void* plan_host, const void* plan_dev,
+                                                const AgcnNormInputs* in, const float* stats, const void* dy, const void* dh,
+                                                const AgcnNormGrads* grads, void* workspace,
+                                                size_t workspace_bytes, void* hip_stream) {
+  const char* who = "agcn_norm_gate_residual_backward";
+  NormArgs a;
+  int rc = check_norm(desc, plan_host, plan_dev, &a, who);
+  if (rc != AGCN_OK) return rc;
+  if ((rc = check_inputs(&a, in, who)) != AGCN_OK) return rc;
+  if (!grads || !grads->dx || !stats || (a.z && !grads->dz)) return fail(AGCN_EINVAL, "%s: null tensor", who);
+  if ((grads->dgate != nullptr) != (a.gate != nullptr) || (grads->dscale && !a.scale) || (grads->dpost_weight && !a.w) ||
+      (grads->dpost_bias && !a.b) || (grads->dpre_weight && !a.w2) || (grads->dpre_bias && !a.b2) || (dy && !a.z) || (dh && !a.w2))
+    return fail(AGCN_EINVAL, "%s: gradients do not agree with the inputs", who);
+  a.units = back_units(a);
+  const size_t need = (size_t)a.units * 4 * a.d.F * sizeof(float);
+  if (!workspace || workspace_bytes < need) return fail(AGCN_ENOSPACE, "%s: workspace too small (%zu < %zu)", who, workspace_bytes, need);
+  a.stats = const_cast<float*>(stats); a.dy = dy; a.dh = dh;
+  a.dz = grads->dz; a.dx = grads->dx; a.dgate = grads->dgate; a.part = static_cast<float*>(workspace);
+  hipStream_t s = static_cast<hipStream_t>(hip_stream);
+  // (no rows: the one workgroup of the grid leaves zero sums, and the parameters' gradients come out zero)
+  launch(true, a, shape_for(a.d.F), a.units, s);
+  ReduceArgs p;
+  std::memset(&p, 0, sizeof(p));
+  p.a = a;
+  p.dscale = grads->dscale; p.dw = grads->dpost_weight; p.db = grads->dpost_bias;
+  p.dw2 = grads->dpre_weight; p.db2 = grads->dpre_bias;
+  if (p.dscale || p.dw || p.db || p.dw2 || p.db2)
+    hipLaunchKernelGGL(norm_params_kernel, dim3((a.d.F + 63) / 64), dim3(1024), 0, s, p);
+  if (a.d.gate == AGCN_GATE_GRAPH)
+    hipLaunchKernelGGL(norm_graph_gate_kernel, dim3(a.B, (a.d.F + 255) / 256), dim3(256), 0, s, a);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return fail(AGCN_EDEVICE, "%s: %s", who, hipGetErrorString(e));
+  return AGCN_OK;
+}

@@ -8,9 +8,13 @@ Consequence for callers: anything that divides by the batch size -- `MultitaskHe
 loss scale -- must be given the GLOBAL batch size (per-rank graphs x world size) on every rank; the SGC layers
 themselves are built with the LOCAL graph count (it is the length of their output lists).  `global_batch_size()`
 returns the number to use."""
+import ctypes as C
+
 import numpy as np
 import torch
 import torch.distributed as dist
+
+from . import _ffi
 
 
 def graph_cost(n, Fin, Fout, K):
@@ -83,6 +87,77 @@ def flatten_grads(tensors):
     return flat, views
 
 
+_CLIP_DT = {torch.float32: 0, torch.bfloat16: 1}
+
+
+def _clip(tensors, clip_norm, out):
+    lib = _ffi.lib()
+    dev = tensors[0].device
+    if dev.type != "cuda":
+        raise _ffi.AgcnError("gradients must live on the GPU: the clipping kernels have no CPU fallback")
+    if any(t.device != dev for t in tensors):
+        raise ValueError("all gradients must be on one device")
+    n = len(tensors)
+    try:
+        dtype = (C.c_int32 * n)(*[_CLIP_DT[t.dtype] for t in tensors])
+    except KeyError:
+        raise TypeError("gradients must be float32 or bfloat16")
+    numel = (C.c_int64 * n)(*[t.numel() for t in tensors])
+    ptr_in = (C.c_void_p * n)(*[t.data_ptr() for t in tensors])
+    ptr_out = None if out is None else (C.c_void_p * n)(*[t.data_ptr() for t in out])
+    with torch.cuda.device(dev):
+        norm = torch.empty((), dtype=torch.float32, device=dev)
+        wbytes = lib.agcn_clip_workspace_bytes(n, numel, dtype)
+        ws = torch.empty(wbytes, dtype=torch.uint8, device=dev)
+        _ffi.check(lib.agcn_clip_by_global_norm(n, ptr_in, ptr_out, numel, dtype, clip_norm, norm.data_ptr(), ws.data_ptr(),
+                                                wbytes, torch.cuda.current_stream(dev).cuda_stream))
+    return norm
+
+
+def global_norm(tensors):
+    """sqrt of the sum of squares over every element of every tensor (float32 or bfloat16, one device; None entries are
+    skipped): a 0-dim device tensor, no synchronisation."""
+    ts = [t.contiguous() for t in tensors if t is not None]
+    if not ts:
+        raise ValueError("no tensors")
+    return _clip(ts, 1.0, None)
+
+
+def clip_by_global_norm(tensors, clip_norm, out=None):
+    """Scales a list of gradient tensors (float32 or bfloat16, one device) so that their global norm is at most `clip_norm`:
+    out_t = t * clip_norm / max(norm, clip_norm).  Returns (list of clipped tensors, norm before clipping as a 0-dim device tensor);
+    nothing synchronises.  None entries stay None.  A norm that is not finite makes every result NaN (the reference's framework
+    does the same: a broken step is seen, not applied).  out: contiguous tensors of the same shapes and types to write to;
+    `out=tensors` clips in place."""
+    tensors = list(tensors)
+    clip_norm = float(clip_norm)
+    if not clip_norm > 0.0:
+        raise ValueError("clip_norm must be positive")
+    at = [i for i, t in enumerate(tensors) if t is not None]
+    if not at:
+        raise ValueError("no tensors")
+    given = [tensors[i] for i in at]
+    ts = [t if t.is_contiguous() else t.contiguous() for t in given]
+    if out is None:
+        os_ = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in ts]
+    else:
+        out = list(out)
+        if len(out) != len(tensors):
+            raise ValueError("out must hold one tensor per gradient (%d), got %d" % (len(tensors), len(out)))
+        os_ = [out[i] for i in at]
+        for t, o in zip(ts, os_):
+            if o is None or o.shape != t.shape or o.dtype != t.dtype or o.device != t.device or not o.is_contiguous():
+                raise ValueError("out must hold contiguous tensors of the gradients' shapes, types and device")
+    norm = _clip(ts, clip_norm, os_)
+    if out is not None:
+        for o in os_:
+            torch.autograd.graph.increment_version(o)      # (written behind torch's back: a saved copy of it is stale)
+    res = list(tensors)
+    for i, o in zip(at, os_):
+        res[i] = o
+    return res, norm
+
+
 class GradBucket(object):
     """ONE flat fp32 bucket behind the `.grad` fields of a list of parameters -- every SGC layer's [weight | bias | M_L | alpha
     (| beta)], the dense tail, the task heads (140 821 floats = 563 KB for SimpleAGCN + DenseMol + 12 heads) -- so
@@ -126,6 +201,11 @@ class GradBucket(object):
 
     def all_reduce(self, group=None):
         return allreduce_bucket(self.flat, group)
+
+    def clip(self, clip_norm):
+        """Clips the whole bucket by its global norm, in place (after `all_reduce`: the norm of the SUMMED gradients, the same on
+        every rank, without another collective).  Returns the norm before clipping (a 0-dim device tensor: no synchronisation)."""
+        return clip_by_global_norm([self.flat], clip_norm, out=[self.flat])[1]
 
     def nbytes(self):
         return self.flat.numel() * 4

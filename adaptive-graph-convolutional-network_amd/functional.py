@@ -741,3 +741,145 @@ class GraphPoolFunction(torch.autograd.Function):
         _ffi.check(lib.agcn_graph_pool_backward(plan.host_ptr, plan.dev_ptr, C.byref(gb), argmax.data_ptr(),
                                                 dOut.data_ptr(), ctx.F, ctx.F, dX.data_ptr(), _stream(dOut.device)))
         return dX, None, None
+
+
+def _rows_ptr(t):
+    """Data pointer of a row matrix; torch gives an EMPTY tensor the null pointer, which the library reads as "no such tensor"
+    (the kernels touch no row of it)."""
+    return None if t is None else (t.data_ptr() or 256)
+
+
+def _row_matrix(t, what, F=None):
+    """`t` as a [rows, F] matrix of f32 or bf16 whose rows are contiguous (any leading dimension)."""
+    _require_gpu(t, what)
+    if t.dtype not in _DT:
+        raise TypeError("%s must be float32 or bfloat16" % what)
+    if t.dim() != 2 or t.shape[1] < 1 or (F is not None and t.shape[1] != F):
+        raise ValueError("%s must be [rows, %s], got %s" % (what, "F" if F is None else F, tuple(t.shape)))
+    if t.stride(1) != 1 or t.stride(0) < t.shape[1]:
+        return t.contiguous()
+    return t
+
+
+def _ld(t):
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _vector(t, what, F, device):
+    if t is None:
+        return None
+    _require_gpu(t, what)
+    t = _f32c(t, what)
+    if tuple(t.shape) != (F,):
+        raise ValueError("%s must be [%d], got %s" % (what, F, tuple(t.shape)))
+    if t.device != device:
+        raise ValueError("%s is on %s, the rows are on %s" % (what, t.device, device))
+    return t
+
+
+class NormGateResidualFunction(torch.autograd.Function):
+    """(y, h) = (x + scale * a(gate) * N(z), N'(y)); see norm_gate_residual."""
+
+    @staticmethod
+    @_on_tensor_device
+    def forward(ctx, z, x, gate, scale, post_weight, post_bias, pre_weight, pre_bias, plan, norm, eps, gate_activation):
+        lib = _ffi.lib()
+        x = _row_matrix(x, "residual rows")
+        rows, F = x.shape
+        dev = x.device
+        for t, what in ((z, "block output"), (gate, "gate")):
+            if t is not None and t.device != dev:
+                raise ValueError("%s is on %s, the rows are on %s" % (what, t.device, dev))
+        if plan is not None:
+            if plan.dev is None or plan.dev.device != dev:
+                raise ValueError("the plan is not on the rows' device")
+            if plan.rows != rows:
+                raise ValueError("the rows are %d, the plan has %d" % (rows, plan.rows))
+        kind = 0
+        if z is not None:
+            z = _row_matrix(z, "block output", F)
+            if z.shape[0] != rows:
+                raise ValueError("block output and residual rows differ in length (%d, %d)" % (z.shape[0], rows))
+            if x.dtype == torch.bfloat16 and z.dtype != torch.bfloat16:
+                raise TypeError("bfloat16 residual rows need a bfloat16 block output")
+        if gate is not None:
+            if z is None:
+                raise ValueError("a gate needs a block output")
+            if gate.dtype != z.dtype:
+                raise TypeError("gate and block output must have one type")
+            gate = _row_matrix(gate, "gate", F)
+            if plan is not None and gate.shape[0] == plan.B:
+                kind = 2
+            elif gate.shape[0] == rows:
+                kind = 1
+            else:
+                raise ValueError("gate must have one row per row (%d)%s, got %d" %
+                                 (rows, "" if plan is None else " or one per graph (%d)" % plan.B, gate.shape[0]))
+        scale = _vector(scale, "scale", F, dev)
+        post_weight, post_bias = _vector(post_weight, "post_weight", F, dev), _vector(post_bias, "post_bias", F, dev)
+        pre_weight, pre_bias = _vector(pre_weight, "pre_weight", F, dev), _vector(pre_bias, "pre_bias", F, dev)
+        zt = x.dtype if z is None else z.dtype
+        desc = _ffi.NormDesc(rows, F, _ffi.NORM[norm], kind, _ffi.GATE_ACT[gate_activation], _DT[x.dtype], _DT[zt], _ld(x),
+                             0 if z is None else _ld(z), 0 if gate is None else _ld(gate), eps)
+        inputs = _ffi.NormInputs(_rows_ptr(z), _rows_ptr(x), _rows_ptr(gate), _ptr(scale), _ptr(post_weight), _ptr(post_bias),
+                                 _ptr(pre_weight), _ptr(pre_bias))
+        y = torch.empty((rows, F), dtype=x.dtype, device=dev) if z is not None else None
+        h = torch.empty((rows, F), dtype=zt, device=dev) if pre_weight is not None else None
+        stats = torch.empty((rows, 4), dtype=torch.float32, device=dev) if any(ctx.needs_input_grad) else None
+        _ffi.check(lib.agcn_norm_gate_residual_forward(
+            C.byref(desc), None if plan is None else plan.host_ptr, None if plan is None else plan.dev_ptr, C.byref(inputs),
+            _rows_ptr(y), _rows_ptr(h), _ptr(stats), _stream(dev)))
+        ctx.desc, ctx.plan = desc, plan
+        ctx.save_for_backward(z, x, gate, scale, post_weight, post_bias, pre_weight, pre_bias, stats)
+        ctx.set_materialize_grads(False)
+        return y, h
+
+    @staticmethod
+    @_on_tensor_device
+    def backward(ctx, dy, dh):
+        lib = _ffi.lib()
+        z, x, gate, scale, post_weight, post_bias, pre_weight, pre_bias, stats = ctx.saved_tensors
+        desc, plan, dev = ctx.desc, ctx.plan, stats.device
+        rows, F = desc.rows, desc.F
+        if dy is None and dh is None:
+            return (None,) * 12
+        dy = None if dy is None else dy.contiguous()
+        dh = None if dh is None else dh.contiguous()
+        xt, zt = (torch.bfloat16 if d else torch.float32 for d in (desc.x_dtype, desc.z_dtype))
+        dx = torch.empty((rows, F), dtype=xt, device=dev)
+        dz = None if z is None else torch.empty((rows, F), dtype=zt, device=dev)
+        dgate = None if gate is None else torch.empty(tuple(gate.shape), dtype=zt, device=dev)
+        params = [None if p is None else torch.empty_like(p) for p in (scale, post_weight, post_bias, pre_weight, pre_bias)]
+        inputs = _ffi.NormInputs(_rows_ptr(z), _rows_ptr(x), _rows_ptr(gate), _ptr(scale), _ptr(post_weight),
+                                 _ptr(post_bias), _ptr(pre_weight), _ptr(pre_bias))
+        grads = _ffi.NormGrads(_rows_ptr(dz), _rows_ptr(dx), _rows_ptr(dgate), *[_ptr(p) for p in params])
+        host, devp = (None, None) if plan is None else (plan.host_ptr, plan.dev_ptr)
+        wbytes = lib.agcn_norm_gate_residual_backward_workspace_bytes(C.byref(desc), host)
+        ws = torch.empty(wbytes, dtype=torch.uint8, device=dev)
+        _ffi.check(lib.agcn_norm_gate_residual_backward(
+            C.byref(desc), host, devp, C.byref(inputs), _rows_ptr(stats), _rows_ptr(dy), _rows_ptr(dh),
+            C.byref(grads), ws.data_ptr(), wbytes, _stream(dev)))
+        dscale, dpw, dpb, dqw, dqb = params
+        return dz, dx, dgate, dscale, dpw, dpb, dqw, dqb, None, None, None, None
+
+
+def norm_gate_residual(z, x, post_weight=None, post_bias=None, gate=None, scale=None, pre_weight=None, pre_bias=None, norm="rms",
+                       eps=1e-6, gate_activation="linear", plan=None):
+    """The frame of a residual block in one pass over the node rows:
+
+        u = N(z; post_weight, post_bias)            z [rows, F]: the block's output (no post_weight: u = z)
+        y = x + scale * a(gate) * u                 x [rows, F]: the residual rows
+        h = N(y; pre_weight, pre_bias)              what the next block reads (no pre_weight: h is None)
+
+    norm: 'rms' (no biases) or 'layer'.  gate: [rows, F], or [B, F] with `plan` (a Plan or GraphBatch): one vector per graph;
+    gate_activation: 'linear', 'tanh' or 'sigmoid'.  Rows are float32, bfloat16, or float32 x with bfloat16 z (h and gate have
+    z's type); the vectors are float32.  z=None: h = N(x) alone.  With `plan`, pad rows come out zero.  Returns (y, h)."""
+    if norm not in _ffi.NORM:
+        raise ValueError("norm must be 'rms' or 'layer'")
+    if gate_activation not in _ffi.GATE_ACT:
+        raise ValueError("gate_activation must be 'linear', 'tanh' or 'sigmoid'")
+    if x is None or not torch.is_tensor(x):
+        raise TypeError("residual rows must be a tensor")
+    plan = getattr(plan, "plan", plan)
+    return NormGateResidualFunction.apply(z, x, gate, scale, post_weight, post_bias, pre_weight, pre_bias, plan, norm, float(eps),
+                                          gate_activation)

@@ -72,6 +72,9 @@ enum { AGCN_MODE_REFERENCE = 0, AGCN_MODE_PAPER = 1 };
 enum { AGCN_SGC_LL = 0, AGCN_SGC_LL_RESLAP = 1 };
 /* activations.get(): the networks only use these */
 enum { AGCN_ACT_LINEAR = 0, AGCN_ACT_RELU = 1, AGCN_ACT_TANH = 2 };
+/* ... and what the gates of the operators without a reference counterpart take (agcn_norm_gate_residual_*: LINEAR, TANH,
+ * SIGMOID; agcn_gated_ffn_*: RELU, SIGMOID, SILU, GELU -- the erf form) */
+enum { AGCN_ACT_SIGMOID = 3, AGCN_ACT_SILU = 4, AGCN_ACT_GELU = 5 };
 
 /* ------------------------------------------------------------------------
  * Plan: the integer bookkeeping of one ragged batch (graph sizes, row and
@@ -409,6 +412,56 @@ AGCN_API int agcn_graph_pool_backward(const void* plan_host, const void* plan_de
 #define AGCN_DTYPE_BF16 1
 AGCN_API int agcn_cast_rows(const void* src, int32_t src_dtype, void* dst, int32_t dst_dtype, int64_t rows, int32_t cols,
                    int32_t ld_src, int32_t ld_dst, void* hip_stream);
+
+/* ---- the frame of a residual block: norms before and after it, its gate and residual scale ----------
+ * Beside BlockEnd (models/layers/blockend.py:67-86, act(x + x_res . W)); no reference counterpart.
+ *   u = N(z; post_weight, post_bias)      the block's output z, normalised     (no post norm: u = z)
+ *   y = x + scale (.) a(gate) (.) u       the new residual rows                (no scale / gate: 1)
+ *   h = N(y; pre_weight, pre_bias)        what the next block reads            (no pre norm: no h)
+ *   N: RMS  v / sqrt(mean v^2 + eps) * w;   LAYER  (v - mean v) / sqrt(var v + eps) * w + b   over the F features of a row
+ * z == NULL: h = N(x) alone (the first norm of a network; y, post norm, gate and scale must be NULL then).
+ * Types: x, y, dx in x_dtype; z, h, gate, dz, dh, dgate in z_dtype (f32 / f32, bf16 / bf16, or f32 rows with bf16 blocks);
+ * parameters and their gradients fp32.  A gate is [rows, ldg] (ROW) or [B, ldg], one vector per graph of the plan (GRAPH).
+ * y, h, dy, dh, dz, dx, dgate are contiguous (leading dimension F).  Pad rows of the plan (nullable: none) come out zero, in
+ * the gradients too, and take part in no sum.  stats [rows, 4] fp32 (nullable: no backward will follow) goes to the backward.
+ * Backward: dy or dh may be NULL (that output was not used); the parameter gradients are nullable. Fixed-order sums. */
+enum { AGCN_NORM_RMS = 0, AGCN_NORM_LAYER = 1 };
+enum { AGCN_GATE_NONE = 0, AGCN_GATE_ROW = 1, AGCN_GATE_GRAPH = 2 };
+typedef struct AgcnNormDesc {
+  int64_t rows;
+  int32_t F;               /* 1 .. 16384 */
+  int32_t norm;            /* AGCN_NORM_* */
+  int32_t gate;            /* AGCN_GATE_* */
+  int32_t gate_activation; /* AGCN_ACT_LINEAR | TANH | SIGMOID */
+  int32_t x_dtype, z_dtype;
+  int32_t ldx, ldz, ldg;   /* leading dimensions of the inputs, in elements */
+  float eps;
+} AgcnNormDesc;
+typedef struct AgcnNormInputs {
+  const void *z, *x, *gate;
+  const float *scale, *post_weight, *post_bias, *pre_weight, *pre_bias; /* [F] each */
+} AgcnNormInputs;
+typedef struct AgcnNormGrads {
+  void *dz, *dx, *dgate;
+  float *dscale, *dpost_weight, *dpost_bias, *dpre_weight, *dpre_bias;
+} AgcnNormGrads;
+AGCN_API int agcn_norm_gate_residual_forward(const AgcnNormDesc* desc, const void* plan_host, const void* plan_dev,
+                                    const AgcnNormInputs* in, void* y, void* h, float* stats, void* hip_stream);
+AGCN_API size_t agcn_norm_gate_residual_backward_workspace_bytes(const AgcnNormDesc* desc, const void* plan_host);
+AGCN_API int agcn_norm_gate_residual_backward(const AgcnNormDesc* desc, const void* plan_host, const void* plan_dev,
+                                     const AgcnNormInputs* in, const float* stats, const void* dy, const void* dh,
+                                     const AgcnNormGrads* grads, void* workspace, size_t workspace_bytes, void* hip_stream);
+
+/* ---- clipping by the global norm of many gradient tensors --------------------------------------------
+ * norm[0] = sqrt(sum over all tensors of the squares), out[t] = in[t] * clip_norm / max(norm, clip_norm); a norm that is not
+ * finite makes every output NaN (the semantics of the reference's framework).  in / out / numel / dtype: HOST tables of
+ * n_tensors entries (device pointers, element counts, AGCN_DTYPE_*); out[t] == in[t] clips in place, any other overlap of an
+ * output with an input or an output is refused; out == NULL: the norm alone.  Squares are added in 64 bits, in a fixed order.
+ * norm: DEVICE float.  workspace: agcn_clip_workspace_bytes of the same table. */
+AGCN_API size_t agcn_clip_workspace_bytes(int32_t n_tensors, const int64_t* numel, const int32_t* dtype);
+AGCN_API int agcn_clip_by_global_norm(int32_t n_tensors, const void* const* in, void* const* out, const int64_t* numel,
+                             const int32_t* dtype, float clip_norm, float* norm, void* workspace, size_t workspace_bytes,
+                             void* hip_stream);
 
 /* Row layout conversion between the reference's padded feed and packed rows.  The reference hands every layer
  * lists of B [max_atom, F] tensors (graph_topology.py:84-91) and slices the real rows off again inside the layer
