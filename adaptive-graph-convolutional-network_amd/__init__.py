@@ -15,7 +15,7 @@ from .store import GraphStore, ResidentStore  # noqa: F401
 from .engine import GraphedStep, SgcLLEpochLanes, SgcLLEpochPipeline, SgcLLEpochStep, SgcLLStep  # noqa: F401
 from .functional import (check_device_status, capture_scope, release_reserve_pool, reserve_pool_bytes,  # noqa: F401
                          dispatch, run_checked, device_timeouts, recovered_calls, param_grad_fork, no_member_flags,
-                         norm_gate_residual)
+                         norm_gate_residual, gated_ffn)
 from . import dist  # noqa: F401
 from .dist import clip_by_global_norm, global_norm  # noqa: F401
 

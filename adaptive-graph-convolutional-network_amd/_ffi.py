@@ -55,6 +55,11 @@ class DenseDesc(C.Structure):
                 ("ldx", C.c_int32), ("ldy", C.c_int32), ("ldadd", C.c_int32), ("flags", C.c_uint32)]
 
 
+class FfnDesc(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("Fin", C.c_int32), ("H", C.c_int32), ("Fout", C.c_int32), ("activation", C.c_int32),
+                ("dtype", C.c_int32), ("ldx", C.c_int32), ("training", C.c_int32), ("reserved", C.c_int32)]
+
+
 class NormDesc(C.Structure):
     _fields_ = [("rows", C.c_int64), ("F", C.c_int32), ("norm", C.c_int32), ("gate", C.c_int32), ("gate_activation", C.c_int32),
                 ("x_dtype", C.c_int32), ("z_dtype", C.c_int32), ("ldx", C.c_int32), ("ldz", C.c_int32), ("ldg", C.c_int32),
@@ -141,6 +146,8 @@ SYMBOLS = [
     "agcn_rows_dense_scaled_forward_ws",
     "agcn_multitask_ce_workspace_bytes", "agcn_multitask_ce_forward", "agcn_multitask_ce_backward",
     "agcn_graph_pool_forward", "agcn_graph_pool_backward",
+    "agcn_gated_ffn_reserve_bytes", "agcn_gated_ffn_forward_workspace_bytes", "agcn_gated_ffn_backward_workspace_bytes",
+    "agcn_gated_ffn_forward", "agcn_gated_ffn_backward",
     "agcn_norm_gate_residual_forward", "agcn_norm_gate_residual_backward_workspace_bytes", "agcn_norm_gate_residual_backward",
     "agcn_clip_workspace_bytes", "agcn_clip_by_global_norm",
     "agcn_store_batch_sizes", "agcn_store_pack_batch", "agcn_store_stage_bytes", "agcn_store_stage_batch",
@@ -204,6 +211,14 @@ def _declare(lib):
     lib.agcn_multitask_ce_forward.argtypes = [I32, I32, I32, P, I32, P, P, P, P, C.c_float, P, P, P, SZ, P]
     lib.agcn_multitask_ce_backward.restype = C.c_int
     lib.agcn_multitask_ce_backward.argtypes = [I32, I32, I32, P, I32, P, P, P, P, C.c_float, P, P, P, P, P, SZ, P]
+    for name in ("agcn_gated_ffn_reserve_bytes", "agcn_gated_ffn_forward_workspace_bytes", "agcn_gated_ffn_backward_workspace_bytes"):
+        f = getattr(lib, name)
+        f.restype = SZ
+        f.argtypes = [C.POINTER(FfnDesc)]
+    lib.agcn_gated_ffn_forward.restype = C.c_int
+    lib.agcn_gated_ffn_forward.argtypes = [C.POINTER(FfnDesc), P, P, P, P, P, P, SZ, P, SZ, P]
+    lib.agcn_gated_ffn_backward.restype = C.c_int
+    lib.agcn_gated_ffn_backward.argtypes = [C.POINTER(FfnDesc), P, P, P, P, P, P, P, P, P, P, SZ, P, SZ, P]
     lib.agcn_norm_gate_residual_forward.restype = C.c_int
     lib.agcn_norm_gate_residual_forward.argtypes = [C.POINTER(NormDesc), P, P, C.POINTER(NormInputs), P, P, P, P]
     lib.agcn_norm_gate_residual_backward_workspace_bytes.restype = SZ

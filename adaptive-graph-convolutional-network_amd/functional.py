@@ -883,3 +883,70 @@ def norm_gate_residual(z, x, post_weight=None, post_bias=None, gate=None, scale=
     plan = getattr(plan, "plan", plan)
     return NormGateResidualFunction.apply(z, x, gate, scale, post_weight, post_bias, pre_weight, pre_bias, plan, norm, float(eps),
                                           gate_activation)
+
+
+class GatedFfnFunction(torch.autograd.Function):
+    """Y = (act(X Wg) * (X Wu)) Wd; see gated_ffn."""
+
+    @staticmethod
+    @_on_tensor_device
+    def forward(ctx, X, Wg, Wu, Wd, activation):
+        lib = _ffi.lib()
+        X = _row_matrix(X, "node features")
+        rows, Fin = X.shape
+        dev = X.device
+        Ws = []
+        for W, what in ((Wg, "w_gate"), (Wu, "w_up"), (Wd, "w_down")):
+            _require_gpu(W, what)
+            if W.dtype != X.dtype:
+                raise TypeError("%s is %s, the node features are %s" % (what, W.dtype, X.dtype))
+            if W.dim() != 2 or W.device != dev:
+                raise ValueError("%s must be a matrix on %s" % (what, dev))
+            Ws.append(W if W.is_contiguous() else W.contiguous())
+        Wg, Wu, Wd = Ws
+        H = Wg.shape[1]
+        if tuple(Wg.shape) != (Fin, H) or tuple(Wu.shape) != (Fin, H) or Wd.shape[0] != H:
+            raise ValueError("w_gate and w_up must be [%d, H] and w_down [H, F_out], got %s, %s, %s" %
+                             (Fin, tuple(Wg.shape), tuple(Wu.shape), tuple(Wd.shape)))
+        Fout = Wd.shape[1]
+        training = any(ctx.needs_input_grad)
+        desc = _ffi.FfnDesc(rows, Fin, H, Fout, _ffi.FFN_ACT[activation], _DT[X.dtype], _ld(X), 1 if training else 0, 0)
+        rbytes, wbytes = lib.agcn_gated_ffn_reserve_bytes(C.byref(desc)), lib.agcn_gated_ffn_forward_workspace_bytes(C.byref(desc))
+        if not rbytes:
+            _ffi.check(-1)
+        reserve = torch.empty(rbytes, dtype=torch.uint8, device=dev)
+        ws = torch.empty(wbytes, dtype=torch.uint8, device=dev)
+        Y = torch.empty((rows, Fout), dtype=X.dtype, device=dev)
+        _ffi.check(lib.agcn_gated_ffn_forward(C.byref(desc), X.data_ptr(), Wg.data_ptr(), Wu.data_ptr(), Wd.data_ptr(), Y.data_ptr(),
+                                              reserve.data_ptr(), rbytes, ws.data_ptr(), wbytes, _stream(dev)))
+        if training:
+            ctx.desc = desc
+            ctx.save_for_backward(X, Wg, Wu, Wd, reserve)
+        return Y
+
+    @staticmethod
+    @_on_tensor_device
+    def backward(ctx, dY):
+        lib = _ffi.lib()
+        X, Wg, Wu, Wd, reserve = ctx.saved_tensors
+        desc, dev = ctx.desc, X.device
+        dY = dY.contiguous()
+        need = ctx.needs_input_grad
+        dX = torch.empty((desc.rows, desc.Fin), dtype=X.dtype, device=dev) if need[0] else None
+        dWg, dWu = (torch.empty_like(Wg), torch.empty_like(Wu)) if need[1] or need[2] else (None, None)
+        dWd = torch.empty_like(Wd) if need[3] else None
+        wbytes = lib.agcn_gated_ffn_backward_workspace_bytes(C.byref(desc))
+        ws = torch.empty(wbytes, dtype=torch.uint8, device=dev)
+        _ffi.check(lib.agcn_gated_ffn_backward(C.byref(desc), X.data_ptr(), Wg.data_ptr(), Wu.data_ptr(), Wd.data_ptr(), dY.data_ptr(),
+                                               _ptr(dX), _ptr(dWg), _ptr(dWu), _ptr(dWd), reserve.data_ptr(), reserve.numel(),
+                                               ws.data_ptr(), wbytes, _stream(dev)))
+        return dX, dWg if need[1] else None, dWu if need[2] else None, dWd, None
+
+
+def gated_ffn(X, w_gate, w_up, w_down, activation="silu"):
+    """Gated feed-forward block over node rows: (act(X w_gate) * (X w_up)) w_down.  X [rows, F], w_gate and w_up [F, H], w_down
+    [H, F_out], all float32 or all bfloat16; activation: 'silu', 'gelu' (the erf form), 'relu' or 'sigmoid'.  Every row is a
+    row of its own: pad rows that are zero come out zero."""
+    if activation not in _ffi.FFN_ACT:
+        raise ValueError("activation must be one of %s" % ", ".join(sorted(_ffi.FFN_ACT)))
+    return GatedFfnFunction.apply(X, w_gate, w_up, w_down, activation)

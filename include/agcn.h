@@ -413,6 +413,33 @@ AGCN_API int agcn_graph_pool_backward(const void* plan_host, const void* plan_de
 AGCN_API int agcn_cast_rows(const void* src, int32_t src_dtype, void* dst, int32_t dst_dtype, int64_t rows, int32_t cols,
                    int32_t ld_src, int32_t ld_dst, void* hip_stream);
 
+/* ---- gated feed-forward block over node rows -----------------------------------------------------------
+ * Beside DenseMol (models/layers/dense_layer.py:33-50); no reference counterpart.
+ *   Y = (act(X Wg) (.) (X Wu)) Wd          X [rows, ldx] (Fin used), Wg, Wu [Fin, H], Wd [H, Fout], Y [rows, Fout]
+ * All matrices are of one type (f32 | bf16).  f32 products run on the bf16 matrix pipe at fp32 accuracy (csrc/bf16_split.h: a row that
+ * holds an infinity or a NaN comes out non-finite, but an infinity may come out as NaN); bf16 calls round the block's inner
+ * matrices to bf16, sums are fp32.  reserve (256-byte aligned, agcn_gated_ffn_reserve_bytes): scratch of the forward; with
+ * training = 1 the backward needs it as the forward left it, and X, Wg, Wu, Wd unchanged at the same addresses.
+ * Backward: dX [rows, Fin], dWg, dWu (together), dWd are each nullable. Fixed-order sums: bit-reproducible.
+ * rows = 0: the forward does nothing, the backward writes zeros. */
+typedef struct AgcnFfnDesc {
+  int64_t rows;
+  int32_t Fin, H, Fout;  /* 1 .. 65536 each */
+  int32_t activation;    /* AGCN_ACT_RELU | SIGMOID | SILU | GELU */
+  int32_t dtype;         /* AGCN_DTYPE_* */
+  int32_t ldx;
+  int32_t training;      /* 1: keep what a backward reads */
+  int32_t reserved;
+} AgcnFfnDesc;
+AGCN_API size_t agcn_gated_ffn_reserve_bytes(const AgcnFfnDesc* desc);
+AGCN_API size_t agcn_gated_ffn_forward_workspace_bytes(const AgcnFfnDesc* desc);
+AGCN_API size_t agcn_gated_ffn_backward_workspace_bytes(const AgcnFfnDesc* desc);
+AGCN_API int agcn_gated_ffn_forward(const AgcnFfnDesc* desc, const void* X, const void* Wg, const void* Wu, const void* Wd, void* Y,
+                           void* reserve, size_t reserve_bytes, void* workspace, size_t workspace_bytes, void* hip_stream);
+AGCN_API int agcn_gated_ffn_backward(const AgcnFfnDesc* desc, const void* X, const void* Wg, const void* Wu, const void* Wd,
+                            const void* dY, void* dX, void* dWg, void* dWu, void* dWd, const void* reserve,
+                            size_t reserve_bytes, void* workspace, size_t workspace_bytes, void* hip_stream);
+
 /* ---- the frame of a residual block: norms before and after it, its gate and residual scale ----------
  * Beside BlockEnd (models/layers/blockend.py:67-86, act(x + x_res . W)); no reference counterpart.
  *   u = N(z; post_weight, post_bias)      the block's output z, normalised     (no post norm: u = z)
