@@ -7,17 +7,20 @@
 //   * Both projections share one pass over X: a workgroup's tile holds the same columns of Wg and Wu, so that the gate and its
 //     partner meet in one lane's registers and the epilogue writes A (and, for a backward, G and U).  dA never reaches memory
 //     either: its epilogue reads G and U and writes dG and dU.  dX is one product over 2 H, dWg and dWu share X's tiles.
-//   * fp32 operands are split exactly into three bf16 pieces (bf16_split.h); a product is then the sum of six piece products
-//     (the dropped ones are below 2^-24), which the kernel runs as six SEGMENTS of one long k loop, small terms first.
-//   * Tiles go from memory to LDS directly (buffer_load .. lds, 16 bytes per lane), two stages.  An operand whose rows run along k
-//     is read back with ds_read_b128, one whose rows run across k (weights in X W, both operands in X^T dG) with the transposing
-//     ds_read_b64_tr_b16: nothing is transposed in memory.  The 16-byte chunks of a tile row are permuted (xor with row bits) so
-//     that the lanes of a read hit different banks; the permutation is in the GLOBAL addresses, the LDS image being linear.
-//     Rows, columns and k beyond the operand read as zeros (the buffer's own bound).
+//   * fp32 operands are split exactly into three bf16 pieces (bf16_split.h), and a product is the sum of six piece products (the
+//     dropped ones are below 2^-24): a stage holds the three planes of both operands, every fragment read serves two of them.
+//   * Tiles go from memory to LDS directly (buffer_load .. lds, 16 bytes per lane), in two or three stages.  An operand whose rows
+//     run along k is read back with ds_read_b128, one whose rows run across k (weights in X W, both operands in X^T dG) with the
+//     transposing ds_read_b64_tr_b16: nothing is transposed in memory.  The 16-byte chunks of a tile row are permuted (xor with
+//     row bits) so that the lanes of a read hit different banks; the permutation is in the GLOBAL addresses, the LDS image being
+//     linear.  Rows, columns and k beyond the operand read as zeros (the buffer's own bound).
+//   * The accumulators leave through LDS, so that a lane gets eight neighbouring columns of one row: wide loads and stores, and
+//     one small loop of epilogue code instead of one copy per fragment.
 //   * Few tiles for the chip: the k loop is cut into splits whose fp32 tiles a second kernel adds in order (no atomics) and
 //     puts through the same epilogue.
-// Roundings of bf16 calls: G, U, A, dG, dU are stored in bf16 for the products that read them (the matrix pipe takes bf16); sums,
-// activations and their slopes are fp32.
+// Roundings of bf16 calls: A, dG, dU are stored in bf16 for the products that read them (the matrix pipe takes bf16); G and U, which
+// only the element-wise slopes read again, keep 24 bits (sign, exponent, 15 bits of the mantissa: in bf16 they would add as
+// much error to every gradient as dG's own rounding); sums, activations and their slopes are fp32.
 #include <hip/hip_bf16.h>
 #include <hip/hip_runtime.h>
 
@@ -30,31 +33,28 @@ namespace agcn {
 namespace {
 typedef uint32_t u32x4u __attribute__((ext_vector_type(4), aligned(4)));   // at the alignment of an element: unaligned access mode
 typedef uint32_t u32x4h __attribute__((ext_vector_type(4), aligned(2)));
-typedef uint32_t u32x2h __attribute__((ext_vector_type(2), aligned(2)));
 #define AGCN_LDS __attribute__((address_space(3)))
-
-constexpr int BK = 64;               // k of a stage
-constexpr int kMaxSeg = 12;
 
 enum { EPI_GATED = 0, EPI_STORE = 1, EPI_DH = 2 };
 
 struct Seg { const uint16_t *a, *b, *b2; };
 
 struct GemmArgs {
-  Seg seg[kMaxSeg];
+  Seg seg[2];                        // the k loop runs over one or two products of the same sizes
   int32_t nseg;
   int32_t M, N, K;                   // N: columns of one B matrix (two B matrices: of each)
   int32_t lda, ldb;
+  int64_t a_plane, b_plane;          // elements between the planes of pieces
   int32_t ktiles, tiles_m, tiles_n, splits;
   float* part;                       // splits > 1: [split][B matrix][M][ldp] fp32
   int32_t ldp;
   // epilogue
-  int32_t act, f32, planes;
+  int32_t act, f32;
   int32_t ldh;                       // leading dimension of G, U, A, dG, dU
   int64_t plane;                     // elements between the planes of A, dG, dU
   void *out, *out2;                  // EPI_STORE: [M, ldo]
   int32_t ldo;
-  void *g, *u;                       // f32 or bf16
+  void *g, *u;                       // f32, or 24 bits: [M, ldh] upper sixteen, then [M, ldh] lower eight
   uint16_t *hid, *dg, *du;           // bf16 pieces
 };
 
@@ -85,192 +85,255 @@ __device__ __forceinline__ void gate_of(int act, float g, float& a, float& da) {
   }
 }
 
-__device__ __forceinline__ f32x4 load4(const void* p, int64_t at, bool f32) {       // 16- / 8-byte aligned rows of the library's own
-  if (f32) return *reinterpret_cast<const f32x4*>(static_cast<const float*>(p) + at);
-  const u32x2 v = *reinterpret_cast<const u32x2*>(static_cast<const uint16_t*>(p) + at);
-  return (f32x4){__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u)};
+// ---- eight neighbouring values of a row -----------------------------------------------------------------------------
+struct F8 { float v[8]; };
+
+// the library's own matrices: rows at multiples of eight elements
+__device__ __forceinline__ void store8_f32(float* p, const F8& x) {
+  *reinterpret_cast<f32x4*>(p) = (f32x4){x.v[0], x.v[1], x.v[2], x.v[3]};
+  *reinterpret_cast<f32x4*>(p + 4) = (f32x4){x.v[4], x.v[5], x.v[6], x.v[7]};
 }
-__device__ __forceinline__ void store4(void* p, int64_t at, bool f32, f32x4 v) {
-  if (f32) *reinterpret_cast<f32x4*>(static_cast<float*>(p) + at) = v;
-  else *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(p) + at) = (u32x2){pk_bf(v.x, v.y), pk_bf(v.z, v.w)};
+__device__ __forceinline__ F8 load8_f32(const float* p) {
+  const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
+  return {{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
 }
-// the bf16 pieces of four values (planes == 1: the rounded value itself)
-__device__ __forceinline__ void store_pieces(uint16_t* p, int64_t at, int planes, int64_t plane, f32x4 v) {
-  if (planes == 1) {
-    *reinterpret_cast<u32x2*>(p + at) = (u32x2){pk_bf(v.x, v.y), pk_bf(v.z, v.w)};
+__device__ __forceinline__ u32x4 bf8(const F8& x) {
+  return (u32x4){pk_bf(x.v[0], x.v[1]), pk_bf(x.v[2], x.v[3]), pk_bf(x.v[4], x.v[5]), pk_bf(x.v[6], x.v[7])};
+}
+// 24 bits of a float, rounded to nearest (ties away; a carry out of the largest finite value gives infinity), NaN kept
+__device__ __forceinline__ uint32_t top24(float x) {
+  const uint32_t b = __float_as_uint(x);
+  return x != x ? (b >> 8) | 0x4000u : (b + 0x80u) >> 8;
+}
+__device__ __forceinline__ void store8_gate(const GemmArgs& g, void* p, int64_t at, const F8& x) {
+  if (g.f32) {
+    store8_f32(static_cast<float*>(p) + at, x);
   } else {
-    uint32_t h[2], m[2], l[2];
-    split3(v.x, v.y, h[0], m[0], l[0]);
-    split3(v.z, v.w, h[1], m[1], l[1]);
-    *reinterpret_cast<u32x2*>(p + at) = (u32x2){h[0], h[1]};
-    *reinterpret_cast<u32x2*>(p + plane + at) = (u32x2){m[0], m[1]};
-    *reinterpret_cast<u32x2*>(p + 2 * plane + at) = (u32x2){l[0], l[1]};
+    uint32_t t[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = top24(x.v[i]);
+    u32x4 hi;
+    u32x2 lo;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) hi[i] = (t[2 * i] >> 8) | (t[2 * i + 1] >> 8) << 16;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      lo[i] = (t[4 * i] & 255u) | (t[4 * i + 1] & 255u) << 8 | (t[4 * i + 2] & 255u) << 16 | t[4 * i + 3] << 24;
+    *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(p) + at) = hi;
+    *reinterpret_cast<u32x2*>(reinterpret_cast<uint8_t*>(static_cast<uint16_t*>(p) + (int64_t)g.M * g.ldh) + at) = lo;
   }
 }
-// four results of a caller's matrix: any alignment, any tail
-__device__ __forceinline__ void store_out(void* p, int64_t row, int ld, int n, int N, bool f32, f32x4 v) {
-  const int64_t at = row * ld + n;
-  if (f32) {
+__device__ __forceinline__ F8 load8_gate(const GemmArgs& g, const void* p, int64_t at) {
+  if (g.f32) return load8_f32(static_cast<const float*>(p) + at);
+  const u32x4 hi = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(p) + at);
+  const u32x2 lo = *reinterpret_cast<const u32x2*>(reinterpret_cast<const uint8_t*>(static_cast<const uint16_t*>(p) + (int64_t)g.M * g.ldh) + at);
+  F8 x;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t h = i & 1 ? hi[i >> 1] & 0xffff0000u : hi[i >> 1] << 16, l = (lo[i >> 2] >> (8 * (i & 3))) & 255u;
+    x.v[i] = __uint_as_float(h | l << 8);
+  }
+  return x;
+}
+// the bf16 pieces of eight values (bf16 calls: the rounded values themselves)
+__device__ __forceinline__ void store8_pieces(const GemmArgs& g, uint16_t* p, int64_t at, const F8& x) {
+  if (!g.f32) {
+    *reinterpret_cast<u32x4*>(p + at) = bf8(x);
+  } else {
+    u32x4 h, m, l;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t a, b, c;
+      split3(x.v[2 * i], x.v[2 * i + 1], a, b, c);
+      h[i] = a; m[i] = b; l[i] = c;
+    }
+    *reinterpret_cast<u32x4*>(p + at) = h;
+    *reinterpret_cast<u32x4*>(p + g.plane + at) = m;
+    *reinterpret_cast<u32x4*>(p + 2 * g.plane + at) = l;
+  }
+}
+// a caller's matrix: any alignment, any tail
+__device__ __forceinline__ void store8_out(const GemmArgs& g, void* p, int64_t row, int n, const F8& x) {
+  const int64_t at = row * g.ldo + n;
+  if (g.f32) {
     float* o = static_cast<float*>(p) + at;
-    if (n + 4 <= N) {
-      *reinterpret_cast<u32x4u*>(o) = (u32x4u){__float_as_uint(v.x), __float_as_uint(v.y), __float_as_uint(v.z), __float_as_uint(v.w)};
+    if (n + 8 <= g.N) {
+#pragma unroll
+      for (int k = 0; k < 8; k += 4)
+        *reinterpret_cast<u32x4u*>(o + k) = (u32x4u){__float_as_uint(x.v[k]), __float_as_uint(x.v[k + 1]), __float_as_uint(x.v[k + 2]), __float_as_uint(x.v[k + 3])};
     } else {
-      for (int i = 0; i < 4; ++i) if (n + i < N) o[i] = v[i];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) if (n + i < g.N) o[i] = x.v[i];
     }
   } else {
     uint16_t* o = static_cast<uint16_t*>(p) + at;
-    const uint32_t a = pk_bf(v.x, v.y), b = pk_bf(v.z, v.w);
-    if (n + 4 <= N) {
-      *reinterpret_cast<u32x2h*>(o) = (u32x2h){a, b};
+    const u32x4 b = bf8(x);
+    if (n + 8 <= g.N) {
+      *reinterpret_cast<u32x4h*>(o) = (u32x4h){b.x, b.y, b.z, b.w};
     } else {
-      if (n < N) o[0] = (uint16_t)a;
-      if (n + 1 < N) o[1] = (uint16_t)(a >> 16);
-      if (n + 2 < N) o[2] = (uint16_t)b;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) if (n + i < g.N) o[i] = (uint16_t)(b[i >> 1] >> (16 * (i & 1)));
     }
   }
 }
 
-// What becomes of four neighbouring columns n .. n + 3 of row m (v1: of the second B matrix)
+// What becomes of columns n .. n + 7 of row m (v1: of the second B matrix)
 template <int EPI, int NB>
-__device__ __forceinline__ void epilogue(const GemmArgs& g, int m, int n, f32x4 v0, f32x4 v1) {
-  const bool f32 = g.f32 != 0;
+__device__ __forceinline__ void epilogue(const GemmArgs& g, int m, int n, const F8& v0, const F8& v1) {
   if (EPI == EPI_STORE) {
     if (n >= g.N) return;
-    store_out(g.out, m, g.ldo, n, g.N, f32, v0);
-    if (NB == 2) store_out(g.out2, m, g.ldo, n, g.N, f32, v1);
+    store8_out(g, g.out, m, n, v0);
+    if (NB == 2) store8_out(g, g.out2, m, n, v1);
     return;
   }
   // (the library's own matrices are padded to eights: the columns behind H get the zeros that the products read there)
   if (n >= g.ldh) return;
   const int64_t at = (int64_t)m * g.ldh + n;
   if (EPI == EPI_GATED) {
-    f32x4 hv;
+    F8 hv;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 8; ++i) {
       float a, da;
-      gate_of(g.act, v0[i], a, da);
-      hv[i] = n + i < g.N ? a * v1[i] : 0.f;
+      gate_of(g.act, v0.v[i], a, da);
+      hv.v[i] = n + i < g.N ? a * v1.v[i] : 0.f;
     }
     if (g.g) {
-      store4(g.g, at, f32, v0);
-      store4(g.u, at, f32, v1);
+      store8_gate(g, g.g, at, v0);
+      store8_gate(g, g.u, at, v1);
     }
-    store_pieces(g.hid, at, g.planes, g.plane, hv);
+    store8_pieces(g, g.hid, at, hv);
   } else {
-    const f32x4 gv = load4(g.g, at, f32), uv = load4(g.u, at, f32);
-    f32x4 dg, du;
+    const F8 gv = load8_gate(g, g.g, at), uv = load8_gate(g, g.u, at);
+    F8 dg, du;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 8; ++i) {
       float a, da;
-      gate_of(g.act, gv[i], a, da);
-      dg[i] = n + i < g.N ? v0[i] * uv[i] * da : 0.f;
-      du[i] = n + i < g.N ? v0[i] * a : 0.f;
+      gate_of(g.act, gv.v[i], a, da);
+      dg.v[i] = n + i < g.N ? v0.v[i] * uv.v[i] * da : 0.f;
+      du.v[i] = n + i < g.N ? v0.v[i] * a : 0.f;
     }
-    store_pieces(g.dg, at, g.planes, g.plane, dg);
-    store_pieces(g.du, at, g.planes, g.plane, du);
+    store8_pieces(g, g.dg, at, dg);
+    store8_pieces(g, g.du, at, du);
   }
 }
 
 #ifdef __HIP_DEVICE_COMPILE__      // (address spaces and builtins that the host pass does not know)
-// One operand's tile of a stage: ROWS rows of the operand (m or n) by BK.  T (transposed): the operand's matrix is [k][rows].
-template <int ROWS, bool T, int THREADS>
-struct Tile {
-  static constexpr int kSlots = ROWS * BK / 8 / THREADS;       // 16-byte chunks per thread
-  static constexpr int kChunks = ROWS / 8;                     // T: chunks per k row
-  static_assert(ROWS * BK / 8 % THREADS == 0, "whole chunks per thread");
+// The tiles of one operand in a stage: NMAT matrices of P planes, each ROWS rows of the operand (m or n) by BK.  T (transposed): the
+// operand's matrix is [k][rows].  Every wave issues kSlots loads of 64 chunks.
+template <int ROWS, bool T, int BK, int P, int NMAT, int WAVES>
+struct Tiles {
+  static constexpr int kBytes = ROWS * BK * 2;                 // of one tile
+  static constexpr int kPerTile = kBytes / 1024;               // loads of a wave (1 KB) for one tile
+  static constexpr int kSlots = kPerTile * P * NMAT / WAVES;
+  static constexpr int kRowChunks = T ? ROWS / 8 : BK / 8;     // 16-byte chunks of a tile row
+  static_assert(kPerTile * P * NMAT % WAVES == 0 && kBytes % 1024 == 0, "whole loads per wave");
   int voff[kSlots], kl[kSlots];
 
-  // permutation of the chunks of k row k (T): flips 32-byte halves, so that the four k rows that sixteen lanes read, and the two
-  // sets eight rows apart, lie in different banks
-  static __device__ __forceinline__ int perm(int k) { return (((k & 3) | ((k >> 3) & 1) << 2) << 1) & (kChunks - 1); }
-
+  // Which chunk of row r lies where (an xor).  Rows along k: sixteen rows of one chunk in different 16-byte columns of the 256-byte
+  // bank line.  Rows across k: the four rows that sixteen lanes read, and the set eight rows on, in different 32-byte columns.
+  static __device__ __forceinline__ int perm(int r) {
+    if (!T) return BK == 64 ? (r >> 1) & 7 : (r >> 2) & 3;
+    if (kRowChunks >= 16) return ((r & 3) | ((r >> 3) & 1) << 2) << 1;
+    if (kRowChunks == 8) return (((r >> 1) & 1) | ((r >> 3) & 1) << 1) << 1;
+    return ((r >> 3) & 1) << 1;
+  }
   __device__ __forceinline__ void init(int row0, int rows, int ld, int wave, int lane) {
 #pragma unroll
     for (int i = 0; i < kSlots; ++i) {
-      const int ci = (wave * kSlots + i) * 64 + lane;
-      int r, k;
-      if (T) {
-        k = ci / kChunks;
-        r = ((ci % kChunks) ^ perm(k)) * 8;
-        voff[i] = (k * ld + r) * 2;
-      } else {
-        r = ci >> 3;
-        k = ((ci & 7) ^ (r & 7)) * 8;
-        voff[i] = (r * ld + k) * 2;
-      }
+      const int ci = ((wave * kSlots + i) % kPerTile) * 64 + lane, tr = ci / kRowChunks, c = (ci % kRowChunks) ^ perm(tr);
+      const int r = T ? c * 8 : tr, k = T ? tr : c * 8;
+      voff[i] = (T ? k * ld + r : r * ld + k) * 2;
       kl[i] = row0 + r < rows ? k : 0x7fffffff;
     }
   }
-  // k tile kt of the operand at p (its row / column row0 already added) into LDS
-  __device__ __forceinline__ void load(const uint16_t* p, int ld, int kt, int K, AGCN_LDS char* dst, int wave) const {
-    const uint16_t* base = p + (T ? (int64_t)kt * BK * ld : (int64_t)kt * BK);
-    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(base), 0, 0x7fffffff, 0x00020000);
-    const int left = K - kt * BK;
+  // k tile kt of the operand at p0 / p1 (its row or column row0 already added) into LDS; `left`: k that remain there
+  __device__ __forceinline__ void load(const uint16_t* p0, const uint16_t* p1, int64_t plane, int ld, int kt, int left, AGCN_LDS char* dst, int wave) const {
+    const int64_t kofs = T ? (int64_t)kt * BK * ld : (int64_t)kt * BK;
 #pragma unroll
-    for (int i = 0; i < kSlots; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (AGCN_LDS void*)(dst + (wave * kSlots + i) * 1024), 16,
-                                               kl[i] < left ? voff[i] : (int)0x80000000, 0, 0, 0);
+    for (int i = 0; i < kSlots; ++i) {
+      const int t = wave * kSlots + i, tile = t / kPerTile;    // tile: matrix * P + plane
+      const uint16_t* base = (NMAT == 2 && tile >= P ? p1 : p0) + (P == 1 ? 0 : (tile % P) * plane) + kofs;
+      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(base), 0, 0x7fffffff, 0x00020000);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (AGCN_LDS void*)(dst + t * 1024), 16, kl[i] < left ? voff[i] : (int)0x80000000, 0, 0, 0);
+    }
   }
+  // Fragment f, k step kk (32 k) of tile `tile`: sixteen rows, lane (r = lane & 15, q = lane / 16) gets k = 8 q .. 8 q + 7 of row r.
+  // T: the lane's place in each of the FR fragments is worked out once and hidden from the compiler: through the chain of additions
+  // that it would build otherwise it does not see which array a transposing read reads, and waits for all loads in flight.
+  template <int FR>
+  struct Reader {
+    int at[T ? FR : 1], lane, row0;
+    __device__ __forceinline__ Reader(int row, int lane_) : lane(lane_), row0(row) {
+      const int l = lane & 15, k = (lane >> 4) * 8 + (l >> 2);
+#pragma unroll
+      for (int f = 0; f < (T ? FR : 0); ++f) {
+        const int chunk = (((row + f * 16) >> 3) + ((l & 3) >> 1)) ^ perm(k);
+        at[f] = k * (ROWS * 2) + chunk * 16 + (l & 1) * 8;
+        asm volatile("" : "+v"(at[f]));
+      }
+    }
+    __device__ __forceinline__ u32x4 operator()(const AGCN_LDS char* s, int tile, int f, int kk) const {
+      if (!T) {
+        const int l = lane & 15, q = lane >> 4;
+        return *reinterpret_cast<const AGCN_LDS u32x4*>(s + tile * kBytes + (row0 + f * 16 + l) * (BK * 2) + (((kk * 4 + q) ^ perm(l)) << 4));
+      } else {
+        const AGCN_LDS char* p = s + at[f] + (tile * BK + kk * 32) * (ROWS * 2);
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((AGCN_LDS s16x4*)p);
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((AGCN_LDS s16x4*)(p + 4 * ROWS * 2));
+        const u32x2 a = __builtin_bit_cast(u32x2, lo), b = __builtin_bit_cast(u32x2, hi);
+        return (u32x4){a.x, a.y, b.x, b.y};
+      }
+    }
+  };
 };
-
-// fragment f (16 rows from row r0 + 16 f) of k step kk (32 k): lane (r = lane & 15, q = lane / 16) gets k = 8 q .. 8 q + 7 of row r
-template <int ROWS, bool T>
-__device__ __forceinline__ u32x4 fragment(const AGCN_LDS char* s, int row, int kk, int lane) {
-  const int l = lane & 15, q = lane >> 4;
-  if (!T) {
-    const int off = (row + l) * (BK * 2) + (((kk * 4 + q) ^ (l & 7)) << 4);
-    return *reinterpret_cast<const AGCN_LDS u32x4*>(s + off);
-  } else {
-    const int k = kk * 32 + q * 8 + (l >> 2);
-    const int chunk = ((row >> 3) + ((l & 3) >> 1)) ^ Tile<ROWS, true, 256>::perm(q * 8 + (l >> 2));
-    const AGCN_LDS char* p = s + k * (ROWS * 2) + chunk * 16 + (l & 1) * 8;
-    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((AGCN_LDS s16x4*)p);
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((AGCN_LDS s16x4*)(p + 4 * ROWS * 2));
-    const u32x2 a = __builtin_bit_cast(u32x2, lo), b = __builtin_bit_cast(u32x2, hi);
-    return (u32x4){a.x, a.y, b.x, b.y};
-  }
-}
-
 #endif
 
-// BM x (NB x BN) tile by WGM x WGN waves; AT / BT: the operand's matrix has k along its rows
-template <int BM, int BN, int WGM, int WGN, bool AT, bool BT, int NB, int EPI>
+// BM x (NB x BN) tile by WGM x WGN waves, P planes of pieces, S (2, 3) stages; AT / BT: the operand's matrix has k along its rows
+template <int P, int BM, int BN, int WGM, int WGN, bool AT, bool BT, int NB, int EPI, int S>
 __global__ __launch_bounds__(64 * WGM * WGN) void ffn_gemm_kernel(GemmArgs g) {
 #ifdef __HIP_DEVICE_COMPILE__
-  constexpr int THREADS = 64 * WGM * WGN, FM = BM / WGM / 16, FN = BN / WGN / 16;
-  constexpr int SA = BM * BK * 2, SB = BN * BK * 2;
-  __shared__ __attribute__((aligned(1024))) char sA0[SA];
-  __shared__ __attribute__((aligned(1024))) char sA1[SA];
-  __shared__ __attribute__((aligned(1024))) char sB0[NB * SB];
-  __shared__ __attribute__((aligned(1024))) char sB1[NB * SB];
+  constexpr int WAVES = WGM * WGN, FM = BM / WGM / 16, FN = BN / WGN / 16, BK = P == 1 ? 64 : 32;
+  typedef Tiles<BM, AT, BK, P, 1, WAVES> TA;
+  typedef Tiles<BN, BT, BK, P, NB, WAVES> TB;
+  constexpr int SA = P * TA::kBytes, SB = NB * P * TB::kBytes;
+  // (arrays of their own for every stage and operand: the compiler then sees that the loads into one do not touch the reads of
+  // another; it would wait for all loads in flight otherwise)
+  __shared__ __attribute__((aligned(1024))) char sa0[SA], sa1[SA], sa2[S > 2 ? SA : 16];
+  __shared__ __attribute__((aligned(1024))) char sb0[SB], sb1[SB], sb2[S > 2 ? SB : 16];
+  AGCN_LDS char *const a0 = (AGCN_LDS char*)sa0, *const a1 = (AGCN_LDS char*)sa1, *const a2 = (AGCN_LDS char*)sa2;
+  AGCN_LDS char *const b0 = (AGCN_LDS char*)sb0, *const b1 = (AGCN_LDS char*)sb1, *const b2 = (AGCN_LDS char*)sb2;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / WGN, wn = wave - wm * WGN;
 
   // workgroup -> tile: workgroups go round the eight dies; a die gets a run of neighbouring tiles (its L2 holds their operands),
   // and within a run four tile rows are walked together
-  const int tiles = g.tiles_m * g.tiles_n, total = tiles * g.splits, run = (total + 7) >> 3;
+  const int total = g.tiles_m * g.tiles_n * g.splits, run = (total + 7) >> 3;
   const int id = (blockIdx.x & 7) * run + (blockIdx.x >> 3);
-  if (id >= total) return;
+  if ((int)(blockIdx.x >> 3) >= run || id >= total) return;
   const int tile = id / g.splits, split = id - tile * g.splits;
   const int per = 4 * g.tiles_n, grp = tile / per, first = grp * 4;
   const int rows_in = g.tiles_m - first < 4 ? g.tiles_m - first : 4;
   const int in = tile - grp * per, tm = first + in % rows_in, tn = in / rows_in;
   const int m0 = tm * BM, n0 = tn * BN;
 
-  Tile<BM, AT, THREADS> ta;
-  Tile<BN, BT, THREADS> tb;
+  TA ta;
+  TB tb;
   ta.init(m0, g.M, g.lda, wave, lane);
   tb.init(n0, g.N, g.ldb, wave, lane);
   const int64_t a_at = AT ? m0 : (int64_t)m0 * g.lda, b_at = BT ? n0 : (int64_t)n0 * g.ldb;
 
   const int iters = g.nseg * g.ktiles;
   const int it0 = (int)((int64_t)iters * split / g.splits), it1 = (int)((int64_t)iters * (split + 1) / g.splits);
-  int seg = it0 / g.ktiles, kt = it0 - seg * g.ktiles;
+  int lit = it0, seg = it0 / g.ktiles, kt = it0 - seg * g.ktiles;      // the next k tile to load
+  // (three stages: past the last one the loads still run, on nothing, so that the count of loads in flight stays what the
+  // waits below expect.  Two stages: no load, and the branch keeps the scheduler from spreading the loads over the products, which
+  // costs it more registers than there are)
   auto load = [&](AGCN_LDS char* a, AGCN_LDS char* b) {
-    const Seg s = g.seg[seg];
-    ta.load(s.a + a_at, g.lda, kt, g.K, a, wave);
-    tb.load(s.b + b_at, g.ldb, kt, g.K, b, wave);
-    if (NB == 2) tb.load(s.b2 + b_at, g.ldb, kt, g.K, b + SB, wave);
+    const Seg s = g.seg[seg < 2 ? seg : 1];
+    const int left = lit < it1 ? g.K - kt * BK : 0;
+    ta.load(s.a + a_at, nullptr, g.a_plane, g.lda, kt, left, a, wave);
+    tb.load(s.b + b_at, NB == 2 ? s.b2 + b_at : nullptr, g.b_plane, g.ldb, kt, left, b, wave);
+    ++lit;
     if (++kt == g.ktiles) { kt = 0; ++seg; }
   };
   f32x4 acc[NB][FM][FN];
@@ -280,78 +343,168 @@ __global__ __launch_bounds__(64 * WGM * WGN) void ffn_gemm_kernel(GemmArgs g) {
     for (int i = 0; i < FM; ++i)
 #pragma unroll
       for (int j = 0; j < FN; ++j) acc[b][i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  const typename TA::template Reader<FM> ra(wm * FM * 16, lane);
+  const typename TB::template Reader<FN> rb(wn * FN * 16, lane);
   auto compute = [&](const AGCN_LDS char* a, const AGCN_LDS char* b) {
 #pragma unroll
     for (int kk = 0; kk < BK / 32; ++kk) {
-      u32x4 fa[FM], fb[NB][FN];
+      u32x4 fa[P][FM], fb[P][NB][FN];
 #pragma unroll
-      for (int i = 0; i < FM; ++i) fa[i] = fragment<BM, AT>(a, wm * FM * 16 + i * 16, kk, lane);
+      for (int p = 0; p < P; ++p) {
 #pragma unroll
-      for (int c = 0; c < NB; ++c)
-#pragma unroll
-        for (int j = 0; j < FN; ++j) fb[c][j] = fragment<BN, BT>(b + c * SB, wn * FN * 16 + j * 16, kk, lane);
-      // (B as the first operand: a lane then holds four neighbouring COLUMNS of one row of the result)
-#pragma unroll
-      for (int i = 0; i < FM; ++i)
+        for (int i = 0; i < FM; ++i) fa[p][i] = ra(a, p, i, kk);
 #pragma unroll
         for (int c = 0; c < NB; ++c)
 #pragma unroll
-          for (int j = 0; j < FN; ++j) acc[c][i][j] = mfma_bf(fb[c][j], fa[i], acc[c][i][j]);
+          for (int j = 0; j < FN; ++j) fb[p][c][j] = rb(b, c * P + p, j, kk);
+      }
+      // (B as the first operand: a lane then holds four neighbouring COLUMNS of one row of the result.  Pieces: small terms first)
+      constexpr int NP = P == 1 ? 1 : 6;
+      constexpr int pa[6] = {P - 1, 0, P == 1 ? 0 : 1, P == 1 ? 0 : 1, 0, 0}, pb[6] = {0, P - 1, P == 1 ? 0 : 1, 0, P == 1 ? 0 : 1, 0};
+#pragma unroll
+      for (int t = 0; t < NP; ++t)
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+          for (int c = 0; c < NB; ++c)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) acc[c][i][j] = mfma_bf(fb[pb[t]][c][j], fa[pa[t]][i], acc[c][i][j]);
     }
   };
-  // a stage is there when every wave's own transfers are (vmcnt) and all waves have said so
+  // a stage is there when every wave's own loads of it are (vmcnt counts the later stages' loads that may still fly) and all
+  // waves have said so; the same barrier says that the stage about to be overwritten has been read
   auto ready = [] {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
+    constexpr int fly = (S - 2) * (TA::kSlots + TB::kSlots);
+    // (not __syncthreads(), whose fence waits for every load in flight; and the builtin, not text, so that the compiler's own
+    // account of the loads in flight sees the wait)
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt((fly & 15) | 7 << 4 | (fly >> 4) << 14);       // vmcnt(fly) lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
   };
-  AGCN_LDS char *a0 = (AGCN_LDS char*)sA0, *a1 = (AGCN_LDS char*)sA1, *b0 = (AGCN_LDS char*)sB0, *b1 = (AGCN_LDS char*)sB1;
+  load(a0, b0);
+  if (S > 2) load(a1, b1);
   int it = it0;
-  if (it < it1) load(a0, b0);
-  while (it < it1) {
-    ready();
-    if (it + 1 < it1) load(a1, b1);
-    compute(a0, b0);
-    if (++it >= it1) break;
-    ready();
-    if (it + 1 < it1) load(a0, b0);
-    compute(a1, b1);
-    ++it;
-  }
-  const int mr = lane & 15, nq = (lane >> 4) * 4;
-#pragma unroll
-  for (int i = 0; i < FM; ++i) {
-    const int m = m0 + (wm * FM + i) * 16 + mr;
-    __builtin_amdgcn_sched_barrier(0);       // (the reads of G and U of one row of fragments in flight at a time: registers)
-    if (m >= g.M) continue;
-#pragma unroll
-    for (int j = 0; j < FN; ++j) {
-      const int n = n0 + (wn * FN + j) * 16 + nq;
-      if (g.splits > 1) {
-        if (n < g.ldp) {
-          float* p = g.part + (((int64_t)split * NB) * g.M + m) * g.ldp + n;
-          *reinterpret_cast<f32x4*>(p) = acc[0][i][j];
-          if (NB == 2) *reinterpret_cast<f32x4*>(p + (int64_t)g.M * g.ldp) = acc[NB - 1][i][j];
-        }
-      } else {
-        epilogue<EPI, NB>(g, m, n, acc[0][i][j], acc[NB - 1][i][j]);
+  if constexpr (S == 2) {
+    // (ifs, not breaks: one way out of the loop, or the accumulators are copied at each)
+    for (; it < it1; it += 2) {
+      ready();
+      if (it + 1 < it1) load(a1, b1);
+      compute(a0, b0);
+      if (it + 1 < it1) {
+        ready();
+        if (it + 2 < it1) load(a0, b0);
+        compute(a1, b1);
       }
     }
+  } else {
+    // (whole turns without branches, in which the compiler can count the loads in flight; then what is left)
+    for (; it + 3 <= it1; it += 3) {
+      ready();
+      load(a2, b2);
+      compute(a0, b0);
+      ready();
+      load(a0, b0);
+      compute(a1, b1);
+      ready();
+      load(a1, b1);
+      compute(a2, b2);
+    }
+    if (it < it1) {
+      ready();
+      load(a2, b2);
+      compute(a0, b0);
+      if (it + 1 < it1) {
+        ready();
+        compute(a1, b1);
+      }
+    }
+  }
+  // Through LDS: a wave's fragments of PR rows at a time, [row][B matrix][column] with the 16-byte chunks permuted by the row
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  constexpr int CH = NB * FN * 4, REGION = (SA < SB ? SA : SB) / (WAVES / 4);      // a quarter of the waves in each array of two stages
+  constexpr int FIT = REGION / (CH * 16) / 16, PF = FIT >= FM ? FM : (FIT >= FM / 2 ? FM / 2 : FM / 4), PR = PF * 16;      // fragments, rows per pass
+  static_assert(PF >= 1 && PF <= FIT && FM % PF == 0 && WAVES % 4 == 0, "the epilogue's rows have to fit the wave's part of the stages");
+  AGCN_LDS char* reg = (wave & 2 ? (wave & 1 ? b1 : b0) : (wave & 1 ? a1 : a0)) + (wave >> 2) * REGION;
+  const int n_wave = n0 + wn * FN * 16;
+#pragma unroll
+  for (int ps = 0; ps < FM / PF; ++ps) {
+    const int mr = lane & 15, q = lane >> 4;
+#pragma unroll
+    for (int i = 0; i < PF; ++i)
+#pragma unroll
+      for (int c = 0; c < NB; ++c)
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+          *reinterpret_cast<AGCN_LDS f32x4*>(reg + (i * 16 + mr) * (CH * 16) + ((((c * FN + j) * 4 + q) ^ (mr & (CH - 1))) << 4)) = acc[c][ps * PF + i][j];
+    // (one wave's own rows: the wait is for its own writes)
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    constexpr int LPR = FN * 2;                       // lanes per row, eight columns each
+    const int c8 = lane % LPR;
+#pragma unroll 1
+    for (int r0 = 0; r0 < PR; r0 += 64 / LPR) {
+      const int r = r0 + lane / LPR, m = m0 + wm * FM * 16 + ps * PR + r, n = n_wave + c8 * 8;
+      F8 v[NB];
+#pragma unroll
+      for (int c = 0; c < NB; ++c) {
+        const int ch = (c * FN * 4 + c8 * 2), x = r & 15 & (CH - 1);
+        const f32x4 lo = *reinterpret_cast<const AGCN_LDS f32x4*>(reg + r * (CH * 16) + ((ch ^ x) << 4));
+        const f32x4 hi = *reinterpret_cast<const AGCN_LDS f32x4*>(reg + r * (CH * 16) + (((ch + 1) ^ x) << 4));
+        v[c] = {{lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w}};
+      }
+      if (m < g.M) {
+        if (g.splits > 1) {
+          if (n < g.ldp) {
+            float* p = g.part + ((int64_t)split * NB * g.M + m) * g.ldp + n;
+            store8_f32(p, v[0]);
+            if (NB == 2) store8_f32(p + (int64_t)g.M * g.ldp, v[NB - 1]);
+          }
+        } else {
+          epilogue<EPI, NB>(g, m, n, v[0], v[NB - 1]);
+        }
+      }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   }
 #endif
 }
 
-// adds the splits' tiles in order and puts the sums through the epilogue; a thread takes four columns
+// Adds the splits' tiles in order and puts the sums through the epilogue.  A workgroup takes 32 times eight columns; eight lanes
+// share the splits of each (a single lane would wait for one load after another), and their sums are added in lane order.
 template <int NB, int EPI>
 __global__ __launch_bounds__(256) void ffn_reduce_kernel(GemmArgs g) {
-  const int64_t per = g.ldp >> 2, e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (e >= per * g.M) return;
-  const int m = (int)(e / per), n = (int)(e - (int64_t)m * per) * 4;
-  f32x4 v[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-  for (int s = 0; s < g.splits; ++s)
+  __shared__ float sums[8][32][NB * 8 + 1];
+  const int64_t per = g.ldp >> 3, e = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
+  const int sl = threadIdx.x >> 5, ev = threadIdx.x & 31;
+  const bool live = e < per * g.M;
+  const int m = live ? (int)(e / per) : 0, n = live ? (int)(e - (int64_t)m * per) * 8 : 0;
+  float v[NB * 8];
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
-      v[b] += *reinterpret_cast<const f32x4*>(g.part + (((int64_t)s * NB + b) * g.M + m) * g.ldp + n);
-  epilogue<EPI, NB>(g, m, n, v[0], v[NB - 1]);
+  for (int i = 0; i < NB * 8; ++i) v[i] = 0.f;
+  if (live) {
+#pragma unroll 4
+    for (int s = sl; s < g.splits; s += 8)
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        const F8 x = load8_f32(g.part + (((int64_t)s * NB + b) * g.M + m) * g.ldp + n);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[b * 8 + i] += x.v[i];
+      }
+  }
+#pragma unroll
+  for (int i = 0; i < NB * 8; ++i) sums[sl][ev][i] = v[i];
+  __syncthreads();
+  if (sl || !live) return;
+  F8 o[NB];
+#pragma unroll
+  for (int i = 0; i < NB * 8; ++i) {
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s += sums[k][ev][i];
+    o[i >> 3].v[i & 7] = s;
+  }
+  epilogue<EPI, NB>(g, m, n, o[0], o[NB - 1]);
 }
 
 // Operand images: bf16 matrices whose rows do not start at 16 bytes or end at eights, padded with zeros; fp32 ones as three planes of
@@ -434,7 +587,7 @@ struct Reserve { uint16_t *x, *wg, *wu, *wd, *hid; void *g, *u; };
 size_t carve_reserve(const AgcnFfnDesc& d, void* mem, Reserve* r) {
   Carve c{static_cast<char*>(mem), 0};
   const int P = d.dtype == AGCN_DTYPE_F32 ? 3 : 1, Hp = pad8(d.H), Fp = pad8(d.Fin), Op = pad8(d.Fout);
-  const size_t e = d.dtype == AGCN_DTYPE_F32 ? 4 : 2;
+  const size_t e = d.dtype == AGCN_DTYPE_F32 ? 4 : 3;
   r->x = static_cast<uint16_t*>(c.take((size_t)P * d.rows * Fp * 2));
   r->wg = static_cast<uint16_t*>(c.take((size_t)P * d.Fin * Hp * 2));
   r->wu = static_cast<uint16_t*>(c.take((size_t)P * d.Fin * Hp * 2));
@@ -445,52 +598,63 @@ size_t carve_reserve(const AgcnFfnDesc& d, void* mem, Reserve* r) {
   return c.off;
 }
 
-struct Config { int bm, bn, splits; };      // bn: columns of one B matrix
-
-// Tile and splits for an [M, N] result over `iters` k stages with nb B matrices.
-Config choose(int64_t M, int64_t N, int nb, int64_t iters) {
-  const int bns = 256 / nb;
-  if (cdiv(M, 256) * cdiv(N, bns) >= 192) return {256, bns, 1};
-  if (cdiv(M, 128) * cdiv(N, 128 / nb) >= 256) return {128, 128 / nb, 1};
-  const int64_t tiles = std::max<int64_t>(1, cdiv(M, 64) * cdiv(N, 64));    // (size queries come here with no rows, too)
-  int64_t s = 1;
-  if (tiles < 512) s = std::min(cdiv(1024, tiles), std::max<int64_t>(1, iters / 4));
-  return {64, 64, (int)s};
+// Tile of a product, its splits, and the kernel's stages: 0 large (256 x 256; three planes: 256 x 128), 1 middle (128 x 128; 128 x 64),
+// 2 small (64 x 64; two B matrices: 64 of each; three planes: 32 of each).
+struct Config { int kind, bm, bn, splits; };      // bn: columns of one B matrix
+Config tile_of(int kind, int planes, int nb, int splits) {
+  if (kind == 0) return {0, 256, (planes == 1 ? 256 : 128) / nb, splits};
+  if (kind == 1) return {1, 128, (planes == 1 ? 128 : 64) / nb, splits};
+  return {2, 64, planes == 1 ? 64 : 64 / nb, splits};
+}
+Config choose(int64_t M, int64_t N, int nb, int planes, int64_t iters) {
+  Config c = tile_of(0, planes, nb, 1);
+  if (cdiv(M, c.bm) * cdiv(N, c.bn) >= 192) return c;
+  c = tile_of(1, planes, nb, 1);
+  if (cdiv(M, c.bm) * cdiv(N, c.bn) >= 256) return c;
+  c = tile_of(2, planes, nb, 1);
+  const int64_t tiles = std::max<int64_t>(1, cdiv(M, c.bm) * cdiv(N, c.bn));    // (size queries come here with no rows, too)
+  if (tiles < 512) c.splits = (int)std::min<int64_t>(64, std::min(cdiv(1024, tiles), std::max<int64_t>(1, iters / 4)));
+  return c;
 }
 
 size_t part_bytes(const Config& c, int64_t M, int64_t N, int nb) {
-  return c.splits > 1 ? (size_t)c.splits * nb * M * ((N + 3) & ~3ll) * sizeof(float) : 0;
+  return c.splits > 1 ? (size_t)c.splits * nb * M * ((N + 7) & ~7ll) * sizeof(float) : 0;
 }
+int planes_of(const AgcnFfnDesc& d) { return d.dtype == AGCN_DTYPE_F32 ? 3 : 1; }
+int64_t ktiles_of(const AgcnFfnDesc& d, int64_t K) { return cdiv(K, d.dtype == AGCN_DTYPE_F32 ? 32 : 64); }
 
-// segments of a product of two piece matrices, small terms first
-int add_segments(GemmArgs* g, int at, const Mat& a, const Mat& b, const Mat* b2) {
-  static const int ia[6] = {2, 0, 1, 1, 0, 0}, ib[6] = {0, 2, 1, 0, 1, 0};
-  const int n = a.plane ? 6 : 1;
-  for (int i = 0; i < n; ++i) {
-    const int x = n == 1 ? 0 : ia[i], y = n == 1 ? 0 : ib[i];
-    g->seg[at + i] = {a.p + x * a.plane, b.p + y * b.plane, b2 ? b2->p + y * b2->plane : nullptr};
-  }
-  return at + n;
-}
-
-template <int BM, int BN, int WGM, int WGN, bool AT, bool BT, int NB, int EPI>
+template <int P, int BM, int BN, int WGM, int WGN, bool AT, bool BT, int NB, int EPI, int S>
 void launch_tile(const GemmArgs& g, hipStream_t s) {
   const int64_t total = (int64_t)g.tiles_m * g.tiles_n * g.splits;
-  hipLaunchKernelGGL((ffn_gemm_kernel<BM, BN, WGM, WGN, AT, BT, NB, EPI>), dim3((unsigned)(cdiv(total, 8) * 8)), dim3(64 * WGM * WGN), 0, s, g);
+  hipLaunchKernelGGL((ffn_gemm_kernel<P, BM, BN, WGM, WGN, AT, BT, NB, EPI, S>), dim3((unsigned)(cdiv(total, 8) * 8)), dim3(64 * WGM * WGN), 0, s, g);
 }
 
 template <bool AT, bool BT, int NB, int EPI>
 void product(GemmArgs& g, void* part, hipStream_t s) {
-  g.ktiles = (int)cdiv(g.K, BK);
+  const int planes = g.f32 ? 3 : 1;
+  g.ktiles = (int)cdiv(g.K, g.f32 ? 32 : 64);
   const int n_all = EPI == EPI_STORE ? g.N : g.ldh;         // columns that the epilogue has to reach
-  const Config c = choose(g.M, n_all, NB, (int64_t)g.nseg * g.ktiles);
+  const Config c = choose(g.M, n_all, NB, planes, (int64_t)g.nseg * g.ktiles);
   g.tiles_m = (int)cdiv(g.M, c.bm); g.tiles_n = (int)cdiv(n_all, c.bn); g.splits = c.splits;
-  g.part = static_cast<float*>(part); g.ldp = (n_all + 3) & ~3;
-  if (c.bm == 256) launch_tile<256, 256 / NB, 2, 4, AT, BT, NB, EPI>(g, s);
-  else if (c.bm == 128) launch_tile<128, 128 / NB, 2, 2, AT, BT, NB, EPI>(g, s);
-  else launch_tile<64, 64, 2, 2, AT, BT, NB, EPI>(g, s);
+  g.part = static_cast<float*>(part); g.ldp = (n_all + 7) & ~7;
+  if (planes == 1) {
+    if (c.kind == 0) launch_tile<1, 256, 256 / NB, 2, 4, AT, BT, NB, EPI, 2>(g, s);
+    else if (c.kind == 1) launch_tile<1, 128, 128 / NB, 2, 2, AT, BT, NB, EPI, 2>(g, s);
+    else launch_tile<1, 64, 64, 2, 2, AT, BT, NB, EPI, 3>(g, s);
+  } else {
+    if (c.kind == 0) launch_tile<3, 256, 128 / NB, 4, 2, AT, BT, NB, EPI, 2>(g, s);
+    else if (c.kind == 1) launch_tile<3, 128, 64 / NB, 2, 2, AT, BT, NB, EPI, 2>(g, s);
+    else launch_tile<3, 64, 64 / NB, 2, 2, AT, BT, NB, EPI, 3>(g, s);
+  }
   if (g.splits > 1)
-    hipLaunchKernelGGL((ffn_reduce_kernel<NB, EPI>), dim3((unsigned)cdiv((int64_t)g.M * (g.ldp / 4), 256)), dim3(256), 0, s, g);
+    hipLaunchKernelGGL((ffn_reduce_kernel<NB, EPI>), dim3((unsigned)cdiv((int64_t)g.M * (g.ldp / 8), 32)), dim3(256), 0, s, g);
+}
+
+// the operands of a product: one or two pairs of matrices
+void operands(GemmArgs* g, const Mat& a, const Mat& b, const Mat* b2) {
+  g->seg[g->nseg++] = {a.p, b.p, b2 ? b2->p : nullptr};
+  g->a_plane = a.plane; g->b_plane = b.plane;
+  g->lda = a.ld; g->ldb = b.ld;
 }
 
 int check_ffn(const AgcnFfnDesc* d, const char* who) {
@@ -530,29 +694,26 @@ Mat same(const AgcnFfnDesc& d, const void* src, int64_t rows, int cols, int ld, 
 GemmArgs base_args(const AgcnFfnDesc& d) {
   GemmArgs g;
   std::memset(&g, 0, sizeof(g));
-  g.act = d.activation; g.f32 = d.dtype == AGCN_DTYPE_F32; g.planes = g.f32 ? 3 : 1;
+  g.act = d.activation; g.f32 = d.dtype == AGCN_DTYPE_F32;
   g.ldh = pad8(d.H); g.plane = (int64_t)d.rows * g.ldh;
   return g;
 }
-int nsegs(const AgcnFfnDesc& d) { return d.dtype == AGCN_DTYPE_F32 ? 6 : 1; }
 
+size_t product_part(const AgcnFfnDesc& d, int64_t M, int64_t N, int nb, int64_t K, int nseg) {
+  return part_bytes(choose(M, N, nb, planes_of(d), nseg * ktiles_of(d, K)), M, N, nb);
+}
 size_t forward_part(const AgcnFfnDesc& d) {
-  const int ns = nsegs(d), Hp = pad8(d.H);
-  return std::max(part_bytes(choose(d.rows, Hp, 2, ns * cdiv(d.Fin, BK)), d.rows, Hp, 2),
-                  part_bytes(choose(d.rows, d.Fout, 1, ns * cdiv(d.H, BK)), d.rows, d.Fout, 1));
+  return std::max(product_part(d, d.rows, pad8(d.H), 2, d.Fin, 1), product_part(d, d.rows, d.Fout, 1, d.H, 1));
 }
 struct BackWs { uint16_t *dy, *dg, *du; void* part; };
 size_t carve_backward(const AgcnFfnDesc& d, void* mem, BackWs* w) {
-  const int ns = nsegs(d), P = ns == 6 ? 3 : 1, Hp = pad8(d.H);
+  const int P = planes_of(d), Hp = pad8(d.H);
   Carve c{static_cast<char*>(mem), 0};
   w->dy = static_cast<uint16_t*>(c.take((size_t)P * d.rows * pad8(d.Fout) * 2));
   w->dg = static_cast<uint16_t*>(c.take((size_t)P * d.rows * Hp * 2));
   w->du = static_cast<uint16_t*>(c.take((size_t)P * d.rows * Hp * 2));
-  const size_t part = std::max(std::max(part_bytes(choose(d.rows, Hp, 1, ns * cdiv(d.Fout, BK)), d.rows, Hp, 1),
-                                        part_bytes(choose(d.rows, d.Fin, 1, 2 * ns * cdiv(d.H, BK)), d.rows, d.Fin, 1)),
-                               std::max(part_bytes(choose(d.Fin, d.H, 2, ns * cdiv(d.rows, BK)), d.Fin, d.H, 2),
-                                        part_bytes(choose(d.H, d.Fout, 1, ns * cdiv(d.rows, BK)), d.H, d.Fout, 1)));
-  w->part = c.take(part);
+  w->part = c.take(std::max(std::max(product_part(d, d.rows, Hp, 1, d.Fout, 1), product_part(d, d.rows, d.Fin, 1, d.H, 2)),
+                            std::max(product_part(d, d.Fin, d.H, 2, d.rows, 1), product_part(d, d.H, d.Fout, 1, d.rows, 1))));
   return c.off;
 }
 void zero(void* p, int64_t bytes, hipStream_t s) {
@@ -602,14 +763,14 @@ extern "C" int agcn_gated_ffn_forward(const AgcnFfnDesc* desc, const void* X, co
   const Mat wd = list.add(d, Wd, d.H, d.Fout, d.Fout, r.wd);
   list.launch(s);
   GemmArgs g = base_args(d);
-  g.nseg = add_segments(&g, 0, x, wg, &wu);
-  g.M = (int)d.rows; g.N = d.H; g.K = d.Fin; g.lda = x.ld; g.ldb = wg.ld;
+  operands(&g, x, wg, &wu);
+  g.M = (int)d.rows; g.N = d.H; g.K = d.Fin;
   g.g = r.g; g.u = r.u; g.hid = r.hid;
   product<false, true, 2, EPI_GATED>(g, workspace, s);
   const Mat hid = {r.hid, g.ldh, g.f32 ? g.plane : 0};
   GemmArgs q = base_args(d);
-  q.nseg = add_segments(&q, 0, hid, wd, nullptr);
-  q.M = (int)d.rows; q.N = d.Fout; q.K = d.H; q.lda = hid.ld; q.ldb = wd.ld;
+  operands(&q, hid, wd, nullptr);
+  q.M = (int)d.rows; q.N = d.Fout; q.K = d.H;
   q.out = Y; q.ldo = d.Fout;
   product<false, true, 1, EPI_STORE>(q, workspace, s);
   hipError_t e = hipGetLastError();
@@ -653,29 +814,30 @@ extern "C" int agcn_gated_ffn_backward(const AgcnFfnDesc* desc, const void* X, c
   const Mat hid = {r.hid, base.ldh, pl}, dg = {w.dg, base.ldh, pl}, du = {w.du, base.ldh, pl};
   if (dX || dWg) {
     GemmArgs g = base;                        // dA = dY Wd^T, and from it dG and dU
-    g.nseg = add_segments(&g, 0, dy, wd, nullptr);
-    g.M = (int)d.rows; g.N = d.H; g.K = d.Fout; g.lda = dy.ld; g.ldb = wd.ld;
+    operands(&g, dy, wd, nullptr);
+    g.M = (int)d.rows; g.N = d.H; g.K = d.Fout;
     g.g = r.g; g.u = r.u; g.dg = w.dg; g.du = w.du;
     product<false, false, 1, EPI_DH>(g, w.part, s);
   }
   if (dX) {
     GemmArgs g = base;
-    g.nseg = add_segments(&g, add_segments(&g, 0, dg, wg, nullptr), du, wu, nullptr);
-    g.M = (int)d.rows; g.N = d.Fin; g.K = d.H; g.lda = dg.ld; g.ldb = wg.ld;
+    operands(&g, dg, wg, nullptr);
+    operands(&g, du, wu, nullptr);
+    g.M = (int)d.rows; g.N = d.Fin; g.K = d.H;
     g.out = dX; g.ldo = d.Fin;
     product<false, false, 1, EPI_STORE>(g, w.part, s);
   }
   if (dWg) {
     GemmArgs g = base;
-    g.nseg = add_segments(&g, 0, x, dg, &du);
-    g.M = d.Fin; g.N = d.H; g.K = (int)d.rows; g.lda = x.ld; g.ldb = dg.ld;
+    operands(&g, x, dg, &du);
+    g.M = d.Fin; g.N = d.H; g.K = (int)d.rows;
     g.out = dWg; g.out2 = dWu; g.ldo = d.H;
     product<true, true, 2, EPI_STORE>(g, w.part, s);
   }
   if (dWd) {
     GemmArgs g = base;
-    g.nseg = add_segments(&g, 0, hid, dy, nullptr);
-    g.M = d.H; g.N = d.Fout; g.K = (int)d.rows; g.lda = hid.ld; g.ldb = dy.ld;
+    operands(&g, hid, dy, nullptr);
+    g.M = d.H; g.N = d.Fout; g.K = (int)d.rows;
     g.out = dWd; g.ldo = d.Fout;
     product<true, true, 1, EPI_STORE>(g, w.part, s);
   }
