@@ -150,6 +150,8 @@ class TileViews(Sequence):
             return [self[j] for j in idx]
         if i < 0:
             i += len(self)
+        if not 0 <= i < len(self):
+            raise IndexError("graph %d of %d" % (i, len(self)))
         n, off = int(self.plan.n[i]), int(self.plan.tile_off[i])
         return self.data[off:off + n * n].view(n, n)
 
@@ -185,6 +187,8 @@ class RowViews(Sequence):
             return [self[j] for j in idx]
         if i < 0:
             i += len(self)
+        if not 0 <= i < len(self):          # (iteration ends here: a slice of the padded copy past its end would be empty, not an error)
+            raise IndexError("graph %d of %d" % (i, len(self)))
         stride = getattr(self.batch, "pad_stride", 0) if self.plan.row_stride == 0 else 0
         if stride:
             return self.padded()[i * stride:(i + 1) * stride]
