@@ -14,7 +14,9 @@ with the four keys above (what `GraphTopologyMol.batch_to_feed_dict` produces, g
 """
 from .batch import GraphBatch
 
-_GRAPH_LAYERS = ("MLP", "GraphGatherMol", "GraphPoolMol", "DenseMol")
+# (GatedFeedForward, NodeNorm and NormBlockEnd have no reference counterpart: they are dispatched as the layers they stand beside,
+#  DenseMol and BlockEnd)
+_GRAPH_LAYERS = ("MLP", "GraphGatherMol", "GraphPoolMol", "DenseMol", "GatedFeedForward", "NodeNorm")
 
 
 class SequentialGraphMol(object):
@@ -54,8 +56,9 @@ class SequentialGraphMol(object):
         if missing:
             raise ValueError("feed is missing %s" % missing)
         topo = {k: batch[k] for k in ("data_slice", "original_laplacian", "lap_slice")}
-        if "graph_batch" in batch:
-            topo["graph_batch"] = batch["graph_batch"]
+        for k in ("graph_batch", "gate"):
+            if k in batch:
+                topo[k] = batch[k]
         return topo, batch["node_features"]
 
     def _input(self, topo, laplacian=True):
@@ -142,9 +145,11 @@ class SequentialGraphMol(object):
 
 
 class ResidualGraphMol(SequentialGraphMol):
-    """tf_graphs.py:107-156: ResNet-style blocks; `BlockEnd` adds the saved output of the previous block."""
+    """tf_graphs.py:107-156: ResNet-style blocks; `BlockEnd` adds the saved output of the previous block.  `NormBlockEnd` does so
+    with norms around the block: its first result is the saved output, its second what the next layer reads; a feed with a
+    'gate' entry (one vector per graph or per row) gates the blocks that end in one."""
 
-    extra_names = ("BlockEnd",)
+    extra_names = ("BlockEnd", "NormBlockEnd")
 
     def _reset(self):
         super(ResidualGraphMol, self)._reset()
@@ -161,6 +166,12 @@ class ResidualGraphMol(SequentialGraphMol):
     def _run_extra(self, layer, topo, idx):
         x = self._input(topo, laplacian=False)
         x["block_outputs"] = self.block_outputs[-1]
+        if type(layer).__name__ == "NormBlockEnd":
+            if "gate" in topo:
+                x["gate"] = topo["gate"]
+            y, self.output = layer(x)
+            self.block_outputs.append(y)
+            return
         self.output = layer(x)
         self.block_outputs.append(self.output)
 
@@ -269,7 +280,8 @@ class SegmentationGraph(SequentialGraphMol):
 
     Calling the container on a batch returns (classification_outputs, segmentation_outputs)."""
 
-    allowed = ("MLP", "GraphGatherMol", "GraphPoolMol", "SGC_LL", "DenseMol", "FCL", "Merge")
+    allowed = ("MLP", "GraphGatherMol", "GraphPoolMol", "SGC_LL", "DenseMol", "FCL", "Merge", "GatedFeedForward",
+               "NodeNorm")
 
     def __init__(self, n_feat, batch_size=50, num_point=128):
         super(SegmentationGraph, self).__init__(n_feat, batch_size, num_point)

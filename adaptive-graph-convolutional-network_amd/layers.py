@@ -25,7 +25,7 @@ import torch
 
 from .batch import GraphBatch, RowViews, TileViews
 from .functional import (CastRowsFunction, GraphGatherFunction, GraphPoolFunction, MultitaskCEFunction,
-                         PackRowsFunction, RowsDenseFunction, SgcLLFunction, _Cfg)
+                         PackRowsFunction, RowsDenseFunction, SgcLLFunction, _Cfg, gated_ffn, norm_gate_residual)
 
 _UID_PREFIXES = defaultdict(int)
 
@@ -631,6 +631,146 @@ class DenseBlockEnd(Layer):
             last = i == len(terms) - 1
             acc = RowsDenseFunction.apply(_in32(A), W, None, acc.contiguous(), gb, act if last else "linear", False, beta)
         return _row_views(_out_as(acc, X.dtype), gb)
+
+
+class _VarsLayer(Layer):
+    """A layer whose parameters are tensors in `.vars`, made on the device of the first batch."""
+
+    def _shapes(self):
+        """{name: (shape, initial value or None for glorot)} in creation order"""
+        raise NotImplementedError
+
+    def _dtype(self):
+        return torch.float32
+
+    def build(self, device=None):
+        if self.vars:
+            return
+        device = self._device if self._device is not None else device
+        for name, (shape, value) in self._shapes().items():
+            t = glorot(shape, self._generator) if value is None else torch.full(shape, float(value))
+            self.vars[name] = t.to(device=device, dtype=self._dtype()).requires_grad_(bool(self.trainable))
+
+    def load_vars(self, arrays):
+        shapes = self._shapes()
+        if sorted(arrays) != sorted(shapes):
+            raise ValueError("expected %s, got %s" % (sorted(shapes), sorted(arrays)))
+        for k, v in arrays.items():
+            t = v.detach() if torch.is_tensor(v) else torch.as_tensor(np.asarray(v))
+            if tuple(t.shape) != tuple(shapes[k][0]):
+                raise ValueError("%s must be %s, got %s" % (k, tuple(shapes[k][0]), tuple(t.shape)))
+            dev = self._device if self._device is not None else t.device
+            self.vars[k] = t.to(device=dev, dtype=self._dtype(), copy=True).requires_grad_(bool(self.trainable))
+
+    def parameters(self):
+        self.build()
+        return list(self.vars.values())
+
+
+class GatedFeedForward(_VarsLayer):
+    """Gated feed-forward layer over node rows: (act(x w_gate) * (x w_up)) w_down, beside DenseMol (no reference counterpart).
+    GatedFeedForward(n_hidden, input_dim, output_dim=input_dim, activation='silu' | 'gelu' | 'relu' | 'sigmoid').
+    dtype 'float32' (default): bf16 features are widened, as in every layer; 'bfloat16': parameters and features in bf16, the
+    products on the bf16 matrix pipe.  Rows are rows of their own (pad rows of zeros give zeros)."""
+
+    def __init__(self, n_hidden, input_dim, output_dim=None, activation="silu", dtype="float32", device=None, generator=None, **kwargs):
+        super(GatedFeedForward, self).__init__(**kwargs)
+        if activation not in ("silu", "gelu", "relu", "sigmoid"):
+            raise ValueError("Invalid activation function: %s" % (activation,))
+        if dtype not in ("float32", "bfloat16"):
+            raise ValueError("dtype must be 'float32' or 'bfloat16'")
+        self.n_hidden, self.input_dim = n_hidden, input_dim
+        self.output_dim = input_dim if output_dim is None else output_dim
+        self.activation, self.dtype = activation, dtype
+        self.vars = {}
+        self._device, self._generator = device, generator
+
+    def _dtype(self):
+        return getattr(torch, self.dtype)
+
+    def _shapes(self):
+        return {"w_gate": ([self.input_dim, self.n_hidden], None), "w_up": ([self.input_dim, self.n_hidden], None),
+                "w_down": ([self.n_hidden, self.output_dim], None)}
+
+    def call(self, x):
+        gb, X = _rows_of(x)
+        self.build(X.device)
+        Y = gated_ffn(X if self.dtype == "bfloat16" else _in32(X), self.vars["w_gate"], self.vars["w_up"], self.vars["w_down"],
+                      self.activation)
+        return _row_views(_out_as(Y, X.dtype) if Y.dtype != X.dtype else Y, gb)
+
+
+class NodeNorm(_VarsLayer):
+    """RMS or layer norm over each node's features: what the first block of a network reads (no reference counterpart).
+    NodeNorm(n_features, norm='rms' | 'layer', eps=1e-6); pad rows 0."""
+
+    def __init__(self, n_features, norm="rms", eps=1e-6, device=None, generator=None, **kwargs):
+        super(NodeNorm, self).__init__(**kwargs)
+        if norm not in ("rms", "layer"):
+            raise ValueError("norm must be 'rms' or 'layer'")
+        self.n_features, self.norm, self.eps = n_features, norm, eps
+        self.vars = {}
+        self._device, self._generator = device, generator
+
+    def _shapes(self):
+        s = {"weight": ([self.n_features], 1.0)}
+        if self.norm == "layer":
+            s["bias"] = ([self.n_features], 0.0)
+        return s
+
+    def call(self, x):
+        gb, X = _rows_of(x)
+        self.build(X.device)
+        _, h = norm_gate_residual(None, X, pre_weight=self.vars["weight"], pre_bias=self.vars.get("bias"), norm=self.norm,
+                                  eps=self.eps, plan=gb)
+        return _row_views(h, gb)
+
+
+class NormBlockEnd(_VarsLayer):
+    """Last layer of a residual block with norms around it, beside BlockEnd (blockend.py:13-86, a sum without norms):
+        y = x + scale * a(gate) * N(block output),   h = N'(y),   pad rows 0
+    in one pass.  NormBlockEnd(block_id, n_features, norm='rms' | 'layer', post_norm=True, pre_norm=True, gate_activation='linear',
+    scale=1.0 (initial value of the learned scale), eps=1e-6).
+    Input keys: node_features (the block's output), block_outputs (the residual rows x) and, where the block is gated, gate:
+    [rows, F], or one vector per graph [B, F].  call(x) -> (y, h): y is the next block's residual, h what it reads
+    (pre_norm=False: h is y)."""
+
+    def __init__(self, block_id, n_features, norm="rms", post_norm=True, pre_norm=True, gate_activation="linear", scale=1.0, eps=1e-6,
+                 device=None, generator=None, **kwargs):
+        super(NormBlockEnd, self).__init__(**kwargs)
+        if norm not in ("rms", "layer"):
+            raise ValueError("norm must be 'rms' or 'layer'")
+        if gate_activation not in ("linear", "tanh", "sigmoid", None):
+            raise ValueError("Invalid activation function: %s" % (gate_activation,))
+        self.block_id, self.n_features, self.norm, self.eps = block_id, n_features, norm, eps
+        self.post_norm, self.pre_norm, self.gate_activation, self.scale = bool(post_norm), bool(pre_norm), gate_activation, scale
+        self.vars = {}
+        self._device, self._generator = device, generator
+
+    def _shapes(self):
+        F, s = [self.n_features], {"scale": ([self.n_features], self.scale)}
+        for on, kind in ((self.post_norm, "post"), (self.pre_norm, "pre")):
+            if on:
+                s[kind + "_weight"] = (F, 1.0)
+                if self.norm == "layer":
+                    s[kind + "_bias"] = (F, 0.0)
+        return s
+
+    def call(self, x):
+        gb, Z = _rows_of(x)
+        X = _source_rows(x["block_outputs"], self.n_features, gb)
+        self.build(Z.device)
+        if X.dtype == torch.bfloat16 and Z.dtype == torch.float32:
+            Z = CastRowsFunction.apply(Z, torch.bfloat16)
+        gate = x.get("gate")
+        if gate is not None and gate.dtype != Z.dtype:
+            gate = CastRowsFunction.apply(gate, Z.dtype)
+        v = self.vars
+        y, h = norm_gate_residual(Z, X, post_weight=v.get("post_weight"), post_bias=v.get("post_bias"), gate=gate, scale=v["scale"],
+                                  pre_weight=v.get("pre_weight"), pre_bias=v.get("pre_bias"), norm=self.norm, eps=self.eps,
+                                  gate_activation=self.gate_activation, plan=gb)
+        y = _row_views(y, gb)
+        return y, (_row_views(h, gb) if self.pre_norm else y)
 
 
 class MultitaskHead(object):
