@@ -8,10 +8,11 @@
 //     with q1 = sum D a zh and q2 = sum D a over the rows:  dw = s q1, db = s q2, ds = w q1 + b q2;
 //     dw' = sum dh yh, db' = sum dh;  a gate per graph:  dg = a'(g) s (w sum D zh + b sum D) over the graph's rows.
 // Bound by memory: every operand is read once and every result written once (the row stays in registers between the two norms
-// and through all reductions).  L lanes share a row (8 consecutive elements per lane and vector, so that a lane keeps the
-// parameters and the column sums of ITS columns in registers over all rows it meets).  Sums, means and column sums are fp32
-// (a column sum's partials, one per workgroup, are added in a fixed order: no atomics); rounding happens where a result is
-// stored, and h is taken from the unrounded y.  Pad rows give zeros and take part in no sum.
+// and through all reductions).  L lanes share a row (eight consecutive elements per lane, so that a lane keeps the parameters and
+// the column sums of ITS columns in registers over all rows it meets); few elements per lane and many waves, which hide the
+// memory's latency where a row after another would not.  Sums, means and column sums are fp32 (a column sum's partials, one per
+// workgroup, are added in a fixed order: no atomics); rounding happens where a result is stored, and h is taken from the unrounded
+// y.  Pad rows give zeros and take part in no sum.
 #include <hip/hip_bf16.h>
 #include <hip/hip_runtime.h>
 
@@ -23,19 +24,18 @@
 namespace agcn {
 namespace {
 constexpr int V = 8;                    // elements per vector
-constexpr int kGraphRows = 64;          // per-graph gates: rows of a graph that one workgroup adds up
 
 struct NormArgs {
   AgcnNormDesc d;
   // plan (nullable: no pad rows, no graphs)
   const int32_t *n, *row_off, *row_graph;
-  int32_t B, splits;
+  int32_t B, splits, graph_rows;        // per-graph gates: workgroups per graph, rows of a graph that one of them adds up
   const void *z, *x, *gate, *dy, *dh;
   const float *scale, *w, *b, *w2, *b2;
   void *y, *h, *dz, *dx, *dgate;
   float* stats;                         // [rows][4]: mean z, 1 / deviation of z, mean y, 1 / deviation of y
   float* part;                          // [units][4][F]
-  int32_t units, pads;
+  int32_t units, stride, pads;          // partial sums; distance between those that the parameters' gradients are made of
 };
 
 typedef uint32_t u4f __attribute__((ext_vector_type(4), aligned(4)));
@@ -43,27 +43,49 @@ typedef uint32_t u4h __attribute__((ext_vector_type(4), aligned(2)));
 
 // eight elements, columns c .. c + 7 of a row of F (0 beyond), as floats.  Vectors are read at the alignment of an element: the
 // target runs in unaligned access mode, and odd widths start every row elsewhere.
-__device__ __forceinline__ void load8(const float* p, int c, int F, float* v) {
+// In two halves: the memory's bits first (so that a row's can be in flight while the row before it is worked on), then floats.
+template <typename T> struct Raw;
+template <> struct Raw<float> { u4f a, b; };
+template <> struct Raw<__hip_bfloat16> { u4h a; };
+__device__ __forceinline__ void fetch8(const float* p, int c, int F, Raw<float>& r) {
   if (c + V <= F) {
-    const u4f a = *reinterpret_cast<const u4f*>(p + c), b = *reinterpret_cast<const u4f*>(p + c + 4);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { v[i] = __uint_as_float(a[i]); v[4 + i] = __uint_as_float(b[i]); }
+    r.a = *reinterpret_cast<const u4f*>(p + c);
+    r.b = *reinterpret_cast<const u4f*>(p + c + 4);
   } else {
 #pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = c + i < F ? p[c + i] : 0.f;
+    for (int i = 0; i < 4; ++i) {
+      r.a[i] = c + i < F ? __float_as_uint(p[c + i]) : 0u;
+      r.b[i] = c + 4 + i < F ? __float_as_uint(p[c + 4 + i]) : 0u;
+    }
   }
 }
-__device__ __forceinline__ void load8(const __hip_bfloat16* p_, int c, int F, float* v) {
+__device__ __forceinline__ void fetch8(const __hip_bfloat16* p_, int c, int F, Raw<__hip_bfloat16>& r) {
   const uint16_t* p = reinterpret_cast<const uint16_t*>(p_);
   if (c + V <= F) {
-    const u4h a = *reinterpret_cast<const u4h*>(p + c);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(a[i] << 16); v[2 * i + 1] = __uint_as_float(a[i] & 0xffff0000u); }
+    r.a = *reinterpret_cast<const u4h*>(p + c);
   } else {
 #pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = c + i < F ? __uint_as_float((uint32_t)p[c + i] << 16) : 0.f;
+    for (int i = 0; i < 4; ++i)
+      r.a[i] = (c + 2 * i < F ? (uint32_t)p[c + 2 * i] : 0u) | (c + 2 * i + 1 < F ? (uint32_t)p[c + 2 * i + 1] << 16 : 0u);
   }
 }
+__device__ __forceinline__ void unpack8(const Raw<float>& r, float* v) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { v[i] = __uint_as_float(r.a[i]); v[4 + i] = __uint_as_float(r.b[i]); }
+}
+__device__ __forceinline__ void unpack8(const Raw<__hip_bfloat16>& r, float* v) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(r.a[i] << 16); v[2 * i + 1] = __uint_as_float(r.a[i] & 0xffff0000u); }
+}
+__device__ __forceinline__ void clear8(Raw<float>& r) { r.a = (u4f)(0u); r.b = (u4f)(0u); }
+__device__ __forceinline__ void clear8(Raw<__hip_bfloat16>& r) { r.a = (u4h)(0u); }
+
+__device__ __forceinline__ void load8(const float* p, int c, int F, float* v) {
+  Raw<float> r;
+  fetch8(p, c, F, r);
+  unpack8(r, v);
+}
+
 __device__ __forceinline__ void store8(float* p, int c, int F, const float* v) {
   if (c + V <= F) {
     u4f a, b;
@@ -105,7 +127,7 @@ __device__ __forceinline__ float gate_slope(int act, float g) {
   return (act == AGCN_ACT_TANH ? 4.f : 1.f) * e * d * d;
 }
 
-// Sums of N values over the L lanes of a row; every lane gets them.  L > 64: over the whole workgroup through `red`
+// Sums of N values over the L lanes of a row; every lane gets them.  L > 64: over the row's waves through `red`
 // (two areas used in turn, so that one barrier per call is enough).
 template <int L, int N>
 __device__ __forceinline__ void row_sums(float (&v)[N], float* red, int& turn) {
@@ -115,17 +137,18 @@ __device__ __forceinline__ void row_sums(float (&v)[N], float* red, int& turn) {
     for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], o);
   if (L > 64) {
     constexpr int W = L > 64 ? L / 64 : 1;
-    float* r = red + turn * (2 * W);
+    float* r = red + turn * 32;
     turn ^= 1;
+    const int wave = threadIdx.x >> 6, first = wave / W * W;
     if ((threadIdx.x & 63) == 0)
 #pragma unroll
-      for (int i = 0; i < N; ++i) r[(threadIdx.x >> 6) * 2 + i] = v[i];
+      for (int i = 0; i < N; ++i) r[wave * 2 + i] = v[i];
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       float s = 0.f;
 #pragma unroll
-      for (int w = 0; w < W; ++w) s += r[w * 2 + i];
+      for (int w = 0; w < W; ++w) s += r[(first + w) * 2 + i];
       v[i] = s;
     }
   }
@@ -135,11 +158,11 @@ template <int L> constexpr int threads_of() { return L < 256 ? 256 : L; }
 
 // Normalises the row in place: v -> vh; returns mean and 1 / deviation.  Two passes over the registers: the sum of squares is
 // taken around the mean, not as a difference of two large sums.
-template <int L, int NV>
+template <int L, int NV, bool LAYER>
 __device__ __forceinline__ void normalise(float (&v)[NV][V], const NormArgs& a, int lane, float& mean, float& r, float* red, int& turn) {
   const float inv = 1.f / (float)a.d.F;
   mean = 0.f;
-  if (a.d.norm == AGCN_NORM_LAYER) {
+  if (LAYER) {
     float s[1] = {0.f};
 #pragma unroll
     for (int k = 0; k < NV; ++k)
@@ -165,12 +188,11 @@ __device__ __forceinline__ void normalise(float (&v)[NV][V], const NormArgs& a, 
     for (int i = 0; i < V; ++i) v[k][i] *= r;
 }
 
-__device__ __forceinline__ void load_params(const NormArgs& a, int c, int F, float* s, float* w, float* b) {
+// eight parameters, or `none` where there are none
+__device__ __forceinline__ void load_param(const float* p, int c, int F, float none, float* v) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) { s[i] = 1.f; w[i] = 1.f; b[i] = 0.f; }
-  if (a.scale) load8(a.scale, c, F, s);
-  if (a.w) load8(a.w, c, F, w);
-  if (a.b) load8(a.b, c, F, b);
+  for (int i = 0; i < V; ++i) v[i] = none;
+  if (p) load8(p, c, F, v);
 }
 
 __device__ __forceinline__ bool is_pad(const NormArgs& a, int64_t row) {
@@ -179,74 +201,86 @@ __device__ __forceinline__ bool is_pad(const NormArgs& a, int64_t row) {
   return (int)row - a.row_off[g] >= a.n[g];
 }
 
-template <typename TX, typename TZ, int L, int NV>
+template <typename TX, typename TZ, int L, int NV, bool LAYER>
 __global__ __launch_bounds__(threads_of<L>()) void norm_forward_kernel(NormArgs a) {
   constexpr int R = threads_of<L>() / L;                    // rows side by side
-  __shared__ float red[4 * (L > 64 ? L / 64 : 1)];
+  __shared__ float red[64];
   const int lane = threadIdx.x % L, F = a.d.F;
   int turn = 0;
-  float w[NV][V], b[NV][V], w2[NV][V], b2[NV][V], s[NV][V];
+  // s w, s b, w', b': y = x + a(g) (zh sw + sb)
+  float sw[NV][V], sb[LAYER ? NV : 1][V], w2[NV][V], b2[LAYER ? NV : 1][V];
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
     const int c = (k * L + lane) * V;
+    float s[V];
+    load_param(a.scale, c, F, 1.f, s);
+    load_param(a.w, c, F, 1.f, sw[k]);
+    load_param(a.w2, c, F, 1.f, w2[k]);
+    if (LAYER) {
+      load_param(a.b, c, F, 0.f, sb[k]);
+      load_param(a.b2, c, F, 0.f, b2[k]);
+    }
 #pragma unroll
-    for (int i = 0; i < V; ++i) { w2[k][i] = 1.f; b2[k][i] = 0.f; }
-    load_params(a, c, F, s[k], w[k], b[k]);
-    if (a.w2) load8(a.w2, c, F, w2[k]);
-    if (a.b2) load8(a.b2, c, F, b2[k]);
+    for (int i = 0; i < V; ++i) {
+      sw[k][i] *= s[i];
+      if (LAYER) sb[k][i] *= s[i];
+    }
   }
   const int64_t step = (int64_t)gridDim.x * R;
-  // (the loop runs on the workgroup's first row: all its lanes meet at the barriers of row_sums)
-  for (int64_t r0 = (int64_t)blockIdx.x * R; r0 < a.d.rows; r0 += step) {
-    const int64_t row = r0 + threadIdx.x / L;
-    const bool live = row < a.d.rows, pad = live && is_pad(a, row);
-    float y[NV][V], zz[NV][V];
+  Raw<TX> nx[NV];
+  Raw<TZ> nz[NV], ng[NV];
+  bool nlive, nuse;
+  auto fetch = [&](int64_t row) {
+    nlive = row < a.d.rows;
+    nuse = nlive && !is_pad(a, row);
+    const int64_t grow = a.d.gate == AGCN_GATE_GRAPH ? (nlive ? a.row_graph[row] : 0) : row;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int c = (k * L + lane) * V;
-#pragma unroll
-      for (int i = 0; i < V; ++i) { y[k][i] = 0.f; zz[k][i] = 0.f; }
-      if (live && !pad) {
-        load8(static_cast<const TX*>(a.x) + row * a.d.ldx, c, F, y[k]);
-        if (a.z) load8(static_cast<const TZ*>(a.z) + row * a.d.ldz, c, F, zz[k]);
+      clear8(nx[k]); clear8(nz[k]); clear8(ng[k]);
+      if (nuse) {
+        fetch8(static_cast<const TX*>(a.x) + row * a.d.ldx, c, F, nx[k]);
+        if (a.z) fetch8(static_cast<const TZ*>(a.z) + row * a.d.ldz, c, F, nz[k]);
+        if (a.gate) fetch8(static_cast<const TZ*>(a.gate) + grow * a.d.ldg, c, F, ng[k]);
       }
     }
+  };
+  fetch((int64_t)blockIdx.x * R + threadIdx.x / L);
+  // (the loop runs on the workgroup's first row: all its lanes meet at the barriers of row_sums)
+  for (int64_t r0 = (int64_t)blockIdx.x * R; r0 < a.d.rows; r0 += step) {
+    const int64_t row = r0 + threadIdx.x / L;
+    const bool live = nlive, use = nuse;
+    float y[NV][V], zz[NV][V], g[NV][V];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      unpack8(nx[k], y[k]);
+      unpack8(nz[k], zz[k]);
+      unpack8(ng[k], g[k]);
+    }
+    fetch(row + step);
     float mz = 0.f, rz = 1.f, my = 0.f, ry = 1.f;
     if (a.z) {
-      if (a.w) normalise<L, NV>(zz, a, lane, mz, rz, red, turn);
-      const int64_t grow = a.d.gate == AGCN_GATE_GRAPH ? (live ? a.row_graph[row] : 0) : row;
+      if (a.w) normalise<L, NV, LAYER>(zz, a, lane, mz, rz, red, turn);
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
         const int c = (k * L + lane) * V;
-        float g[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) g[i] = 1.f;
-        if (a.gate && live && !pad) {
-          load8(static_cast<const TZ*>(a.gate) + grow * a.d.ldg, c, F, g);
-#pragma unroll
-          for (int i = 0; i < V; ++i) g[i] = gate_act(a.d.gate_activation, g[i]);
+        for (int i = 0; i < V; ++i) {
+          const float ga = a.gate ? gate_act(a.d.gate_activation, g[k][i]) : 1.f;
+          const float u = LAYER ? fmaf(zz[k][i], sw[k][i], sb[k][i]) : zz[k][i] * sw[k][i];
+          y[k][i] = c + i < F && use ? fmaf(ga, u, y[k][i]) : 0.f;
         }
-#pragma unroll
-        for (int i = 0; i < V; ++i) y[k][i] = fmaf(s[k][i] * g[i], fmaf(zz[k][i], w[k][i], b[k][i]), y[k][i]);
-        if (c + V > F)
-#pragma unroll
-          for (int i = 0; i < V; ++i) if (c + i >= F) y[k][i] = 0.f;
-        if (live) {
-          if (pad)
-#pragma unroll
-            for (int i = 0; i < V; ++i) y[k][i] = 0.f;
-          store8(static_cast<TX*>(a.y) + row * F, c, F, y[k]);
-        }
+        if (live) store8(static_cast<TX*>(a.y) + row * F, c, F, y[k]);
       }
     }
     if (a.h) {
-      normalise<L, NV>(y, a, lane, my, ry, red, turn);
+      normalise<L, NV, LAYER>(y, a, lane, my, ry, red, turn);
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
         const int c = (k * L + lane) * V;
         float o[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) o[i] = pad ? 0.f : fmaf(y[k][i], w2[k][i], b2[k][i]);
+        for (int i = 0; i < V; ++i) o[i] = !use ? 0.f : (LAYER ? fmaf(y[k][i], w2[k][i], b2[k][i]) : y[k][i] * w2[k][i]);
         if (live) store8(static_cast<TZ*>(a.h) + row * F, c, F, o);
       }
     }
@@ -254,90 +288,120 @@ __global__ __launch_bounds__(threads_of<L>()) void norm_forward_kernel(NormArgs 
   }
 }
 
-// One workgroup walks a strip of rows (no gate per graph: rows block, block + grid, ..; with one: up to kGraphRows rows of one
-// graph) and leaves the partial sums of its columns: q1, q2 (per graph: sum D zh, sum D), q3 = sum dh yh, q4 = sum dh.
+// One workgroup walks a strip of rows (no gate per graph: rows block, block + grid, ..; with one: up to graph_rows rows of one
+// graph) and leaves the partial sums of its columns: q1, q2 (per graph: sum D zh, sum D), q3 = sum dh yh, q4 = sum dh (q2 and q4
+// for the biases of layer norms alone).
 // y is formed again from x, z and the gate, which have to be read anyway (x in y's place): the stored y may be rounded to
 // bf16, and a row whose features differ by less than that rounding would get a wrong yh.
-template <typename TX, typename TZ, int L, int NV>
-__global__ __launch_bounds__(threads_of<L>(), 2) void norm_backward_kernel(NormArgs a) {
-  constexpr int T = threads_of<L>(), R = T / L;
-  __shared__ float red[4 * (L > 64 ? L / 64 : 1)];
+// AHEAD: the next row's operands are fetched while a row is worked on.  It pays where it costs few registers (bf16 rows, no gate, no
+// means: 32768 x 4096 463 -> AHEADUS us); with more it spills.
+template <typename TX, typename TZ, int L, int NV, bool LAYER, bool GATED>
+__global__ __launch_bounds__(threads_of<L>(), LAYER || GATED ? 3 : 4) void norm_backward_kernel(NormArgs a) {
+  constexpr bool AHEAD = !LAYER && !GATED && NV == 1 && sizeof(TX) == 2;
+  constexpr int T = threads_of<L>(), R = T / L, NL = LAYER ? NV : 1;
+  __shared__ float red[64];
   __shared__ float cols[R > 1 ? T * V : 1];
   const int lane = threadIdx.x % L, rl = threadIdx.x / L, F = a.d.F;
   int turn = 0;
   const float inv = 1.f / (float)F;
-  const bool per_graph = a.d.gate == AGCN_GATE_GRAPH, layer = a.d.norm == AGCN_NORM_LAYER;
+  const bool per_graph = GATED && a.d.gate == AGCN_GATE_GRAPH;
   int64_t row_begin, row_end, step;
   if (per_graph) {
     const int g = blockIdx.x / a.splits, sp = blockIdx.x - g * a.splits;
-    const int lo = sp * kGraphRows, all = a.row_off[g + 1] - a.row_off[g];   // pad rows too: their gradients are written (0)
+    const int lo = sp * a.graph_rows, all = a.row_off[g + 1] - a.row_off[g];   // pad rows too: their gradients are written (0)
     if (lo >= all) return;
     row_begin = a.row_off[g] + lo;
-    row_end = a.row_off[g] + (all < lo + kGraphRows ? all : lo + kGraphRows);
+    row_end = a.row_off[g] + (all < lo + a.graph_rows ? all : lo + a.graph_rows);
     step = R;
   } else {
     row_begin = (int64_t)blockIdx.x * R;
     row_end = a.d.rows;
     step = (int64_t)gridDim.x * R;
   }
-  float q1[NV][V], q2[NV][V], q3[NV][V], q4[NV][V];
+  float q1[NV][V], q2[NL][V], q3[NV][V], q4[NL][V];
 #pragma unroll
   for (int k = 0; k < NV; ++k)
 #pragma unroll
-    for (int i = 0; i < V; ++i) { q1[k][i] = 0.f; q2[k][i] = 0.f; q3[k][i] = 0.f; q4[k][i] = 0.f; }
-  for (int64_t r0 = row_begin; r0 < row_end; r0 += step) {
-    const int64_t row = r0 + rl;
-    const bool live = row < row_end, pad = live && is_pad(a, row), use = live && !pad;
-    f32x4 st = {0.f, 1.f, 0.f, 1.f};
-    if (use) st = *reinterpret_cast<const f32x4*>(a.stats + row * 4);
-    // D: the gradient of y (dx); yh: y, then normalised; zh; g: the gate before its activation
-    float D[NV][V], yh[NV][V], zh[NV][V], g[NV][V];
+    for (int i = 0; i < V; ++i) {
+      q1[k][i] = 0.f; q3[k][i] = 0.f;
+      if (LAYER) { q2[k][i] = 0.f; q4[k][i] = 0.f; }
+    }
+  Raw<TX> nx[NV], ny[NV];
+  Raw<TZ> nz[NV], ng[NV], nh[NV];
+  f32x4 nst;
+  bool nlive, nuse;
+  auto fetch = [&](int64_t row) {
+    nlive = row < row_end;
+    nuse = nlive && !is_pad(a, row);
+    nst = (f32x4){0.f, 1.f, 0.f, 1.f};
+    if (nuse) nst = *reinterpret_cast<const f32x4*>(a.stats + row * 4);
+    const int64_t grow = per_graph ? (nlive ? a.row_graph[row] : 0) : row;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int c = (k * L + lane) * V;
-#pragma unroll
-      for (int i = 0; i < V; ++i) { D[k][i] = 0.f; yh[k][i] = 0.f; zh[k][i] = 0.f; g[k][i] = 0.f; }
-      if (use) {
-        load8(static_cast<const TX*>(a.x) + row * a.d.ldx, c, F, yh[k]);
-        if (a.z) load8(static_cast<const TZ*>(a.z) + row * a.d.ldz, c, F, zh[k]);
-        if (a.dy) load8(static_cast<const TX*>(a.dy) + row * F, c, F, D[k]);
-        if (a.gate) {
-          load8(static_cast<const TZ*>(a.gate) + (per_graph ? (int64_t)a.row_graph[row] : row) * a.d.ldg, c, F, g[k]);
-        }
+      clear8(nx[k]); clear8(ny[k]); clear8(nz[k]); clear8(ng[k]); clear8(nh[k]);
+      if (nuse) {
+        fetch8(static_cast<const TX*>(a.x) + row * a.d.ldx, c, F, nx[k]);
+        if (a.z) fetch8(static_cast<const TZ*>(a.z) + row * a.d.ldz, c, F, nz[k]);
+        if (GATED) fetch8(static_cast<const TZ*>(a.gate) + grow * a.d.ldg, c, F, ng[k]);
+        if (a.dy) fetch8(static_cast<const TX*>(a.dy) + row * F, c, F, ny[k]);
+        if (a.dh) fetch8(static_cast<const TZ*>(a.dh) + row * F, c, F, nh[k]);
       }
+    }
+  };
+  if (AHEAD) fetch(row_begin + rl);
+  for (int64_t r0 = row_begin; r0 < row_end; r0 += step) {
+    const int64_t row = r0 + rl;
+    if (!AHEAD) fetch(row);
+    const bool live = nlive, use = nuse;
+    const f32x4 st = nst;
+    // D: the gradient of y (dx); e: dh, then times w'; yh: y, then normalised; zh; g: the gate before its activation
+    float D[NV][V], e[NV][V], yh[NV][V], zh[NV][V], g[NV][V];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      unpack8(nx[k], yh[k]);
+      unpack8(nz[k], zh[k]);
+      unpack8(ng[k], g[k]);
+      unpack8(ny[k], D[k]);
+      unpack8(nh[k], e[k]);
+    }
+    if (AHEAD) fetch(row + step);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int c = (k * L + lane) * V;
       if (a.z) {
         float s[V], w[V], b[V];
-        load_params(a, c, F, s, w, b);
+        load_param(a.scale, c, F, 1.f, s);
+        load_param(a.w, c, F, 1.f, w);
+        if (LAYER) load_param(a.b, c, F, 0.f, b);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          zh[k][i] = c + i < F && use ? (zh[k][i] - st.x) * st.y : 0.f;   // (no post norm: mean 0, deviation 1)
-          const float ga = a.gate ? gate_act(a.d.gate_activation, g[k][i]) : 1.f;
-          yh[k][i] = fmaf(s[i] * ga, fmaf(zh[k][i], w[i], b[i]), yh[k][i]);
+          zh[k][i] = c + i < F && use ? (LAYER ? zh[k][i] - st.x : zh[k][i]) * st.y : 0.f;   // (no post norm: mean 0, deviation 1)
+          const float ga = GATED ? gate_act(a.d.gate_activation, g[k][i]) : 1.f;
+          const float sw = s[i] * w[i], u = LAYER ? fmaf(zh[k][i], sw, s[i] * b[i]) : zh[k][i] * sw;
+          yh[k][i] = fmaf(ga, u, yh[k][i]);
         }
       }
     }
     if (a.dh) {
-      float e[NV][V], m[2] = {0.f, 0.f};
+      float m[2] = {0.f, 0.f};
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
         const int c = (k * L + lane) * V;
         float w2[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) e[k][i] = 0.f;
-        if (use) load8(static_cast<const TZ*>(a.dh) + row * F, c, F, e[k]);
         load8(a.w2, c, F, w2);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          yh[k][i] = c + i < F && use ? (yh[k][i] - st.z) * st.w : 0.f;
+          yh[k][i] = c + i < F && use ? (LAYER ? yh[k][i] - st.z : yh[k][i]) * st.w : 0.f;
           q3[k][i] = fmaf(e[k][i], yh[k][i], q3[k][i]);
-          q4[k][i] += e[k][i];
+          if (LAYER) q4[k][i] += e[k][i];
           e[k][i] *= w2[i];
           m[0] = fmaf(e[k][i], yh[k][i], m[0]);
-          m[1] += e[k][i];
+          if (LAYER) m[1] += e[k][i];
         }
       }
-      row_sums<L, 2>(m, red, turn);
-      const float m0 = m[0] * inv, m1 = layer ? m[1] * inv : 0.f;
+      row_sums<L, LAYER ? 2 : 1>(reinterpret_cast<float(&)[LAYER ? 2 : 1]>(m), red, turn);
+      const float m0 = m[0] * inv, m1 = LAYER ? m[1] * inv : 0.f;
 #pragma unroll
       for (int k = 0; k < NV; ++k)
 #pragma unroll
@@ -356,25 +420,28 @@ __global__ __launch_bounds__(threads_of<L>(), 2) void norm_backward_kernel(NormA
       for (int k = 0; k < NV; ++k) {
         const int c = (k * L + lane) * V;
         float s[V], w[V], b[V], dg[V];
-        load_params(a, c, F, s, w, b);
+        load_param(a.scale, c, F, 1.f, s);
+        load_param(a.w, c, F, 1.f, w);
+        if (LAYER) load_param(a.b, c, F, 0.f, b);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          const float ga = a.gate ? gate_act(a.d.gate_activation, g[k][i]) : 1.f;
+          const float ga = GATED ? gate_act(a.d.gate_activation, g[k][i]) : 1.f;
           const float Dq = per_graph ? D[k][i] : D[k][i] * ga;
           q1[k][i] = fmaf(Dq, zh[k][i], q1[k][i]);
-          q2[k][i] += Dq;
-          dg[i] = a.gate ? D[k][i] * s[i] * fmaf(zh[k][i], w[i], b[i]) * gate_slope(a.d.gate_activation, g[k][i]) : 0.f;
-          D[k][i] *= s[i] * ga * w[i];                           // gradient of zh
+          if (LAYER) q2[k][i] += Dq;
+          const float u = LAYER ? fmaf(zh[k][i], w[i], b[i]) : zh[k][i] * w[i];
+          dg[i] = GATED ? D[k][i] * s[i] * u * gate_slope(a.d.gate_activation, g[k][i]) : 0.f;
+          D[k][i] *= s[i] * ga * w[i];                                 // gradient of zh
           m[0] = fmaf(D[k][i], zh[k][i], m[0]);
-          m[1] += D[k][i];
+          if (LAYER) m[1] += D[k][i];
         }
-        if (a.d.gate == AGCN_GATE_ROW && live) store8(static_cast<TZ*>(a.dgate) + row * F, c, F, dg);
+        if (GATED && a.d.gate == AGCN_GATE_ROW && live) store8(static_cast<TZ*>(a.dgate) + row * F, c, F, dg);
       }
       float m0 = 0.f, m1 = 0.f;
       if (a.w) {
-        row_sums<L, 2>(m, red, turn);
+        row_sums<L, LAYER ? 2 : 1>(reinterpret_cast<float(&)[LAYER ? 2 : 1]>(m), red, turn);
         m0 = m[0] * inv;
-        m1 = layer ? m[1] * inv : 0.f;
+        m1 = LAYER ? m[1] * inv : 0.f;
       }
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
@@ -390,14 +457,14 @@ __global__ __launch_bounds__(threads_of<L>(), 2) void norm_backward_kernel(NormA
   float* part = a.part + (int64_t)blockIdx.x * 4 * F;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    if ((j < 2 && !a.z) || (j >= 2 && !a.dh)) continue;
-    float(&q)[NV][V] = j == 0 ? q1 : j == 1 ? q2 : j == 2 ? q3 : q4;
+    if ((j < 2 && !a.z) || (j >= 2 && !a.dh) || (!LAYER && (j & 1))) continue;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
+      const float* q = j == 0 ? q1[k] : j == 1 ? q2[LAYER ? k : 0] : j == 2 ? q3[k] : q4[LAYER ? k : 0];
       if (R > 1) {
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < V; ++i) cols[(rl * L + lane) * V + i] = q[k][i];
+        for (int i = 0; i < V; ++i) cols[(rl * L + lane) * V + i] = q[i];
         __syncthreads();
         for (int e = threadIdx.x; e < L * V; e += T) {
           float sum = 0.f;
@@ -405,7 +472,7 @@ __global__ __launch_bounds__(threads_of<L>(), 2) void norm_backward_kernel(NormA
           if (k * L * V + e < F) part[(int64_t)j * F + k * L * V + e] = sum;
         }
       } else {
-        store8(part + (int64_t)j * F, (k * L + lane) * V, F, q[k]);
+        store8(part + (int64_t)j * F, (k * L + lane) * V, F, q);
       }
     }
   }
@@ -416,40 +483,52 @@ struct ReduceArgs {
   float *dscale, *dw, *db, *dw2, *db2;
 };
 
-// Adds the workgroups' partial column sums (64 columns per workgroup, 16 row lanes, then those in order) and forms the
-// parameters' gradients.
+// Adds the partial column sums (sixteen columns per workgroup, 64 row lanes that add theirs in order, then the lanes' sums in
+// order) and forms the parameters' gradients.
+template <bool Z, bool H, bool TWO>
+__device__ __forceinline__ void add_parts(const float* t, int u0, int units, int64_t step, int F, float (&q)[4]) {
+#pragma unroll 4
+  for (int u = u0; u < units; u += 64) {       // (no branch inside: the loads of four turns fly together)
+    const float* x = t + u * step;
+    if (Z) q[0] += x[0];
+    if (Z && TWO) q[1] += x[F];
+    if (H) q[2] += x[2 * F];
+    if (H && TWO) q[3] += x[3 * F];
+  }
+}
 __global__ __launch_bounds__(1024) void norm_params_kernel(ReduceArgs p) {
-  __shared__ float s[4][16][64];
+  __shared__ float s[4][64][17];
   const NormArgs& a = p.a;
-  const int F = a.d.F, cl = threadIdx.x & 63, rl = threadIdx.x >> 6, c = blockIdx.x * 64 + cl;
+  const int F = a.d.F, cl = threadIdx.x & 15, rl = threadIdx.x >> 4, c = blockIdx.x * 16 + cl;
+  const bool two = a.d.norm == AGCN_NORM_LAYER;
   float q[4] = {0.f, 0.f, 0.f, 0.f};
   if (c < F) {
-    const bool per_graph = a.d.gate == AGCN_GATE_GRAPH;
-    for (int u = rl; u < a.units; u += 16) {
-      float f = 1.f;
-      if (per_graph) {
-        const int g = u / a.splits, sp = u - g * a.splits;
-        if (sp * kGraphRows >= a.row_off[g + 1] - a.row_off[g]) continue;
-        const int64_t at = (int64_t)g * a.d.ldg + c;
-        const float gv = a.d.z_dtype == AGCN_DTYPE_BF16
-                             ? __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(a.gate)[at] << 16)
-                             : static_cast<const float*>(a.gate)[at];
-        f = gate_act(a.d.gate_activation, gv);
-      }
-      const float* t = a.part + (int64_t)u * 4 * F + c;
-      if (a.z) { q[0] = fmaf(f, t[0], q[0]); q[1] = fmaf(f, t[F], q[1]); }
-      if (a.dh) { q[2] += t[2 * (int64_t)F]; q[3] += t[3 * (int64_t)F]; }
-    }
+    const int64_t step = (int64_t)a.stride * 4 * F;
+    const float* t = a.part + c;
+    if (a.z && a.dh && two) add_parts<true, true, true>(t, rl, a.units, step, F, q);
+    else if (a.z && a.dh) add_parts<true, true, false>(t, rl, a.units, step, F, q);
+    else if (a.z && two) add_parts<true, false, true>(t, rl, a.units, step, F, q);
+    else if (a.z) add_parts<true, false, false>(t, rl, a.units, step, F, q);
+    else if (two) add_parts<false, true, true>(t, rl, a.units, step, F, q);
+    else add_parts<false, true, false>(t, rl, a.units, step, F, q);
   }
 #pragma unroll
   for (int j = 0; j < 4; ++j) s[j][rl][cl] = q[j];
   __syncthreads();
-  if (rl || c >= F) return;
+  // one wave per sum: four lanes of a column add sixteen rows each
+  if (threadIdx.x >= 256) return;
+  const int j = threadIdx.x >> 6, part = (threadIdx.x >> 4) & 3;
+  float v = 0.f;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    q[j] = 0.f;
-    for (int r = 0; r < 16; ++r) q[j] += s[j][r][cl];
-  }
+  for (int r = 0; r < 16; ++r) v += s[j][part * 16 + r][cl];
+  v += __shfl_xor(v, 16);
+  v += __shfl_xor(v, 32);
+  __syncthreads();
+  if (part == 0) s[j][0][cl] = v;
+  __syncthreads();
+  if (threadIdx.x >= 16 || c >= F) return;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) q[k] = s[k][0][cl];
   const float sc = a.scale ? a.scale[c] : 1.f, w = a.w ? a.w[c] : 1.f, b = a.b ? a.b[c] : 0.f;
   if (p.dscale) p.dscale[c] = fmaf(w, q[0], b * q[1]);
   if (p.dw) p.dw[c] = sc * q[0];
@@ -458,60 +537,77 @@ __global__ __launch_bounds__(1024) void norm_params_kernel(ReduceArgs p) {
   if (p.db2) p.db2[c] = q[3];
 }
 
-// dg[graph] = a'(g) s (w sum D zh + b sum D): one thread per graph and column
-__global__ __launch_bounds__(256) void norm_graph_gate_kernel(NormArgs a) {
-  const int F = a.d.F, g = blockIdx.x, c = blockIdx.y * 256 + threadIdx.x;
+// A gate per graph: dg[graph] = a'(g) s (w sum D zh + b sum D), one thread per graph and column; and the graph's sums for the
+// parameters (those over z times a(g)), left in the place of its first partial.
+__global__ __launch_bounds__(64) void norm_graph_gate_kernel(NormArgs a) {
+  const int F = a.d.F, g = blockIdx.x, c = blockIdx.y * 64 + threadIdx.x;
   if (c >= F) return;
-  const int all = a.row_off[g + 1] - a.row_off[g];
-  float q1 = 0.f, q2 = 0.f;
-  for (int sp = 0; sp * kGraphRows < all; ++sp) {
-    const float* t = a.part + ((int64_t)g * a.splits + sp) * 4 * F + c;
-    q1 += t[0];
-    q2 += t[F];
+  const int n = (a.row_off[g + 1] - a.row_off[g] + a.graph_rows - 1) / a.graph_rows;
+  const bool two = a.d.norm == AGCN_NORM_LAYER;
+  float* first = a.part + (int64_t)g * a.splits * 4 * F + c;
+  float q[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int sp = 0; sp < n; ++sp) {
+    const float* t = first + (int64_t)sp * 4 * F;
+    q[0] += t[0];
+    if (two) q[1] += t[F];
+    if (a.dh) {
+      q[2] += t[2 * (int64_t)F];
+      if (two) q[3] += t[3 * (int64_t)F];
+    }
   }
   const bool bf = a.d.z_dtype == AGCN_DTYPE_BF16;
   const int64_t at = (int64_t)g * a.d.ldg + c;
   const float gv = bf ? __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(a.gate)[at] << 16) : static_cast<const float*>(a.gate)[at];
-  const float da = gate_slope(a.d.gate_activation, gv);
+  const float ga = gate_act(a.d.gate_activation, gv), da = gate_slope(a.d.gate_activation, gv);
   const float sc = a.scale ? a.scale[c] : 1.f, w = a.w ? a.w[c] : 1.f, b = a.b ? a.b[c] : 0.f;
-  const float o = da * sc * fmaf(w, q1, b * q2);
+  const float o = da * sc * fmaf(w, q[0], b * q[1]);
   if (bf) reinterpret_cast<uint16_t*>(a.dgate)[(int64_t)g * F + c] = (uint16_t)pk_bf(o, 0.f);
   else static_cast<float*>(a.dgate)[(int64_t)g * F + c] = o;
+  first[0] = ga * q[0];
+  if (two) first[F] = ga * q[1];
+  if (a.dh) {
+    first[2 * (int64_t)F] = q[2];
+    if (two) first[3 * (int64_t)F] = q[3];
+  }
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------------
 
-// lanes per row and vectors per lane for a width: the fewest lanes that hold the row in one vector each, then two
+// lanes per row and vectors per lane for a width: the fewest lanes that hold the row in one vector each (two beyond 8192)
 struct Shape { int L, NV; };
 Shape shape_for(int F) {
   const int vecs = (F + V - 1) / V;
-  if (vecs <= 8) return {8, 1};
-  if (vecs <= 16) return {16, 1};
-  if (vecs <= 32) return {32, 1};
-  if (vecs <= 64) return {64, 1};
-  if (vecs <= 128) return {64, 2};
-  if (vecs <= 256) return {256, 1};
-  if (vecs <= 512) return {256, 2};
-  if (vecs <= 1024) return {512, 2};
+  for (int L = 16; L <= 1024; L *= 2)
+    if (vecs <= L) return {L, 1};
   return {1024, 2};
 }
 
 template <typename TX, typename TZ, int L, int NV>
 void launch_one(bool back, const NormArgs& a, int grid, hipStream_t s) {
-  if (back) hipLaunchKernelGGL((norm_backward_kernel<TX, TZ, L, NV>), dim3(grid), dim3(threads_of<L>()), 0, s, a);
-  else hipLaunchKernelGGL((norm_forward_kernel<TX, TZ, L, NV>), dim3(grid), dim3(threads_of<L>()), 0, s, a);
+  const dim3 g(grid), t(threads_of<L>());
+  const bool layer = a.d.norm == AGCN_NORM_LAYER;
+  if (!back) {
+    if (layer) hipLaunchKernelGGL((norm_forward_kernel<TX, TZ, L, NV, true>), g, t, 0, s, a);
+    else hipLaunchKernelGGL((norm_forward_kernel<TX, TZ, L, NV, false>), g, t, 0, s, a);
+  } else if (a.gate) {
+    if (layer) hipLaunchKernelGGL((norm_backward_kernel<TX, TZ, L, NV, true, true>), g, t, 0, s, a);
+    else hipLaunchKernelGGL((norm_backward_kernel<TX, TZ, L, NV, false, true>), g, t, 0, s, a);
+  } else {
+    if (layer) hipLaunchKernelGGL((norm_backward_kernel<TX, TZ, L, NV, true, false>), g, t, 0, s, a);
+    else hipLaunchKernelGGL((norm_backward_kernel<TX, TZ, L, NV, false, false>), g, t, 0, s, a);
+  }
 }
 template <typename TX, typename TZ>
 void launch_shape(bool back, const NormArgs& a, Shape sh, int grid, hipStream_t s) {
-  if (sh.L == 8) launch_one<TX, TZ, 8, 1>(back, a, grid, s);
+  if (sh.NV == 2) launch_one<TX, TZ, 1024, 2>(back, a, grid, s);
   else if (sh.L == 16) launch_one<TX, TZ, 16, 1>(back, a, grid, s);
   else if (sh.L == 32) launch_one<TX, TZ, 32, 1>(back, a, grid, s);
-  else if (sh.L == 64 && sh.NV == 1) launch_one<TX, TZ, 64, 1>(back, a, grid, s);
-  else if (sh.L == 64) launch_one<TX, TZ, 64, 2>(back, a, grid, s);
-  else if (sh.L == 256 && sh.NV == 1) launch_one<TX, TZ, 256, 1>(back, a, grid, s);
-  else if (sh.L == 256) launch_one<TX, TZ, 256, 2>(back, a, grid, s);
-  else if (sh.L == 512) launch_one<TX, TZ, 512, 2>(back, a, grid, s);
-  else launch_one<TX, TZ, 1024, 2>(back, a, grid, s);
+  else if (sh.L == 64) launch_one<TX, TZ, 64, 1>(back, a, grid, s);
+  else if (sh.L == 128) launch_one<TX, TZ, 128, 1>(back, a, grid, s);
+  else if (sh.L == 256) launch_one<TX, TZ, 256, 1>(back, a, grid, s);
+  else if (sh.L == 512) launch_one<TX, TZ, 512, 1>(back, a, grid, s);
+  else launch_one<TX, TZ, 1024, 1>(back, a, grid, s);
 }
 void launch(bool back, const NormArgs& a, Shape sh, int grid, hipStream_t s) {
   if (a.d.x_dtype == AGCN_DTYPE_F32 && a.d.z_dtype == AGCN_DTYPE_F32) launch_shape<float, float>(back, a, sh, grid, s);
@@ -519,10 +615,11 @@ void launch(bool back, const NormArgs& a, Shape sh, int grid, hipStream_t s) {
   else launch_shape<__hip_bfloat16, __hip_bfloat16>(back, a, sh, grid, s);
 }
 
-// workgroups that walk the rows: as many as the rows ask for, up to four (forward) / two (backward) of 256 threads per CU
+int rows_at_once(Shape sh) { return sh.L < 256 ? 256 / sh.L : 1; }
+// workgroups that walk the rows: as many as the rows ask for, up to what the chip holds (2048 threads per CU forward, 1024 backward)
 int row_grid(const AgcnNormDesc& d, Shape sh, bool back) {
-  const int T = sh.L < 256 ? 256 : sh.L, R = T / sh.L;
-  const int64_t want = (d.rows + R - 1) / R, cap = (int64_t)256 * (T > 256 ? 1024 / T : (back ? 2 : 4));
+  const int T = sh.L < 256 ? 256 : sh.L;
+  const int64_t want = (d.rows + rows_at_once(sh) - 1) / rows_at_once(sh), cap = (int64_t)256 * (back ? 1024 : 2048) / T;
   return (int)std::max<int64_t>(1, std::min(want, cap));
 }
 
@@ -552,7 +649,11 @@ int check_norm(const AgcnNormDesc* d, const void* plan_host, const void* plan_de
     a->pads = host.info.rows != host.info.N1;
     int32_t most = 0;                       // rows of the largest graph, its pad rows counted
     for (int32_t g = 0; g < host.info.B; ++g) most = std::max(most, host.row_off[g + 1] - host.row_off[g]);
-    a->splits = (most + kGraphRows - 1) / kGraphRows;
+    // rows of a graph per workgroup: few enough for a thousand workgroups, up to 64 (each leaves four sums per column)
+    const int R = rows_at_once(shape_for(d->F));
+    a->graph_rows = R;
+    while (a->graph_rows < 64 && d->rows / a->graph_rows > 1024) a->graph_rows *= 2;
+    a->splits = (most + a->graph_rows - 1) / a->graph_rows;
   } else if (d->gate == AGCN_GATE_GRAPH) {
     return fail(AGCN_EINVAL, "%s: a gate per graph needs a plan", who);
   }
@@ -633,10 +734,14 @@ extern "C" int agcn_norm_gate_residual_backward(const AgcnNormDesc* desc, const 
   p.a = a;
   p.dscale = grads->dscale; p.dw = grads->dpost_weight; p.db = grads->dpost_bias;
   p.dw2 = grads->dpre_weight; p.db2 = grads->dpre_bias;
+  p.a.stride = 1;
+  if (a.d.gate == AGCN_GATE_GRAPH) {
+    hipLaunchKernelGGL(norm_graph_gate_kernel, dim3(a.B, (a.d.F + 63) / 64), dim3(64), 0, s, a);
+    p.a.units = a.B;
+    p.a.stride = a.splits;
+  }
   if (p.dscale || p.dw || p.db || p.dw2 || p.db2)
-    hipLaunchKernelGGL(norm_params_kernel, dim3((a.d.F + 63) / 64), dim3(1024), 0, s, p);
-  if (a.d.gate == AGCN_GATE_GRAPH)
-    hipLaunchKernelGGL(norm_graph_gate_kernel, dim3(a.B, (a.d.F + 255) / 256), dim3(256), 0, s, a);
+    hipLaunchKernelGGL(norm_params_kernel, dim3((a.d.F + 15) / 16), dim3(1024), 0, s, p);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return fail(AGCN_EDEVICE, "%s: %s", who, hipGetErrorString(e));
   return AGCN_OK;

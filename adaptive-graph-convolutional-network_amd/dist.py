@@ -8,7 +8,7 @@ Consequence for callers: anything that divides by the batch size -- `MultitaskHe
 loss scale -- must be given the GLOBAL batch size (per-rank graphs x world size) on every rank; the SGC layers
 themselves are built with the LOCAL graph count (it is the length of their output lists).  `global_batch_size()`
 returns the number to use."""
-import ctypes as C
+from array import array
 
 import numpy as np
 import torch
@@ -88,29 +88,40 @@ def flatten_grads(tensors):
 
 
 _CLIP_DT = {torch.float32: 0, torch.bfloat16: 1}
+_T = torch.Tensor
 
 
-def _clip(tensors, clip_norm, out):
+def _each(method, ts):
+    return list(map(method, ts))
+
+
+def _clip(ts, clip_norm, out):
+    """(lists of a hundred tensors and more: every step below is one pass in C over the list)"""
     lib = _ffi.lib()
-    dev = tensors[0].device
-    if dev.type != "cuda":
-        raise _ffi.AgcnError("gradients must live on the GPU: the clipping kernels have no CPU fallback")
-    if any(t.device != dev for t in tensors):
+    where = _each(_T.get_device, ts)
+    if min(where) != max(where):
         raise ValueError("all gradients must be on one device")
-    n = len(tensors)
+    if where[0] < 0:
+        raise _ffi.AgcnError("gradients must live on the GPU: the clipping kernels have no CPU fallback")
+    n = len(ts)
     try:
-        dtype = (C.c_int32 * n)(*[_CLIP_DT[t.dtype] for t in tensors])
+        dtype = array("i", [_CLIP_DT[t.dtype] for t in ts])
     except KeyError:
         raise TypeError("gradients must be float32 or bfloat16")
-    numel = (C.c_int64 * n)(*[t.numel() for t in tensors])
-    ptr_in = (C.c_void_p * n)(*[t.data_ptr() for t in tensors])
-    ptr_out = None if out is None else (C.c_void_p * n)(*[t.data_ptr() for t in out])
+    numel = array("q", map(_T.numel, ts))
+    ins = array("Q", map(_T.data_ptr, ts))
+    outs = None
+    if out is not None:
+        outs = ins if out is ts else array("Q", map(_T.data_ptr, out))
+    dev = ts[0].device
     with torch.cuda.device(dev):
         norm = torch.empty((), dtype=torch.float32, device=dev)
-        wbytes = lib.agcn_clip_workspace_bytes(n, numel, dtype)
+        ln, ld = numel.buffer_info()[0], dtype.buffer_info()[0]
+        wbytes = lib.agcn_clip_workspace_bytes(n, ln, ld)
         ws = torch.empty(wbytes, dtype=torch.uint8, device=dev)
-        _ffi.check(lib.agcn_clip_by_global_norm(n, ptr_in, ptr_out, numel, dtype, clip_norm, norm.data_ptr(), ws.data_ptr(),
-                                                wbytes, torch.cuda.current_stream(dev).cuda_stream))
+        _ffi.check(lib.agcn_clip_by_global_norm(n, ins.buffer_info()[0], None if outs is None else outs.buffer_info()[0], ln, ld,
+                                                clip_norm, norm.data_ptr(), ws.data_ptr(), wbytes,
+                                                torch._C._cuda_getCurrentRawStream(where[0])))
     return norm
 
 
@@ -127,35 +138,41 @@ def clip_by_global_norm(tensors, clip_norm, out=None):
     """Scales a list of gradient tensors (float32 or bfloat16, one device) so that their global norm is at most `clip_norm`:
     out_t = t * clip_norm / max(norm, clip_norm).  Returns (list of clipped tensors, norm before clipping as a 0-dim device tensor);
     nothing synchronises.  None entries stay None.  A norm that is not finite makes every result NaN (the reference's framework
-    does the same: a broken step is seen, not applied).  out: contiguous tensors of the same shapes and types to write to;
+    does the same: a broken step is seen, not applied).  out: contiguous tensors of the same sizes and types to write to;
     `out=tensors` clips in place."""
-    tensors = list(tensors)
     clip_norm = float(clip_norm)
     if not clip_norm > 0.0:
         raise ValueError("clip_norm must be positive")
+    given, tensors = tensors, list(tensors)
+    out = None if out is None else (tensors if out is given else list(out))
+    if out is not None and len(out) != len(tensors):
+        raise ValueError("out must hold one tensor per gradient (%d), got %d" % (len(tensors), len(out)))
     at = [i for i, t in enumerate(tensors) if t is not None]
     if not at:
         raise ValueError("no tensors")
-    given = [tensors[i] for i in at]
-    ts = [t if t.is_contiguous() else t.contiguous() for t in given]
+    whole = len(at) == len(tensors)
+    ts = tensors if whole else [tensors[i] for i in at]
+    if not all(map(_T.is_contiguous, ts)):
+        ts = [t.contiguous() for t in ts]
     if out is None:
         os_ = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in ts]
     else:
-        out = list(out)
-        if len(out) != len(tensors):
-            raise ValueError("out must hold one tensor per gradient (%d), got %d" % (len(tensors), len(out)))
-        os_ = [out[i] for i in at]
-        for t, o in zip(ts, os_):
-            if o is None or o.shape != t.shape or o.dtype != t.dtype or o.device != t.device or not o.is_contiguous():
-                raise ValueError("out must hold contiguous tensors of the gradients' shapes, types and device")
+        os_ = out if whole else [out[i] for i in at]
+        if any(o is None for o in os_):
+            raise ValueError("out must hold a tensor for every gradient")
+        if (not all(map(_T.is_contiguous, os_)) or _each(_T.numel, os_) != _each(_T.numel, ts) or
+                [o.dtype for o in os_] != [t.dtype for t in ts] or _each(_T.get_device, os_) != _each(_T.get_device, ts)):
+            raise ValueError("out must hold contiguous tensors of the gradients' sizes, types and device")
     norm = _clip(ts, clip_norm, os_)
-    if out is not None:
-        for o in os_:
-            torch.autograd.graph.increment_version(o)      # (written behind torch's back: a saved copy of it is stale)
-    res = list(tensors)
-    for i, o in zip(at, os_):
-        res[i] = o
-    return res, norm
+    if out is None:
+        if whole:
+            return os_, norm
+        out = list(tensors)
+        for i, o in zip(at, os_):
+            out[i] = o
+        return out, norm
+    torch.autograd.graph.increment_version(os_)            # (written behind torch's back: a saved copy of them is stale)
+    return out, norm
 
 
 class GradBucket(object):

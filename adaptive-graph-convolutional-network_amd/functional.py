@@ -15,7 +15,8 @@ def _ptr(t):
 
 
 def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+    # (what torch.cuda.current_stream(device).cuda_stream returns, without the stream object: 0.1 instead of 1.9 us)
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if device.index is None else device.index)
 
 
 def _on_tensor_device(fn):
@@ -765,102 +766,128 @@ def _ld(t):
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _vector(t, what, F, device):
+def _vector(t, what, F, like):
+    """`t` as a contiguous float32 vector of F elements on the device of `like`."""
     if t is None:
         return None
+    if t.dtype is torch.float32 and t.shape == (F,) and t.get_device() == like.get_device() and t.is_contiguous():
+        return t
     _require_gpu(t, what)
     t = _f32c(t, what)
-    if tuple(t.shape) != (F,):
+    if t.shape != (F,):
         raise ValueError("%s must be [%d], got %s" % (what, F, tuple(t.shape)))
-    if t.device != device:
-        raise ValueError("%s is on %s, the rows are on %s" % (what, t.device, device))
+    if t.device != like.device:
+        raise ValueError("%s is on %s, the rows are on %s" % (what, t.device, like.device))
     return t
+
+
+def _wants_grad(tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _on_device_of(t, fn, *args):
+    """fn(*args) with the device of `t` made current (see _on_tensor_device)."""
+    i = t.get_device()
+    if i < 0 or i == torch.cuda.current_device():
+        return fn(*args)
+    with torch.cuda.device(i):
+        return fn(*args)
+
+
+def _norm_forward(z, x, gate, scale, post_weight, post_bias, pre_weight, pre_bias, plan, norm, eps, gate_activation, keep):
+    """-> (y, h, what a backward needs: the tensors as the kernel read them, its row statistics, the descriptor)"""
+    x = _row_matrix(x, "residual rows")
+    rows, F = x.shape
+    dev = x.device
+    if plan is not None:
+        if plan.dev is None or plan.dev.get_device() != x.get_device():
+            raise ValueError("the plan is not on the rows' device")
+        if plan.rows != rows:
+            raise ValueError("the rows are %d, the plan has %d" % (rows, plan.rows))
+    kind = 0
+    if z is not None:
+        z = _row_matrix(z, "block output", F)
+        if z.get_device() != x.get_device():
+            raise ValueError("block output is on %s, the rows are on %s" % (z.device, dev))
+        if z.shape[0] != rows:
+            raise ValueError("block output and residual rows differ in length (%d, %d)" % (z.shape[0], rows))
+        if x.dtype is torch.bfloat16 and z.dtype is not torch.bfloat16:
+            raise TypeError("bfloat16 residual rows need a bfloat16 block output")
+    if gate is not None:
+        if z is None:
+            raise ValueError("a gate needs a block output")
+        if gate.dtype is not z.dtype:
+            raise TypeError("gate and block output must have one type")
+        gate = _row_matrix(gate, "gate", F)
+        if gate.get_device() != x.get_device():
+            raise ValueError("gate is on %s, the rows are on %s" % (gate.device, dev))
+        if plan is not None and gate.shape[0] == plan.B:
+            kind = 2
+        elif gate.shape[0] == rows:
+            kind = 1
+        else:
+            raise ValueError("gate must have one row per row (%d)%s, got %d" %
+                             (rows, "" if plan is None else " or one per graph (%d)" % plan.B, gate.shape[0]))
+    scale = _vector(scale, "scale", F, x)
+    post_weight, post_bias = _vector(post_weight, "post_weight", F, x), _vector(post_bias, "post_bias", F, x)
+    pre_weight, pre_bias = _vector(pre_weight, "pre_weight", F, x), _vector(pre_bias, "pre_bias", F, x)
+    zt = x.dtype if z is None else z.dtype
+    desc = _ffi.NormDesc(rows, F, _ffi.NORM[norm], kind, _ffi.GATE_ACT[gate_activation], _DT[x.dtype], _DT[zt], _ld(x),
+                         0 if z is None else _ld(z), 0 if gate is None else _ld(gate), eps)
+    inputs = _ffi.NormInputs(_rows_ptr(z), _rows_ptr(x), _rows_ptr(gate), _ptr(scale), _ptr(post_weight), _ptr(post_bias),
+                             _ptr(pre_weight), _ptr(pre_bias))
+    y = torch.empty((rows, F), dtype=x.dtype, device=dev) if z is not None else None
+    h = torch.empty((rows, F), dtype=zt, device=dev) if pre_weight is not None else None
+    stats = torch.empty((rows, 4), dtype=torch.float32, device=dev) if keep else None
+    host, devp = (None, None) if plan is None else (plan.host_ptr, plan.dev_ptr)
+    _ffi.check(_ffi.lib().agcn_norm_gate_residual_forward(C.byref(desc), host, devp, C.byref(inputs), _rows_ptr(y), _rows_ptr(h),
+                                                          _ptr(stats), _stream(dev)))
+    return y, h, (z, x, gate, scale, post_weight, post_bias, pre_weight, pre_bias, stats), desc
 
 
 class NormGateResidualFunction(torch.autograd.Function):
     """(y, h) = (x + scale * a(gate) * N(z), N'(y)); see norm_gate_residual."""
 
     @staticmethod
-    @_on_tensor_device
     def forward(ctx, z, x, gate, scale, post_weight, post_bias, pre_weight, pre_bias, plan, norm, eps, gate_activation):
-        lib = _ffi.lib()
-        x = _row_matrix(x, "residual rows")
-        rows, F = x.shape
-        dev = x.device
-        for t, what in ((z, "block output"), (gate, "gate")):
-            if t is not None and t.device != dev:
-                raise ValueError("%s is on %s, the rows are on %s" % (what, t.device, dev))
-        if plan is not None:
-            if plan.dev is None or plan.dev.device != dev:
-                raise ValueError("the plan is not on the rows' device")
-            if plan.rows != rows:
-                raise ValueError("the rows are %d, the plan has %d" % (rows, plan.rows))
-        kind = 0
-        if z is not None:
-            z = _row_matrix(z, "block output", F)
-            if z.shape[0] != rows:
-                raise ValueError("block output and residual rows differ in length (%d, %d)" % (z.shape[0], rows))
-            if x.dtype == torch.bfloat16 and z.dtype != torch.bfloat16:
-                raise TypeError("bfloat16 residual rows need a bfloat16 block output")
-        if gate is not None:
-            if z is None:
-                raise ValueError("a gate needs a block output")
-            if gate.dtype != z.dtype:
-                raise TypeError("gate and block output must have one type")
-            gate = _row_matrix(gate, "gate", F)
-            if plan is not None and gate.shape[0] == plan.B:
-                kind = 2
-            elif gate.shape[0] == rows:
-                kind = 1
-            else:
-                raise ValueError("gate must have one row per row (%d)%s, got %d" %
-                                 (rows, "" if plan is None else " or one per graph (%d)" % plan.B, gate.shape[0]))
-        scale = _vector(scale, "scale", F, dev)
-        post_weight, post_bias = _vector(post_weight, "post_weight", F, dev), _vector(post_bias, "post_bias", F, dev)
-        pre_weight, pre_bias = _vector(pre_weight, "pre_weight", F, dev), _vector(pre_bias, "pre_bias", F, dev)
-        zt = x.dtype if z is None else z.dtype
-        desc = _ffi.NormDesc(rows, F, _ffi.NORM[norm], kind, _ffi.GATE_ACT[gate_activation], _DT[x.dtype], _DT[zt], _ld(x),
-                             0 if z is None else _ld(z), 0 if gate is None else _ld(gate), eps)
-        inputs = _ffi.NormInputs(_rows_ptr(z), _rows_ptr(x), _rows_ptr(gate), _ptr(scale), _ptr(post_weight), _ptr(post_bias),
-                                 _ptr(pre_weight), _ptr(pre_bias))
-        y = torch.empty((rows, F), dtype=x.dtype, device=dev) if z is not None else None
-        h = torch.empty((rows, F), dtype=zt, device=dev) if pre_weight is not None else None
-        stats = torch.empty((rows, 4), dtype=torch.float32, device=dev) if any(ctx.needs_input_grad) else None
-        _ffi.check(lib.agcn_norm_gate_residual_forward(
-            C.byref(desc), None if plan is None else plan.host_ptr, None if plan is None else plan.dev_ptr, C.byref(inputs),
-            _rows_ptr(y), _rows_ptr(h), _ptr(stats), _stream(dev)))
+        y, h, saved, desc = _on_device_of(x, _norm_forward, z, x, gate, scale, post_weight, post_bias, pre_weight, pre_bias, plan,
+                                          norm, eps, gate_activation, True)
         ctx.desc, ctx.plan = desc, plan
-        ctx.save_for_backward(z, x, gate, scale, post_weight, post_bias, pre_weight, pre_bias, stats)
+        ctx.save_for_backward(*saved)
         ctx.set_materialize_grads(False)
         return y, h
 
     @staticmethod
-    @_on_tensor_device
     def backward(ctx, dy, dh):
-        lib = _ffi.lib()
-        z, x, gate, scale, post_weight, post_bias, pre_weight, pre_bias, stats = ctx.saved_tensors
-        desc, plan, dev = ctx.desc, ctx.plan, stats.device
-        rows, F = desc.rows, desc.F
         if dy is None and dh is None:
             return (None,) * 12
+        saved = ctx.saved_tensors
+        return _on_device_of(saved[-1], NormGateResidualFunction._backward, ctx.desc, ctx.plan, saved, dy, dh) + (None,) * 4
+
+    @staticmethod
+    def _backward(desc, plan, saved, dy, dh):
+        lib = _ffi.lib()
+        z, x, gate, scale, post_weight, post_bias, pre_weight, pre_bias, stats = saved
+        dev, rows, F = stats.device, desc.rows, desc.F
         dy = None if dy is None else dy.contiguous()
         dh = None if dh is None else dh.contiguous()
-        xt, zt = (torch.bfloat16 if d else torch.float32 for d in (desc.x_dtype, desc.z_dtype))
-        dx = torch.empty((rows, F), dtype=xt, device=dev)
-        dz = None if z is None else torch.empty((rows, F), dtype=zt, device=dev)
-        dgate = None if gate is None else torch.empty(tuple(gate.shape), dtype=zt, device=dev)
-        params = [None if p is None else torch.empty_like(p) for p in (scale, post_weight, post_bias, pre_weight, pre_bias)]
-        inputs = _ffi.NormInputs(_rows_ptr(z), _rows_ptr(x), _rows_ptr(gate), _ptr(scale), _ptr(post_weight),
-                                 _ptr(post_bias), _ptr(pre_weight), _ptr(pre_bias))
+        dx = torch.empty((rows, F), dtype=x.dtype, device=dev)
+        dz = None if z is None else torch.empty((rows, F), dtype=z.dtype, device=dev)
+        dgate = None if gate is None else torch.empty(gate.shape, dtype=gate.dtype, device=dev)
+        # (the vectors' gradients: rows of one small matrix)
+        vectors = (scale, post_weight, post_bias, pre_weight, pre_bias)
+        made = iter(torch.empty((5 - vectors.count(None), F), dtype=torch.float32, device=dev).unbind(0))
+        params = [None if p is None else next(made) for p in vectors]
+        inputs = _ffi.NormInputs(_rows_ptr(z), _rows_ptr(x), _rows_ptr(gate), _ptr(scale), _ptr(post_weight), _ptr(post_bias),
+                                 _ptr(pre_weight), _ptr(pre_bias))
         grads = _ffi.NormGrads(_rows_ptr(dz), _rows_ptr(dx), _rows_ptr(dgate), *[_ptr(p) for p in params])
         host, devp = (None, None) if plan is None else (plan.host_ptr, plan.dev_ptr)
         wbytes = lib.agcn_norm_gate_residual_backward_workspace_bytes(C.byref(desc), host)
         ws = torch.empty(wbytes, dtype=torch.uint8, device=dev)
         _ffi.check(lib.agcn_norm_gate_residual_backward(
-            C.byref(desc), host, devp, C.byref(inputs), _rows_ptr(stats), _rows_ptr(dy), _rows_ptr(dh),
-            C.byref(grads), ws.data_ptr(), wbytes, _stream(dev)))
-        dscale, dpw, dpb, dqw, dqb = params
-        return dz, dx, dgate, dscale, dpw, dpb, dqw, dqb, None, None, None, None
+            C.byref(desc), host, devp, C.byref(inputs), _rows_ptr(stats), _rows_ptr(dy), _rows_ptr(dh), C.byref(grads),
+            ws.data_ptr(), wbytes, _stream(dev)))
+        return (dz, dx, dgate) + tuple(params)
 
 
 def norm_gate_residual(z, x, post_weight=None, post_bias=None, gate=None, scale=None, pre_weight=None, pre_bias=None, norm="rms",
@@ -881,57 +908,62 @@ def norm_gate_residual(z, x, post_weight=None, post_bias=None, gate=None, scale=
     if x is None or not torch.is_tensor(x):
         raise TypeError("residual rows must be a tensor")
     plan = getattr(plan, "plan", plan)
-    return NormGateResidualFunction.apply(z, x, gate, scale, post_weight, post_bias, pre_weight, pre_bias, plan, norm, float(eps),
-                                          gate_activation)
+    args = (z, x, gate, scale, post_weight, post_bias, pre_weight, pre_bias)
+    if _wants_grad(args):
+        return NormGateResidualFunction.apply(*args, plan, norm, float(eps), gate_activation)
+    return _on_device_of(x, _norm_forward, *args, plan, norm, float(eps), gate_activation, False)[:2]
+
+
+def _ffn_forward(X, Wg, Wu, Wd, activation, keep):
+    """-> (Y, what a backward needs: the tensors as the kernels read them and the reserve, the descriptor)"""
+    lib = _ffi.lib()
+    X = _row_matrix(X, "node features")
+    rows, Fin = X.shape
+    dev = X.device
+    Ws = []
+    for W, what in ((Wg, "w_gate"), (Wu, "w_up"), (Wd, "w_down")):
+        if W.dtype is not X.dtype:
+            raise TypeError("%s is %s, the node features are %s" % (what, W.dtype, X.dtype))
+        _require_gpu(W, what)
+        if W.dim() != 2 or W.get_device() != X.get_device():
+            raise ValueError("%s must be a matrix on %s" % (what, dev))
+        Ws.append(W if W.is_contiguous() else W.contiguous())
+    Wg, Wu, Wd = Ws
+    H, Fout = Wg.shape[1], Wd.shape[1]
+    if Wg.shape[0] != Fin or Wu.shape != Wg.shape or Wd.shape[0] != H:
+        raise ValueError("w_gate and w_up must be [%d, H] and w_down [H, F_out], got %s, %s, %s" %
+                         (Fin, tuple(Wg.shape), tuple(Wu.shape), tuple(Wd.shape)))
+    desc = _ffi.FfnDesc(rows, Fin, H, Fout, _ffi.FFN_ACT[activation], _DT[X.dtype], _ld(X), 1 if keep else 0, 0)
+    rbytes, wbytes = lib.agcn_gated_ffn_reserve_bytes(C.byref(desc)), lib.agcn_gated_ffn_forward_workspace_bytes(C.byref(desc))
+    if not rbytes:
+        _ffi.check(-1)
+    reserve = torch.empty(rbytes, dtype=torch.uint8, device=dev)
+    ws = torch.empty(wbytes, dtype=torch.uint8, device=dev)
+    Y = torch.empty((rows, Fout), dtype=X.dtype, device=dev)
+    _ffi.check(lib.agcn_gated_ffn_forward(C.byref(desc), X.data_ptr(), Wg.data_ptr(), Wu.data_ptr(), Wd.data_ptr(), Y.data_ptr(),
+                                          reserve.data_ptr(), rbytes, ws.data_ptr(), wbytes, _stream(dev)))
+    return Y, (X, Wg, Wu, Wd, reserve), desc
 
 
 class GatedFfnFunction(torch.autograd.Function):
     """Y = (act(X Wg) * (X Wu)) Wd; see gated_ffn."""
 
     @staticmethod
-    @_on_tensor_device
     def forward(ctx, X, Wg, Wu, Wd, activation):
-        lib = _ffi.lib()
-        X = _row_matrix(X, "node features")
-        rows, Fin = X.shape
-        dev = X.device
-        Ws = []
-        for W, what in ((Wg, "w_gate"), (Wu, "w_up"), (Wd, "w_down")):
-            _require_gpu(W, what)
-            if W.dtype != X.dtype:
-                raise TypeError("%s is %s, the node features are %s" % (what, W.dtype, X.dtype))
-            if W.dim() != 2 or W.device != dev:
-                raise ValueError("%s must be a matrix on %s" % (what, dev))
-            Ws.append(W if W.is_contiguous() else W.contiguous())
-        Wg, Wu, Wd = Ws
-        H = Wg.shape[1]
-        if tuple(Wg.shape) != (Fin, H) or tuple(Wu.shape) != (Fin, H) or Wd.shape[0] != H:
-            raise ValueError("w_gate and w_up must be [%d, H] and w_down [H, F_out], got %s, %s, %s" %
-                             (Fin, tuple(Wg.shape), tuple(Wu.shape), tuple(Wd.shape)))
-        Fout = Wd.shape[1]
-        training = any(ctx.needs_input_grad)
-        desc = _ffi.FfnDesc(rows, Fin, H, Fout, _ffi.FFN_ACT[activation], _DT[X.dtype], _ld(X), 1 if training else 0, 0)
-        rbytes, wbytes = lib.agcn_gated_ffn_reserve_bytes(C.byref(desc)), lib.agcn_gated_ffn_forward_workspace_bytes(C.byref(desc))
-        if not rbytes:
-            _ffi.check(-1)
-        reserve = torch.empty(rbytes, dtype=torch.uint8, device=dev)
-        ws = torch.empty(wbytes, dtype=torch.uint8, device=dev)
-        Y = torch.empty((rows, Fout), dtype=X.dtype, device=dev)
-        _ffi.check(lib.agcn_gated_ffn_forward(C.byref(desc), X.data_ptr(), Wg.data_ptr(), Wu.data_ptr(), Wd.data_ptr(), Y.data_ptr(),
-                                              reserve.data_ptr(), rbytes, ws.data_ptr(), wbytes, _stream(dev)))
-        if training:
-            ctx.desc = desc
-            ctx.save_for_backward(X, Wg, Wu, Wd, reserve)
+        Y, saved, ctx.desc = _on_device_of(X, _ffn_forward, X, Wg, Wu, Wd, activation, True)
+        ctx.save_for_backward(*saved)
         return Y
 
     @staticmethod
-    @_on_tensor_device
     def backward(ctx, dY):
+        return _on_device_of(dY, GatedFfnFunction._backward, ctx.desc, ctx.saved_tensors, dY, ctx.needs_input_grad)
+
+    @staticmethod
+    def _backward(desc, saved, dY, need):
         lib = _ffi.lib()
-        X, Wg, Wu, Wd, reserve = ctx.saved_tensors
-        desc, dev = ctx.desc, X.device
+        X, Wg, Wu, Wd, reserve = saved
+        dev = X.device
         dY = dY.contiguous()
-        need = ctx.needs_input_grad
         dX = torch.empty((desc.rows, desc.Fin), dtype=X.dtype, device=dev) if need[0] else None
         dWg, dWu = (torch.empty_like(Wg), torch.empty_like(Wu)) if need[1] or need[2] else (None, None)
         dWd = torch.empty_like(Wd) if need[3] else None
@@ -949,4 +981,6 @@ def gated_ffn(X, w_gate, w_up, w_down, activation="silu"):
     row of its own: pad rows that are zero come out zero."""
     if activation not in _ffi.FFN_ACT:
         raise ValueError("activation must be one of %s" % ", ".join(sorted(_ffi.FFN_ACT)))
-    return GatedFfnFunction.apply(X, w_gate, w_up, w_down, activation)
+    if _wants_grad((X, w_gate, w_up, w_down)):
+        return GatedFfnFunction.apply(X, w_gate, w_up, w_down, activation)
+    return _on_device_of(X, _ffn_forward, X, w_gate, w_up, w_down, activation, False)[0]
