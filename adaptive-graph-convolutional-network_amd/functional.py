@@ -876,8 +876,10 @@ class NormGateResidualFunction(torch.autograd.Function):
         dgate = None if gate is None else torch.empty(gate.shape, dtype=gate.dtype, device=dev)
         # (the vectors' gradients: rows of one small matrix)
         vectors = (scale, post_weight, post_bias, pre_weight, pre_bias)
-        made = iter(torch.empty((5 - vectors.count(None), F), dtype=torch.float32, device=dev).unbind(0))
-        params = [None if p is None else next(made) for p in vectors]
+        given = [i for i, p in enumerate(vectors) if p is not None]
+        params = [None] * 5
+        for i, g in zip(given, torch.empty((len(given), F), dtype=torch.float32, device=dev).unbind(0)):
+            params[i] = g
         inputs = _ffi.NormInputs(_rows_ptr(z), _rows_ptr(x), _rows_ptr(gate), _ptr(scale), _ptr(post_weight), _ptr(post_bias),
                                  _ptr(pre_weight), _ptr(pre_bias))
         grads = _ffi.NormGrads(_rows_ptr(dz), _rows_ptr(dx), _rows_ptr(dgate), *[_ptr(p) for p in params])
