@@ -5,8 +5,9 @@
 // Bound by the matrix pipe (18 M F H operations a training pass), for few rows by the weights' bytes.  Everything is one tiled
 // product kernel on v_mfma_f32_16x16x32_bf16 with fp32 accumulators:
 //   * Both projections share one pass over X: a workgroup's tile holds the same columns of Wg and Wu, so that the gate and its
-//     partner meet in one lane's registers and the epilogue writes A (and, for a backward, G and U).  dA never reaches memory
-//     either: its epilogue reads G and U and writes dG and dU.  dX is one product over 2 H, dWg and dWu share X's tiles.
+//     partner meet in one lane's registers and the epilogue writes A (and, for a backward, P = U act'(G) and Q = act(G)).  dA never
+//     reaches memory either: its epilogue reads P and Q and writes dG = dA P and dU = dA Q.  dX is one product over 2 H, dWg and
+//     dWu share X's tiles.
 //   * fp32 operands are split exactly into three bf16 pieces (bf16_split.h), and a product is the sum of six piece products (the
 //     dropped ones are below 2^-24): a stage holds the three planes of both operands, every fragment read serves two of them.
 //   * Tiles go from memory to LDS directly (buffer_load .. lds, 16 bytes per lane), in two or three stages.  An operand whose rows
@@ -18,8 +19,8 @@
 //     one small loop of epilogue code instead of one copy per fragment.
 //   * Few tiles for the chip: the k loop is cut into splits whose fp32 tiles a second kernel adds in order (no atomics) and
 //     puts through the same epilogue.
-// Roundings of bf16 calls: A, dG, dU are stored in bf16 for the products that read them (the matrix pipe takes bf16); G and U, which
-// only the element-wise slopes read again, keep 24 bits (sign, exponent, 15 bits of the mantissa: in bf16 they would add as
+// Roundings of bf16 calls: A, dG, dU are stored in bf16 for the products that read them (the matrix pipe takes bf16); P and Q, which
+// are only multiplied element by element, keep 24 bits (sign, exponent, 15 bits of the mantissa: in bf16 they would add as
 // much error to every gradient as dG's own rounding); sums, activations and their slopes are fp32.
 #include <hip/hip_bf16.h>
 #include <hip/hip_runtime.h>
@@ -50,11 +51,11 @@ struct GemmArgs {
   int32_t ldp;
   // epilogue
   int32_t act, f32;
-  int32_t ldh;                       // leading dimension of G, U, A, dG, dU
+  int32_t ldh;                       // leading dimension of P, Q, A, dG, dU
   int64_t plane;                     // elements between the planes of A, dG, dU
   void *out, *out2;                  // EPI_STORE: [M, ldo]
   int32_t ldo;
-  void *g, *u;                       // f32, or 24 bits: [M, ldh] upper sixteen, then [M, ldh] lower eight
+  void *p, *q;                       // U act'(G) and act(G): f32, or 24 bits: [M, ldh] upper sixteen, then [M, ldh] lower eight
   uint16_t *hid, *dg, *du;           // bf16 pieces
 };
 
@@ -75,6 +76,32 @@ __device__ __forceinline__ void gate_of(int act, float g, float& a, float& da) {
   } else {
     const float e = expf(-fabsf(g)), d = 1.f / (1.f + e);
     const float s = g >= 0.f ? d : e * d, ns = g >= 0.f ? e * d : d;    // sigmoid(g), sigmoid(-g)
+    if (act == AGCN_ACT_SIGMOID) {
+      a = s;
+      da = s * ns;
+    } else {
+      a = g * s;
+      da = s * fmaf(g, ns, 1.f);
+    }
+  }
+}
+// The same for bf16 calls, whose results are rounded to eight bits: the hardware's exp2 and reciprocal (a few 2^-24, and
+// |g| 2^-23 from the exponent's rounding), and for the normal distribution function the five-term fit of Abramowitz and Stegun,
+// 7.1.26 (1.4e-7; relative to the tail 3e-5 at g = -2.8, beyond which the library function takes over).
+__device__ __forceinline__ void gate_of_bf16(int act, float g, float& a, float& da) {
+  if (act == AGCN_ACT_RELU) {
+    gate_of(AGCN_ACT_RELU, g, a, da);
+  } else if (act == AGCN_ACT_GELU) {
+    const float x = 0.70710678f * fabsf(g), t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.f));
+    const float e = __builtin_amdgcn_exp2f(-0.72134752f * g * g);       // e^(-g^2 / 2)
+    float q = fmaf(fmaf(fmaf(fmaf(1.061405429f, t, -1.453152027f), t, 1.421413741f), t, -0.284496736f), t, 0.254829592f) * t * e;
+    if (g < -2.828427f) q = erfcf(x);
+    const float c = g < 0.f ? 0.5f * q : fmaf(-0.5f, q, 1.f);
+    a = g * c;
+    da = fmaf(g, 0.39894228f * e, c);
+  } else {
+    const float e = __builtin_amdgcn_exp2f(-1.44269504f * fabsf(g)), d = __builtin_amdgcn_rcpf(1.f + e);
+    const float s = g >= 0.f ? d : e * d, ns = g >= 0.f ? e * d : d;
     if (act == AGCN_ACT_SIGMOID) {
       a = s;
       da = s * ns;
@@ -105,7 +132,7 @@ __device__ __forceinline__ uint32_t top24(float x) {
   const uint32_t b = __float_as_uint(x);
   return x != x ? (b >> 8) | 0x4000u : (b + 0x80u) >> 8;
 }
-__device__ __forceinline__ void store8_gate(const GemmArgs& g, void* p, int64_t at, const F8& x) {
+__device__ __forceinline__ void store8_kept(const GemmArgs& g, void* p, int64_t at, const F8& x) {
   if (g.f32) {
     store8_f32(static_cast<float*>(p) + at, x);
   } else {
@@ -123,7 +150,7 @@ __device__ __forceinline__ void store8_gate(const GemmArgs& g, void* p, int64_t 
     *reinterpret_cast<u32x2*>(reinterpret_cast<uint8_t*>(static_cast<uint16_t*>(p) + (int64_t)g.M * g.ldh) + at) = lo;
   }
 }
-__device__ __forceinline__ F8 load8_gate(const GemmArgs& g, const void* p, int64_t at) {
+__device__ __forceinline__ F8 load8_kept(const GemmArgs& g, const void* p, int64_t at) {
   if (g.f32) return load8_f32(static_cast<const float*>(p) + at);
   const u32x4 hi = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(p) + at);
   const u32x2 lo = *reinterpret_cast<const u32x2*>(reinterpret_cast<const uint8_t*>(static_cast<const uint16_t*>(p) + (int64_t)g.M * g.ldh) + at);
@@ -190,27 +217,28 @@ __device__ __forceinline__ void epilogue(const GemmArgs& g, int m, int n, const 
   if (n >= g.ldh) return;
   const int64_t at = (int64_t)m * g.ldh + n;
   if (EPI == EPI_GATED) {
-    F8 hv;
+    F8 hv, pv, qv;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       float a, da;
-      gate_of(g.act, v0.v[i], a, da);
+      if (g.f32) gate_of(g.act, v0.v[i], a, da);
+      else gate_of_bf16(g.act, v0.v[i], a, da);
+      qv.v[i] = n + i < g.N ? a : 0.f;
       hv.v[i] = n + i < g.N ? a * v1.v[i] : 0.f;
+      pv.v[i] = n + i < g.N ? da * v1.v[i] : 0.f;
     }
-    if (g.g) {
-      store8_gate(g, g.g, at, v0);
-      store8_gate(g, g.u, at, v1);
+    if (g.p) {
+      store8_kept(g, g.p, at, pv);
+      store8_kept(g, g.q, at, qv);
     }
     store8_pieces(g, g.hid, at, hv);
   } else {
-    const F8 gv = load8_gate(g, g.g, at), uv = load8_gate(g, g.u, at);
+    const F8 pv = load8_kept(g, g.p, at), qv = load8_kept(g, g.q, at);
     F8 dg, du;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      float a, da;
-      gate_of(g.act, gv.v[i], a, da);
-      dg.v[i] = n + i < g.N ? v0.v[i] * uv.v[i] * da : 0.f;
-      du.v[i] = n + i < g.N ? v0.v[i] * a : 0.f;
+      dg.v[i] = v0.v[i] * pv.v[i];
+      du.v[i] = v0.v[i] * qv.v[i];
     }
     store8_pieces(g, g.dg, at, dg);
     store8_pieces(g, g.du, at, du);
@@ -583,7 +611,7 @@ bool direct(const AgcnFfnDesc& d, const void* p, int cols, int ld) {
 
 // What the forward leaves for the backward.  The images are there only where a matrix cannot be read as it is; room is kept for
 // them whenever the SIZES alone would not rule them out (an address can be odd).
-struct Reserve { uint16_t *x, *wg, *wu, *wd, *hid; void *g, *u; };
+struct Reserve { uint16_t *x, *wg, *wu, *wd, *hid; void *p, *q; };
 size_t carve_reserve(const AgcnFfnDesc& d, void* mem, Reserve* r) {
   Carve c{static_cast<char*>(mem), 0};
   const int P = d.dtype == AGCN_DTYPE_F32 ? 3 : 1, Hp = pad8(d.H), Fp = pad8(d.Fin), Op = pad8(d.Fout);
@@ -593,8 +621,8 @@ size_t carve_reserve(const AgcnFfnDesc& d, void* mem, Reserve* r) {
   r->wu = static_cast<uint16_t*>(c.take((size_t)P * d.Fin * Hp * 2));
   r->wd = static_cast<uint16_t*>(c.take((size_t)P * d.H * Op * 2));
   r->hid = static_cast<uint16_t*>(c.take((size_t)P * d.rows * Hp * 2));
-  r->g = d.training ? c.take(e * d.rows * Hp) : nullptr;
-  r->u = d.training ? c.take(e * d.rows * Hp) : nullptr;
+  r->p = d.training ? c.take(e * d.rows * Hp) : nullptr;
+  r->q = d.training ? c.take(e * d.rows * Hp) : nullptr;
   return c.off;
 }
 
@@ -765,7 +793,7 @@ extern "C" int agcn_gated_ffn_forward(const AgcnFfnDesc* desc, const void* X, co
   GemmArgs g = base_args(d);
   operands(&g, x, wg, &wu);
   g.M = (int)d.rows; g.N = d.H; g.K = d.Fin;
-  g.g = r.g; g.u = r.u; g.hid = r.hid;
+  g.p = r.p; g.q = r.q; g.hid = r.hid;
   product<false, true, 2, EPI_GATED>(g, workspace, s);
   const Mat hid = {r.hid, g.ldh, g.f32 ? g.plane : 0};
   GemmArgs q = base_args(d);
@@ -816,7 +844,7 @@ extern "C" int agcn_gated_ffn_backward(const AgcnFfnDesc* desc, const void* X, c
     GemmArgs g = base;                        // dA = dY Wd^T, and from it dG and dU
     operands(&g, dy, wd, nullptr);
     g.M = (int)d.rows; g.N = d.H; g.K = d.Fout;
-    g.g = r.g; g.u = r.u; g.dg = w.dg; g.du = w.du;
+    g.p = r.p; g.q = r.q; g.dg = w.dg; g.du = w.du;
     product<false, false, 1, EPI_DH>(g, w.part, s);
   }
   if (dX) {
