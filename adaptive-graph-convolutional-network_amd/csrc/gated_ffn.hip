@@ -127,44 +127,64 @@ __device__ __forceinline__ F8 load8_f32(const float* p) {
 __device__ __forceinline__ u32x4 bf8(const F8& x) {
   return (u32x4){pk_bf(x.v[0], x.v[1]), pk_bf(x.v[2], x.v[3]), pk_bf(x.v[4], x.v[5]), pk_bf(x.v[6], x.v[7])};
 }
-// 24 bits of a float, rounded to nearest (ties away; a carry out of the largest finite value gives infinity), NaN kept
-__device__ __forceinline__ uint32_t top24(float x) {
-  const uint32_t b = __float_as_uint(x);
-  return x != x ? (b >> 8) | 0x4000u : (b + 0x80u) >> 8;
+// What the backward's epilogue reads: P and Q.  fp32 calls: as they are.  bf16 calls: 24 bits of each value, rounded to nearest (ties
+// away; a carry out of the largest finite value gives infinity), the upper sixteen and the lower eight in planes of their own;
+// bytes are moved with v_perm.  (A NaN stays one: those of a bf16 call have nothing in the low bits that the rounding could carry
+// out of.)
+template <bool F32> struct Kept8;
+template <> struct Kept8<true> { f32x4 a, b; };
+template <> struct Kept8<false> { u32x4 hi; u32x2 lo; };
+__device__ __forceinline__ uint8_t* low_plane(const GemmArgs& g, const void* p) {
+  return reinterpret_cast<uint8_t*>(const_cast<uint16_t*>(static_cast<const uint16_t*>(p)) + (int64_t)g.M * g.ldh);
 }
+template <bool F32>
 __device__ __forceinline__ void store8_kept(const GemmArgs& g, void* p, int64_t at, const F8& x) {
-  if (g.f32) {
+  if constexpr (F32) {
     store8_f32(static_cast<float*>(p) + at, x);
   } else {
-    uint32_t t[8];
+    uint32_t r[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) t[i] = top24(x.v[i]);
+    for (int i = 0; i < 8; ++i) r[i] = __float_as_uint(x.v[i]) + 0x80u;
     u32x4 hi;
     u32x2 lo;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) hi[i] = (t[2 * i] >> 8) | (t[2 * i + 1] >> 8) << 16;
+    for (int i = 0; i < 4; ++i) hi[i] = __builtin_amdgcn_perm(r[2 * i + 1], r[2 * i], 0x07060302u);
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-      lo[i] = (t[4 * i] & 255u) | (t[4 * i + 1] & 255u) << 8 | (t[4 * i + 2] & 255u) << 16 | t[4 * i + 3] << 24;
+      lo[i] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(r[4 * i + 3], r[4 * i + 2], 0x0c0c0501u),
+                                    __builtin_amdgcn_perm(r[4 * i + 1], r[4 * i], 0x0c0c0501u), 0x05040100u);
     *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(p) + at) = hi;
-    *reinterpret_cast<u32x2*>(reinterpret_cast<uint8_t*>(static_cast<uint16_t*>(p) + (int64_t)g.M * g.ldh) + at) = lo;
+    *reinterpret_cast<u32x2*>(low_plane(g, p) + at) = lo;
   }
 }
-__device__ __forceinline__ F8 load8_kept(const GemmArgs& g, const void* p, int64_t at) {
-  if (g.f32) return load8_f32(static_cast<const float*>(p) + at);
-  const u32x4 hi = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(p) + at);
-  const u32x2 lo = *reinterpret_cast<const u32x2*>(reinterpret_cast<const uint8_t*>(static_cast<const uint16_t*>(p) + (int64_t)g.M * g.ldh) + at);
+template <bool F32>
+__device__ __forceinline__ void fetch8_kept(const GemmArgs& g, const void* p, int64_t at, Kept8<F32>& k) {
+  if constexpr (F32) {
+    const float* q = static_cast<const float*>(p) + at;
+    k.a = *reinterpret_cast<const f32x4*>(q);
+    k.b = *reinterpret_cast<const f32x4*>(q + 4);
+  } else {
+    k.hi = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(p) + at);
+    k.lo = *reinterpret_cast<const u32x2*>(low_plane(g, p) + at);
+  }
+}
+template <bool F32>
+__device__ __forceinline__ F8 kept8(const Kept8<F32>& k) {
   F8 x;
+  if constexpr (F32) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t h = i & 1 ? hi[i >> 1] & 0xffff0000u : hi[i >> 1] << 16, l = (lo[i >> 2] >> (8 * (i & 3))) & 255u;
-    x.v[i] = __uint_as_float(h | l << 8);
+    for (int i = 0; i < 4; ++i) { x.v[i] = k.a[i]; x.v[4 + i] = k.b[i]; }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      x.v[i] = __uint_as_float(__builtin_amdgcn_perm(k.hi[i >> 1], k.lo[i >> 2], (i & 1 ? 0x07060000u : 0x05040000u) | (uint32_t)(i & 3) << 8 | 0x0cu));
   }
   return x;
 }
 // the bf16 pieces of eight values (bf16 calls: the rounded values themselves)
+template <bool F32>
 __device__ __forceinline__ void store8_pieces(const GemmArgs& g, uint16_t* p, int64_t at, const F8& x) {
-  if (!g.f32) {
+  if constexpr (!F32) {
     *reinterpret_cast<u32x4*>(p + at) = bf8(x);
   } else {
     u32x4 h, m, l;
@@ -180,9 +200,10 @@ __device__ __forceinline__ void store8_pieces(const GemmArgs& g, uint16_t* p, in
   }
 }
 // a caller's matrix: any alignment, any tail
+template <bool F32>
 __device__ __forceinline__ void store8_out(const GemmArgs& g, void* p, int64_t row, int n, const F8& x) {
   const int64_t at = row * g.ldo + n;
-  if (g.f32) {
+  if constexpr (F32) {
     float* o = static_cast<float*>(p) + at;
     if (n + 8 <= g.N) {
 #pragma unroll
@@ -204,13 +225,13 @@ __device__ __forceinline__ void store8_out(const GemmArgs& g, void* p, int64_t r
   }
 }
 
-// What becomes of columns n .. n + 7 of row m (v1: of the second B matrix)
-template <int EPI, int NB>
-__device__ __forceinline__ void epilogue(const GemmArgs& g, int m, int n, const F8& v0, const F8& v1) {
+// What becomes of columns n .. n + 7 of row m (v1: of the second B matrix; P, Q: fetched by the caller)
+template <int EPI, int NB, bool F32>
+__device__ __forceinline__ void epilogue(const GemmArgs& g, int m, int n, const F8& v0, const F8& v1, const Kept8<F32>& P, const Kept8<F32>& Q) {
   if (EPI == EPI_STORE) {
     if (n >= g.N) return;
-    store8_out(g, g.out, m, n, v0);
-    if (NB == 2) store8_out(g, g.out2, m, n, v1);
+    store8_out<F32>(g, g.out, m, n, v0);
+    if (NB == 2) store8_out<F32>(g, g.out2, m, n, v1);
     return;
   }
   // (the library's own matrices are padded to eights: the columns behind H get the zeros that the products read there)
@@ -221,27 +242,27 @@ __device__ __forceinline__ void epilogue(const GemmArgs& g, int m, int n, const 
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       float a, da;
-      if (g.f32) gate_of(g.act, v0.v[i], a, da);
+      if (F32) gate_of(g.act, v0.v[i], a, da);
       else gate_of_bf16(g.act, v0.v[i], a, da);
       qv.v[i] = n + i < g.N ? a : 0.f;
       hv.v[i] = n + i < g.N ? a * v1.v[i] : 0.f;
       pv.v[i] = n + i < g.N ? da * v1.v[i] : 0.f;
     }
     if (g.p) {
-      store8_kept(g, g.p, at, pv);
-      store8_kept(g, g.q, at, qv);
+      store8_kept<F32>(g, g.p, at, pv);
+      store8_kept<F32>(g, g.q, at, qv);
     }
-    store8_pieces(g, g.hid, at, hv);
+    store8_pieces<F32>(g, g.hid, at, hv);
   } else {
-    const F8 pv = load8_kept(g, g.p, at), qv = load8_kept(g, g.q, at);
+    const F8 pv = kept8<F32>(P), qv = kept8<F32>(Q);
     F8 dg, du;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       dg.v[i] = v0.v[i] * pv.v[i];
       du.v[i] = v0.v[i] * qv.v[i];
     }
-    store8_pieces(g, g.dg, at, dg);
-    store8_pieces(g, g.du, at, du);
+    store8_pieces<F32>(g, g.dg, at, dg);
+    store8_pieces<F32>(g, g.du, at, du);
   }
 }
 
@@ -468,28 +489,45 @@ __global__ __launch_bounds__(64 * WGM * WGN) void ffn_gemm_kernel(GemmArgs g) {
           *reinterpret_cast<AGCN_LDS f32x4*>(reg + (i * 16 + mr) * (CH * 16) + ((((c * FN + j) * 4 + q) ^ (mr & (CH - 1))) << 4)) = acc[c][ps * PF + i][j];
     // (one wave's own rows: the wait is for its own writes)
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    constexpr int LPR = FN * 2;                       // lanes per row, eight columns each
-    const int c8 = lane % LPR;
+    constexpr int LPR = FN * 2, RPI = 64 / LPR;       // lanes per row, eight columns each; rows at a time
+    // (dA's epilogue: the reads of P and Q of UN turns fly together; one turn's at a time left the matrix pipe waiting for memory, 36
+    // us a tile of 8192 x 8192)
+    constexpr int UN = EPI == EPI_DH ? (PR / RPI < 4 ? PR / RPI : 4) : 1;
+    const int c8 = lane % LPR, n = n_wave + c8 * 8;
 #pragma unroll 1
-    for (int r0 = 0; r0 < PR; r0 += 64 / LPR) {
-      const int r = r0 + lane / LPR, m = m0 + wm * FM * 16 + ps * PR + r, n = n_wave + c8 * 8;
-      F8 v[NB];
+    for (int r0 = 0; r0 < PR; r0 += RPI * UN) {
+      Kept8<P == 3> kp[UN], kq[UN];
+      if (EPI == EPI_DH && g.splits == 1) {
 #pragma unroll
-      for (int c = 0; c < NB; ++c) {
-        const int ch = (c * FN * 4 + c8 * 2), x = r & 15 & (CH - 1);
-        const f32x4 lo = *reinterpret_cast<const AGCN_LDS f32x4*>(reg + r * (CH * 16) + ((ch ^ x) << 4));
-        const f32x4 hi = *reinterpret_cast<const AGCN_LDS f32x4*>(reg + r * (CH * 16) + (((ch + 1) ^ x) << 4));
-        v[c] = {{lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w}};
-      }
-      if (m < g.M) {
-        if (g.splits > 1) {
-          if (n < g.ldp) {
-            float* p = g.part + ((int64_t)split * NB * g.M + m) * g.ldp + n;
-            store8_f32(p, v[0]);
-            if (NB == 2) store8_f32(p + (int64_t)g.M * g.ldp, v[NB - 1]);
+        for (int u = 0; u < UN; ++u) {
+          const int m = m0 + wm * FM * 16 + ps * PR + r0 + u * RPI + lane / LPR;
+          if (m < g.M && n < g.ldh) {
+            fetch8_kept<P == 3>(g, g.p, (int64_t)m * g.ldh + n, kp[u]);
+            fetch8_kept<P == 3>(g, g.q, (int64_t)m * g.ldh + n, kq[u]);
           }
-        } else {
-          epilogue<EPI, NB>(g, m, n, v[0], v[NB - 1]);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < UN; ++u) {
+        const int r = r0 + u * RPI + lane / LPR, m = m0 + wm * FM * 16 + ps * PR + r;
+        F8 v[NB];
+#pragma unroll
+        for (int c = 0; c < NB; ++c) {
+          const int ch = (c * FN * 4 + c8 * 2), x = r & 15 & (CH - 1);
+          const f32x4 lo = *reinterpret_cast<const AGCN_LDS f32x4*>(reg + r * (CH * 16) + ((ch ^ x) << 4));
+          const f32x4 hi = *reinterpret_cast<const AGCN_LDS f32x4*>(reg + r * (CH * 16) + (((ch + 1) ^ x) << 4));
+          v[c] = {{lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w}};
+        }
+        if (m < g.M) {
+          if (g.splits > 1) {
+            if (n < g.ldp) {
+              float* p = g.part + ((int64_t)split * NB * g.M + m) * g.ldp + n;
+              store8_f32(p, v[0]);
+              if (NB == 2) store8_f32(p + (int64_t)g.M * g.ldp, v[NB - 1]);
+            }
+          } else {
+            epilogue<EPI, NB, P == 3>(g, m, n, v[0], v[NB - 1], kp[u], kq[u]);
+          }
         }
       }
     }
@@ -500,7 +538,7 @@ __global__ __launch_bounds__(64 * WGM * WGN) void ffn_gemm_kernel(GemmArgs g) {
 
 // Adds the splits' tiles in order and puts the sums through the epilogue.  A workgroup takes 32 times eight columns; eight lanes
 // share the splits of each (a single lane would wait for one load after another), and their sums are added in lane order.
-template <int NB, int EPI>
+template <int NB, int EPI, bool F32>
 __global__ __launch_bounds__(256) void ffn_reduce_kernel(GemmArgs g) {
   __shared__ float sums[8][32][NB * 8 + 1];
   const int64_t per = g.ldp >> 3, e = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
@@ -532,7 +570,12 @@ __global__ __launch_bounds__(256) void ffn_reduce_kernel(GemmArgs g) {
     for (int k = 0; k < 8; ++k) s += sums[k][ev][i];
     o[i >> 3].v[i & 7] = s;
   }
-  epilogue<EPI, NB>(g, m, n, o[0], o[NB - 1]);
+  Kept8<F32> kp, kq;
+  if (EPI == EPI_DH) {
+    fetch8_kept<F32>(g, g.p, (int64_t)m * g.ldh + n, kp);
+    fetch8_kept<F32>(g, g.q, (int64_t)m * g.ldh + n, kq);
+  }
+  epilogue<EPI, NB, F32>(g, m, n, o[0], o[NB - 1], kp, kq);
 }
 
 // Operand images: bf16 matrices whose rows do not start at 16 bytes or end at eights, padded with zeros; fp32 ones as three planes of
@@ -674,8 +717,9 @@ void product(GemmArgs& g, void* part, hipStream_t s) {
     else if (c.kind == 1) launch_tile<3, 128, 64 / NB, 2, 2, AT, BT, NB, EPI, 2>(g, s);
     else launch_tile<3, 64, 64 / NB, 2, 2, AT, BT, NB, EPI, 3>(g, s);
   }
-  if (g.splits > 1)
-    hipLaunchKernelGGL((ffn_reduce_kernel<NB, EPI>), dim3((unsigned)cdiv((int64_t)g.M * (g.ldp / 8), 32)), dim3(256), 0, s, g);
+  const dim3 rg((unsigned)cdiv((int64_t)g.M * (g.ldp / 8), 32));
+  if (g.splits > 1 && planes == 1) hipLaunchKernelGGL((ffn_reduce_kernel<NB, EPI, false>), rg, dim3(256), 0, s, g);
+  else if (g.splits > 1) hipLaunchKernelGGL((ffn_reduce_kernel<NB, EPI, true>), rg, dim3(256), 0, s, g);
 }
 
 // the operands of a product: one or two pairs of matrices
