@@ -677,15 +677,35 @@ Config tile_of(int kind, int planes, int nb, int splits) {
   if (kind == 1) return {1, 128, (planes == 1 ? 128 : 64) / nb, splits};
   return {2, 64, planes == 1 ? 64 : 64 / nb, splits};
 }
-Config choose(int64_t M, int64_t N, int nb, int planes, int64_t iters) {
-  Config c = tile_of(0, planes, nb, 1);
-  if (cdiv(M, c.bm) * cdiv(N, c.bn) >= 192) return c;
-  c = tile_of(1, planes, nb, 1);
-  if (cdiv(M, c.bm) * cdiv(N, c.bn) >= 256) return c;
-  c = tile_of(2, planes, nb, 1);
-  const int64_t tiles = std::max<int64_t>(1, cdiv(M, c.bm) * cdiv(N, c.bn));    // (size queries come here with no rows, too)
-  if (tiles < 512) c.splits = (int)std::min<int64_t>(64, std::min(cdiv(1024, tiles), std::max<int64_t>(1, iters / 4)));
-  return c;
+// The choice: the least time by a model of the chip's 256 CUs.  per_it[w - 1]: a k stage with w workgroups on the CU (the large tile's
+// 8 waves fill it; two middle or two to three small ones share it), fixed: a tile's first loads and its epilogue -- microseconds,
+// measured on 5003 x 1001 x 2731 (bf16) and 32768 x 128 x 512 (fp32) with every kind in turn: e.g. X^T dG, 344 middle tiles of 79
+// stages 84 us, 172 large ones in two splits 82 + 17, small ones 105; A^T dY, 176 middle tiles 70 us, in two splits 54 + 9.
+// Splits cost their fp32 tiles' way to memory and back (4 MB a microsecond; half that through the gates' epilogues).
+Config choose(int64_t M, int64_t N, int nb, int planes, int64_t iters, bool gates) {
+  struct Cost { float per_it[3], fixed; int at_once, most; };
+  static const Cost kBf16[3] = {{{2.0f, 0.f, 0.f}, 8.f, 1, 4}, {{0.82f, 1.08f, 0.f}, 6.f, 2, 8}, {{0.45f, 0.65f, 0.86f}, 4.f, 3, 64}};
+  static const Cost kF32[3] = {{{2.8f, 0.f, 0.f}, 8.f, 1, 4}, {{1.0f, 1.6f, 0.f}, 5.f, 2, 8}, {{0.6f, 0.9f, 0.f}, 4.f, 2, 64}};
+  Config best = tile_of(2, planes, nb, 1);
+  float least = 1e30f;
+  for (int kind = 0; kind < 3; ++kind) {
+    const Cost& k = planes == 1 ? kBf16[kind] : kF32[kind];
+    const int at_once = kind == 2 && nb == 2 ? 2 : k.at_once;            // (the LDS of two B matrices: two workgroups)
+    const Config c = tile_of(kind, planes, nb, 1);
+    const int64_t tiles = std::max<int64_t>(1, cdiv(M, c.bm) * cdiv(N, c.bn));     // (size queries come here with no rows, too)
+    for (int s = 1; s <= k.most && s <= std::max<int64_t>(1, iters / 2); s += s < 8 ? 1 : 4) {
+      const int64_t per_cu = cdiv(tiles * s, 256), its = cdiv(iters, s);
+      const int rest = (int)(per_cu % at_once);
+      float t = (float)(per_cu / at_once) * (its * k.per_it[at_once - 1] + k.fixed);
+      if (rest) t += its * k.per_it[rest - 1] + k.fixed;
+      if (s > 1) t += 4.f + (float)s * nb * M * N * 8.f / (gates ? 2e6f : 4e6f);
+      if (t < least) {
+        least = t;
+        best = tile_of(kind, planes, nb, s);
+      }
+    }
+  }
+  return best;
 }
 
 size_t part_bytes(const Config& c, int64_t M, int64_t N, int nb) {
@@ -705,7 +725,7 @@ void product(GemmArgs& g, void* part, hipStream_t s) {
   const int planes = g.f32 ? 3 : 1;
   g.ktiles = (int)cdiv(g.K, g.f32 ? 32 : 64);
   const int n_all = EPI == EPI_STORE ? g.N : g.ldh;         // columns that the epilogue has to reach
-  const Config c = choose(g.M, n_all, NB, planes, (int64_t)g.nseg * g.ktiles);
+  const Config c = choose(g.M, n_all, NB, planes, (int64_t)g.nseg * g.ktiles, EPI != EPI_STORE);
   g.tiles_m = (int)cdiv(g.M, c.bm); g.tiles_n = (int)cdiv(n_all, c.bn); g.splits = c.splits;
   g.part = static_cast<float*>(part); g.ldp = (n_all + 7) & ~7;
   if (planes == 1) {
@@ -771,11 +791,11 @@ GemmArgs base_args(const AgcnFfnDesc& d) {
   return g;
 }
 
-size_t product_part(const AgcnFfnDesc& d, int64_t M, int64_t N, int nb, int64_t K, int nseg) {
-  return part_bytes(choose(M, N, nb, planes_of(d), nseg * ktiles_of(d, K)), M, N, nb);
+size_t product_part(const AgcnFfnDesc& d, int64_t M, int64_t N, int nb, int64_t K, int nseg, bool gates) {
+  return part_bytes(choose(M, N, nb, planes_of(d), nseg * ktiles_of(d, K), gates), M, N, nb);
 }
 size_t forward_part(const AgcnFfnDesc& d) {
-  return std::max(product_part(d, d.rows, pad8(d.H), 2, d.Fin, 1), product_part(d, d.rows, d.Fout, 1, d.H, 1));
+  return std::max(product_part(d, d.rows, pad8(d.H), 2, d.Fin, 1, true), product_part(d, d.rows, d.Fout, 1, d.H, 1, false));
 }
 struct BackWs { uint16_t *dy, *dg, *du; void* part; };
 size_t carve_backward(const AgcnFfnDesc& d, void* mem, BackWs* w) {
@@ -784,8 +804,8 @@ size_t carve_backward(const AgcnFfnDesc& d, void* mem, BackWs* w) {
   w->dy = static_cast<uint16_t*>(c.take((size_t)P * d.rows * pad8(d.Fout) * 2));
   w->dg = static_cast<uint16_t*>(c.take((size_t)P * d.rows * Hp * 2));
   w->du = static_cast<uint16_t*>(c.take((size_t)P * d.rows * Hp * 2));
-  w->part = c.take(std::max(std::max(product_part(d, d.rows, Hp, 1, d.Fout, 1), product_part(d, d.rows, d.Fin, 1, d.H, 2)),
-                            std::max(product_part(d, d.Fin, d.H, 2, d.rows, 1), product_part(d, d.H, d.Fout, 1, d.rows, 1))));
+  w->part = c.take(std::max(std::max(product_part(d, d.rows, Hp, 1, d.Fout, 1, true), product_part(d, d.rows, d.Fin, 1, d.H, 2, false)),
+                            std::max(product_part(d, d.Fin, d.H, 2, d.rows, 1, false), product_part(d, d.H, d.Fout, 1, d.rows, 1, false))));
   return c.off;
 }
 void zero(void* p, int64_t bytes, hipStream_t s) {
