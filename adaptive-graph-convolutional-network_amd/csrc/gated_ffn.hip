@@ -9,7 +9,8 @@
 //     reaches memory either: its epilogue reads P and Q and writes dG = dA P and dU = dA Q.  dX is one product over 2 H, dWg and
 //     dWu share X's tiles.
 //   * fp32 operands are split exactly into three bf16 pieces (bf16_split.h), and a product is the sum of six piece products (the
-//     dropped ones are below 2^-24): a stage holds the three planes of both operands, every fragment read serves two of them.
+//     dropped ones are below 2^-24).  Much work: planes of pieces in memory, a stage holds the three of both operands, and every
+//     fragment read serves two products.  Few rows or little work: fp32 in memory and LDS, split in registers.
 //   * Tiles go from memory to LDS directly (buffer_load .. lds, 16 bytes per lane), in two or three stages.  An operand whose rows
 //     run along k is read back with ds_read_b128, one whose rows run across k (weights in X W, both operands in X^T dG) with the
 //     transposing ds_read_b64_tr_b16: nothing is transposed in memory.  The 16-byte chunks of a tile row are permuted (xor with
@@ -38,7 +39,11 @@ typedef uint32_t u32x4h __attribute__((ext_vector_type(4), aligned(2)));
 
 enum { EPI_GATED = 0, EPI_STORE = 1, EPI_DH = 2 };
 
-struct Seg { const uint16_t *a, *b, *b2; };
+// How operands lie in memory: bf16 matrices, three bf16 planes of an fp32 one, or fp32 matrices that are split on the way to the
+// matrix pipe (few rows or little work: no launch for the planes, and a third of the bytes that they cost)
+enum { OP_BF16 = 1, OP_FP32 = 2, OP_PLANES = 3 };
+
+struct Seg { const void *a, *b, *b2; };
 
 struct GemmArgs {
   Seg seg[2];                        // the k loop runs over one or two products of the same sizes
@@ -50,13 +55,13 @@ struct GemmArgs {
   float* part;                       // splits > 1: [split][B matrix][M][ldp] fp32
   int32_t ldp;
   // epilogue
-  int32_t act, f32;
+  int32_t act, f32, op;
   int32_t ldh;                       // leading dimension of P, Q, A, dG, dU
   int64_t plane;                     // elements between the planes of A, dG, dU
   void *out, *out2;                  // EPI_STORE: [M, ldo]
   int32_t ldo;
   void *p, *q;                       // U act'(G) and act(G): f32, or 24 bits: [M, ldh] upper sixteen, then [M, ldh] lower eight
-  uint16_t *hid, *dg, *du;           // bf16 pieces
+  void *hid, *dg, *du;               // as the products read them (OP_*)
 };
 
 __device__ __forceinline__ uint32_t pk_bf(float a, float b) {
@@ -181,11 +186,14 @@ __device__ __forceinline__ F8 kept8(const Kept8<F32>& k) {
   }
   return x;
 }
-// the bf16 pieces of eight values (bf16 calls: the rounded values themselves)
+// eight values of a matrix that a later product reads
 template <bool F32>
-__device__ __forceinline__ void store8_pieces(const GemmArgs& g, uint16_t* p, int64_t at, const F8& x) {
+__device__ __forceinline__ void store8_operand(const GemmArgs& g, void* dst, int64_t at, const F8& x) {
+  uint16_t* p = static_cast<uint16_t*>(dst);
   if constexpr (!F32) {
     *reinterpret_cast<u32x4*>(p + at) = bf8(x);
+  } else if (g.op == OP_FP32) {
+    store8_f32(static_cast<float*>(dst) + at, x);
   } else {
     u32x4 h, m, l;
 #pragma unroll
@@ -252,7 +260,7 @@ __device__ __forceinline__ void epilogue(const GemmArgs& g, int m, int n, const 
       store8_kept<F32>(g, g.p, at, pv);
       store8_kept<F32>(g, g.q, at, qv);
     }
-    store8_pieces<F32>(g, g.hid, at, hv);
+    store8_operand<F32>(g, g.hid, at, hv);
   } else {
     const F8 pv = kept8<F32>(P), qv = kept8<F32>(Q);
     F8 dg, du;
@@ -261,27 +269,30 @@ __device__ __forceinline__ void epilogue(const GemmArgs& g, int m, int n, const 
       dg.v[i] = v0.v[i] * pv.v[i];
       du.v[i] = v0.v[i] * qv.v[i];
     }
-    store8_pieces<F32>(g, g.dg, at, dg);
-    store8_pieces<F32>(g, g.du, at, du);
+    store8_operand<F32>(g, g.dg, at, dg);
+    store8_operand<F32>(g, g.du, at, du);
   }
 }
 
 #ifdef __HIP_DEVICE_COMPILE__      // (address spaces and builtins that the host pass does not know)
-// The tiles of one operand in a stage: NMAT matrices of P planes, each ROWS rows of the operand (m or n) by BK.  T (transposed): the
-// operand's matrix is [k][rows].  Every wave issues kSlots loads of 64 chunks.
-template <int ROWS, bool T, int BK, int P, int NMAT, int WAVES>
+// The tiles of one operand in a stage: NMAT matrices of PL planes, each ROWS rows of the operand (m or n) by BK, ES bytes an element.
+// T (transposed): the operand's matrix is [k][rows].  Every wave issues kSlots loads of 64 chunks.
+template <int ROWS, bool T, int BK, int PL, int ES, int NMAT, int WAVES>
 struct Tiles {
-  static constexpr int kBytes = ROWS * BK * 2;                 // of one tile
+  static constexpr int kEpc = 16 / ES;                         // elements of a chunk
+  static constexpr int kRowBytes = (T ? ROWS : BK) * ES, kRowChunks = kRowBytes / 16;
+  static constexpr int kBytes = ROWS * BK * ES;                // of one tile
   static constexpr int kPerTile = kBytes / 1024;               // loads of a wave (1 KB) for one tile
-  static constexpr int kSlots = kPerTile * P * NMAT / WAVES;
-  static constexpr int kRowChunks = T ? ROWS / 8 : BK / 8;     // 16-byte chunks of a tile row
-  static_assert(kPerTile * P * NMAT % WAVES == 0 && kBytes % 1024 == 0, "whole loads per wave");
+  static constexpr int kSlots = kPerTile * PL * NMAT / WAVES;
+  static_assert(kPerTile * PL * NMAT % WAVES == 0 && kBytes % 1024 == 0, "whole loads per wave");
   int voff[kSlots], kl[kSlots];
 
   // Which chunk of row r lies where (an xor).  Rows along k: sixteen rows of one chunk in different 16-byte columns of the 256-byte
-  // bank line.  Rows across k: the four rows that sixteen lanes read, and the set eight rows on, in different 32-byte columns.
+  // bank line.  Rows across k, bf16: the four rows that sixteen lanes read, and the set eight rows on, in different 32-byte
+  // columns; fp32: the rows that the four sixteens of lanes read, eight apart, in different 64-byte columns.
   static __device__ __forceinline__ int perm(int r) {
-    if (!T) return BK == 64 ? (r >> 1) & 7 : (r >> 2) & 3;
+    if (!T) return kRowBytes == 128 ? (r >> 1) & 7 : (r >> 2) & 3;
+    if (ES == 4) return ((r >> 3) & 3) << 2 & (kRowChunks - 1);
     if (kRowChunks >= 16) return ((r & 3) | ((r >> 3) & 1) << 2) << 1;
     if (kRowChunks == 8) return (((r >> 1) & 1) | ((r >> 3) & 1) << 1) << 1;
     return ((r >> 3) & 1) << 1;
@@ -290,19 +301,19 @@ struct Tiles {
 #pragma unroll
     for (int i = 0; i < kSlots; ++i) {
       const int ci = ((wave * kSlots + i) % kPerTile) * 64 + lane, tr = ci / kRowChunks, c = (ci % kRowChunks) ^ perm(tr);
-      const int r = T ? c * 8 : tr, k = T ? tr : c * 8;
-      voff[i] = (T ? k * ld + r : r * ld + k) * 2;
+      const int r = T ? c * kEpc : tr, k = T ? tr : c * kEpc;
+      voff[i] = (T ? k * ld + r : r * ld + k) * ES;
       kl[i] = row0 + r < rows ? k : 0x7fffffff;
     }
   }
-  // k tile kt of the operand at p0 / p1 (its row or column row0 already added) into LDS; `left`: k that remain there
-  __device__ __forceinline__ void load(const uint16_t* p0, const uint16_t* p1, int64_t plane, int ld, int kt, int left, AGCN_LDS char* dst, int wave) const {
-    const int64_t kofs = T ? (int64_t)kt * BK * ld : (int64_t)kt * BK;
+  // k tile kt of the operand at p0 / p1, its row (T: column) row0 on, into LDS; `left`: k that remain there
+  __device__ __forceinline__ void load(const void* p0, const void* p1, int row0, int64_t plane, int ld, int kt, int left, AGCN_LDS char* dst, int wave) const {
+    const int64_t at = (T ? (int64_t)kt * BK * ld + row0 : (int64_t)row0 * ld + (int64_t)kt * BK) * ES;
 #pragma unroll
     for (int i = 0; i < kSlots; ++i) {
-      const int t = wave * kSlots + i, tile = t / kPerTile;    // tile: matrix * P + plane
-      const uint16_t* base = (NMAT == 2 && tile >= P ? p1 : p0) + (P == 1 ? 0 : (tile % P) * plane) + kofs;
-      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(base), 0, 0x7fffffff, 0x00020000);
+      const int t = wave * kSlots + i, tile = t / kPerTile;    // tile: matrix * PL + plane
+      const char* base = static_cast<const char*>(NMAT == 2 && tile >= PL ? p1 : p0) + (PL == 1 ? 0 : (tile % PL) * plane * ES) + at;
+      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, 0x7fffffff, 0x00020000);
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (AGCN_LDS void*)(dst + t * 1024), 16, kl[i] < left ? voff[i] : (int)0x80000000, 0, 0, 0);
     }
   }
@@ -313,38 +324,60 @@ struct Tiles {
   struct Reader {
     int at[T ? FR : 1], lane, row0;
     __device__ __forceinline__ Reader(int row, int lane_) : lane(lane_), row0(row) {
-      const int l = lane & 15, k = (lane >> 4) * 8 + (l >> 2);
+      const int l = lane & 15, q = lane >> 4, k = ES == 4 ? q * 8 : q * 8 + (l >> 2);
 #pragma unroll
       for (int f = 0; f < (T ? FR : 0); ++f) {
-        const int chunk = (((row + f * 16) >> 3) + ((l & 3) >> 1)) ^ perm(k);
-        at[f] = k * (ROWS * 2) + chunk * 16 + (l & 1) * 8;
+        // (fp32: a column's 32 bits; bf16: where the transposing read wants this lane to point, four columns of one k)
+        const int col = row + f * 16 + (ES == 4 ? l : (l & 3) * 4), chunk = (col / kEpc) ^ perm(k);
+        at[f] = k * kRowBytes + chunk * 16 + col % kEpc * ES;
         asm volatile("" : "+v"(at[f]));
       }
     }
+    // bf16 elements
     __device__ __forceinline__ u32x4 operator()(const AGCN_LDS char* s, int tile, int f, int kk) const {
       if (!T) {
         const int l = lane & 15, q = lane >> 4;
-        return *reinterpret_cast<const AGCN_LDS u32x4*>(s + tile * kBytes + (row0 + f * 16 + l) * (BK * 2) + (((kk * 4 + q) ^ perm(l)) << 4));
+        return *reinterpret_cast<const AGCN_LDS u32x4*>(s + tile * kBytes + (row0 + f * 16 + l) * kRowBytes + (((kk * 4 + q) ^ perm(l)) << 4));
       } else {
-        const AGCN_LDS char* p = s + at[f] + (tile * BK + kk * 32) * (ROWS * 2);
+        const AGCN_LDS char* p = s + at[f] + (tile * BK + kk * 32) * kRowBytes;
         const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((AGCN_LDS s16x4*)p);
-        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((AGCN_LDS s16x4*)(p + 4 * ROWS * 2));
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((AGCN_LDS s16x4*)(p + 4 * kRowBytes));
         const u32x2 a = __builtin_bit_cast(u32x2, lo), b = __builtin_bit_cast(u32x2, hi);
         return (u32x4){a.x, a.y, b.x, b.y};
       }
+    }
+    // fp32 elements, as their three pieces (BK == 32: one k step)
+    __device__ __forceinline__ Pieces pieces(const AGCN_LDS char* s, int tile, int f) const {
+      f32x4 lo, hi;
+      if (!T) {
+        const int l = lane & 15, q = lane >> 4;
+        const AGCN_LDS char* p = s + tile * kBytes + (row0 + f * 16 + l) * kRowBytes;
+        lo = *reinterpret_cast<const AGCN_LDS f32x4*>(p + (((q * 2) ^ perm(l)) << 4));
+        hi = *reinterpret_cast<const AGCN_LDS f32x4*>(p + (((q * 2 + 1) ^ perm(l)) << 4));
+      } else {
+        const AGCN_LDS char* p = s + at[f] + tile * kBytes;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          lo[i] = *reinterpret_cast<const AGCN_LDS float*>(p + i * kRowBytes);
+          hi[i] = *reinterpret_cast<const AGCN_LDS float*>(p + (4 + i) * kRowBytes);
+        }
+      }
+      return split3x8(lo, hi);
     }
   };
 };
 #endif
 
-// BM x (NB x BN) tile by WGM x WGN waves, P planes of pieces, S (2, 3) stages; AT / BT: the operand's matrix has k along its rows
-template <int P, int BM, int BN, int WGM, int WGN, bool AT, bool BT, int NB, int EPI, int S>
+// BM x (NB x BN) tile by WGM x WGN waves, operands as OP says, S (2, 3) stages; AT / BT: the operand's matrix has k along its rows
+template <int OP, int BM, int BN, int WGM, int WGN, bool AT, bool BT, int NB, int EPI, int S>
 __global__ __launch_bounds__(64 * WGM * WGN) void ffn_gemm_kernel(GemmArgs g) {
 #ifdef __HIP_DEVICE_COMPILE__
-  constexpr int WAVES = WGM * WGN, FM = BM / WGM / 16, FN = BN / WGN / 16, BK = P == 1 ? 64 : 32;
-  typedef Tiles<BM, AT, BK, P, 1, WAVES> TA;
-  typedef Tiles<BN, BT, BK, P, NB, WAVES> TB;
-  constexpr int SA = P * TA::kBytes, SB = NB * P * TB::kBytes;
+  constexpr int WAVES = WGM * WGN, FM = BM / WGM / 16, FN = BN / WGN / 16, BK = OP == OP_BF16 ? 64 : 32;
+  constexpr int PL = OP == OP_PLANES ? 3 : 1, ES = OP == OP_FP32 ? 4 : 2, P = OP == OP_BF16 ? 1 : 3;      // planes; element's bytes; pieces
+  constexpr bool F32 = OP != OP_BF16;
+  typedef Tiles<BM, AT, BK, PL, ES, 1, WAVES> TA;
+  typedef Tiles<BN, BT, BK, PL, ES, NB, WAVES> TB;
+  constexpr int SA = PL * TA::kBytes, SB = NB * PL * TB::kBytes;
   // (arrays of their own for every stage and operand: the compiler then sees that the loads into one do not touch the reads of
   // another; it would wait for all loads in flight otherwise)
   __shared__ __attribute__((aligned(1024))) char sa0[SA], sa1[SA], sa2[S > 2 ? SA : 16];
@@ -369,7 +402,6 @@ __global__ __launch_bounds__(64 * WGM * WGN) void ffn_gemm_kernel(GemmArgs g) {
   TB tb;
   ta.init(m0, g.M, g.lda, wave, lane);
   tb.init(n0, g.N, g.ldb, wave, lane);
-  const int64_t a_at = AT ? m0 : (int64_t)m0 * g.lda, b_at = BT ? n0 : (int64_t)n0 * g.ldb;
 
   const int iters = g.nseg * g.ktiles;
   const int it0 = (int)((int64_t)iters * split / g.splits), it1 = (int)((int64_t)iters * (split + 1) / g.splits);
@@ -380,8 +412,8 @@ __global__ __launch_bounds__(64 * WGM * WGN) void ffn_gemm_kernel(GemmArgs g) {
   auto load = [&](AGCN_LDS char* a, AGCN_LDS char* b) {
     const Seg s = g.seg[seg < 2 ? seg : 1];
     const int left = lit < it1 ? g.K - kt * BK : 0;
-    ta.load(s.a + a_at, nullptr, g.a_plane, g.lda, kt, left, a, wave);
-    tb.load(s.b + b_at, NB == 2 ? s.b2 + b_at : nullptr, g.b_plane, g.ldb, kt, left, b, wave);
+    ta.load(s.a, nullptr, m0, g.a_plane, g.lda, kt, left, a, wave);
+    tb.load(s.b, s.b2, n0, g.b_plane, g.ldb, kt, left, b, wave);
     ++lit;
     if (++kt == g.ktiles) { kt = 0; ++seg; }
   };
@@ -398,14 +430,29 @@ __global__ __launch_bounds__(64 * WGM * WGN) void ffn_gemm_kernel(GemmArgs g) {
 #pragma unroll
     for (int kk = 0; kk < BK / 32; ++kk) {
       u32x4 fa[P][FM], fb[P][NB][FN];
+      if constexpr (OP == OP_FP32) {
 #pragma unroll
-      for (int p = 0; p < P; ++p) {
-#pragma unroll
-        for (int i = 0; i < FM; ++i) fa[p][i] = ra(a, p, i, kk);
+        for (int i = 0; i < FM; ++i) {
+          const Pieces x = ra.pieces(a, 0, i);
+          fa[0][i] = x.h; fa[1][i] = x.m; fa[2][i] = x.l;
+        }
 #pragma unroll
         for (int c = 0; c < NB; ++c)
 #pragma unroll
-          for (int j = 0; j < FN; ++j) fb[p][c][j] = rb(b, c * P + p, j, kk);
+          for (int j = 0; j < FN; ++j) {
+            const Pieces x = rb.pieces(b, c, j);
+            fb[0][c][j] = x.h; fb[1][c][j] = x.m; fb[2][c][j] = x.l;
+          }
+      } else {
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+#pragma unroll
+          for (int i = 0; i < FM; ++i) fa[p][i] = ra(a, p, i, kk);
+#pragma unroll
+          for (int c = 0; c < NB; ++c)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) fb[p][c][j] = rb(b, c * P + p, j, kk);
+        }
       }
       // (B as the first operand: a lane then holds four neighbouring COLUMNS of one row of the result.  Pieces: small terms first)
       constexpr int NP = P == 1 ? 1 : 6;
@@ -496,14 +543,14 @@ __global__ __launch_bounds__(64 * WGM * WGN) void ffn_gemm_kernel(GemmArgs g) {
     const int c8 = lane % LPR, n = n_wave + c8 * 8;
 #pragma unroll 1
     for (int r0 = 0; r0 < PR; r0 += RPI * UN) {
-      Kept8<P == 3> kp[UN], kq[UN];
+      Kept8<F32> kp[UN], kq[UN];
       if (EPI == EPI_DH && g.splits == 1) {
 #pragma unroll
         for (int u = 0; u < UN; ++u) {
           const int m = m0 + wm * FM * 16 + ps * PR + r0 + u * RPI + lane / LPR;
           if (m < g.M && n < g.ldh) {
-            fetch8_kept<P == 3>(g, g.p, (int64_t)m * g.ldh + n, kp[u]);
-            fetch8_kept<P == 3>(g, g.q, (int64_t)m * g.ldh + n, kq[u]);
+            fetch8_kept<F32>(g, g.p, (int64_t)m * g.ldh + n, kp[u]);
+            fetch8_kept<F32>(g, g.q, (int64_t)m * g.ldh + n, kq[u]);
           }
         }
       }
@@ -526,7 +573,7 @@ __global__ __launch_bounds__(64 * WGM * WGN) void ffn_gemm_kernel(GemmArgs g) {
               if (NB == 2) store8_f32(p + (int64_t)g.M * g.ldp, v[NB - 1]);
             }
           } else {
-            epilogue<EPI, NB, P == 3>(g, m, n, v[0], v[NB - 1], kp[u], kq[u]);
+            epilogue<EPI, NB, F32>(g, m, n, v[0], v[NB - 1], kp[u], kq[u]);
           }
         }
       }
@@ -580,7 +627,7 @@ __global__ __launch_bounds__(256) void ffn_reduce_kernel(GemmArgs g) {
 
 // Operand images: bf16 matrices whose rows do not start at 16 bytes or end at eights, padded with zeros; fp32 ones as three planes of
 // bf16 pieces.  One launch for all matrices of a call; a thread makes eight columns.
-struct Image { const void* src; uint16_t* dst; int64_t rows, plane, chunk0; int32_t cols, ld_src, ld_dst, f32; };
+struct Image { const void* src; void* dst; int64_t rows, plane, chunk0; int32_t cols, ld_src, ld_dst, f32; /* 1: as planes, 2: as it is */ };
 struct ImageArgs { Image im[4]; int32_t n; int64_t chunks; };
 __global__ __launch_bounds__(256) void ffn_image_kernel(ImageArgs a) {
   const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -590,7 +637,7 @@ __global__ __launch_bounds__(256) void ffn_image_kernel(ImageArgs a) {
   const Image& im = a.im[k];
   const int64_t at = e - im.chunk0, per = im.ld_dst >> 3, r = at / per;
   const int c = (int)(at - r * per) * 8;
-  uint16_t* dst = im.dst + r * im.ld_dst + c;
+  uint16_t* dst = static_cast<uint16_t*>(im.dst) + r * im.ld_dst + c;
   if (im.f32) {
     const float* p = static_cast<const float*>(im.src) + r * im.ld_src + c;
     float v[8];
@@ -601,6 +648,12 @@ __global__ __launch_bounds__(256) void ffn_image_kernel(ImageArgs a) {
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = c + i < im.cols ? p[i] : 0.f;
+    }
+    if (im.f32 == 2) {          // (as they are: rows that do not start at 16 bytes)
+      float* d = static_cast<float*>(im.dst) + r * im.ld_dst + c;
+      *reinterpret_cast<f32x4*>(d) = (f32x4){v[0], v[1], v[2], v[3]};
+      *reinterpret_cast<f32x4*>(d + 4) = (f32x4){v[4], v[5], v[6], v[7]};
+      return;
     }
     u32x4 h, m, l;
 #pragma unroll
@@ -635,8 +688,8 @@ __global__ __launch_bounds__(256) void ffn_zero_kernel(void* p, int64_t bytes) {
 inline int pad8(int v) { return (v + 7) & ~7; }
 inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// A matrix as the products read it: its own memory where that is bf16 with rows at 16 bytes, an image otherwise
-struct Mat { const uint16_t* p; int32_t ld; int64_t plane; };
+// A matrix as the products read it: its own memory, or an image of it
+struct Mat { const void* p; int32_t ld; int64_t plane; };
 
 struct Carve {
   char* base;
@@ -648,50 +701,60 @@ struct Carve {
   }
 };
 
+// How an fp32 call lays its operands out, by its sizes alone (the backward has to come to the same answer): as they are while few
+// rows meet many weights -- the planes of 2048 x 8001 weights cost 150 us, more than 16 rows' whole pass over them -- or the work is
+// little; as planes otherwise, which the matrix pipe reads faster.
+int op_of(const AgcnFfnDesc& d) {
+  if (d.dtype == AGCN_DTYPE_BF16) return OP_BF16;
+  return d.rows <= 128 || d.rows * (int64_t)d.H * (d.Fin + d.Fout) <= (int64_t)160 << 20 ? OP_FP32 : OP_PLANES;
+}
+// read in place: rows at 16 bytes, whole chunks
 bool direct(const AgcnFfnDesc& d, const void* p, int cols, int ld) {
-  return d.dtype == AGCN_DTYPE_BF16 && cols % 8 == 0 && ld % 8 == 0 && ((uintptr_t)p & 15) == 0;
+  const int epc = d.dtype == AGCN_DTYPE_BF16 ? 8 : 4;
+  return op_of(d) != OP_PLANES && cols % epc == 0 && ld % epc == 0 && ((uintptr_t)p & 15) == 0;
 }
 
 // What the forward leaves for the backward.  The images are there only where a matrix cannot be read as it is; room is kept for
 // them whenever the SIZES alone would not rule them out (an address can be odd).
-struct Reserve { uint16_t *x, *wg, *wu, *wd, *hid; void *p, *q; };
+struct Reserve { void *x, *wg, *wu, *wd, *hid, *p, *q; };
 size_t carve_reserve(const AgcnFfnDesc& d, void* mem, Reserve* r) {
   Carve c{static_cast<char*>(mem), 0};
-  const int P = d.dtype == AGCN_DTYPE_F32 ? 3 : 1, Hp = pad8(d.H), Fp = pad8(d.Fin), Op = pad8(d.Fout);
-  const size_t e = d.dtype == AGCN_DTYPE_F32 ? 4 : 3;
-  r->x = static_cast<uint16_t*>(c.take((size_t)P * d.rows * Fp * 2));
-  r->wg = static_cast<uint16_t*>(c.take((size_t)P * d.Fin * Hp * 2));
-  r->wu = static_cast<uint16_t*>(c.take((size_t)P * d.Fin * Hp * 2));
-  r->wd = static_cast<uint16_t*>(c.take((size_t)P * d.H * Op * 2));
-  r->hid = static_cast<uint16_t*>(c.take((size_t)P * d.rows * Hp * 2));
-  r->p = d.training ? c.take(e * d.rows * Hp) : nullptr;
-  r->q = d.training ? c.take(e * d.rows * Hp) : nullptr;
+  const int op = op_of(d), Hp = pad8(d.H), Fp = pad8(d.Fin), Op = pad8(d.Fout);
+  const size_t e = op == OP_BF16 ? 2 : op == OP_FP32 ? 4 : 6, kept = d.dtype == AGCN_DTYPE_F32 ? 4 : 3;
+  r->x = c.take(e * d.rows * Fp);
+  r->wg = c.take(e * d.Fin * Hp);
+  r->wu = c.take(e * d.Fin * Hp);
+  r->wd = c.take(e * d.H * Op);
+  r->hid = c.take(e * d.rows * Hp);
+  r->p = d.training ? c.take(kept * d.rows * Hp) : nullptr;
+  r->q = d.training ? c.take(kept * d.rows * Hp) : nullptr;
   return c.off;
 }
 
 // Tile of a product, its splits, and the kernel's stages: 0 large (256 x 256; three planes: 256 x 128), 1 middle (128 x 128; 128 x 64),
-// 2 small (64 x 64; two B matrices: 64 of each; three planes: 32 of each).
+// 2 small (64 x 64; two B matrices: 64 of each; fp32: 32 of each).
 struct Config { int kind, bm, bn, splits; };      // bn: columns of one B matrix
-Config tile_of(int kind, int planes, int nb, int splits) {
-  if (kind == 0) return {0, 256, (planes == 1 ? 256 : 128) / nb, splits};
-  if (kind == 1) return {1, 128, (planes == 1 ? 128 : 64) / nb, splits};
-  return {2, 64, planes == 1 ? 64 : 64 / nb, splits};
+Config tile_of(int kind, int op, int nb, int splits) {
+  if (kind == 0) return {0, 256, (op == OP_BF16 ? 256 : 128) / nb, splits};
+  if (kind == 1) return {1, 128, (op == OP_BF16 ? 128 : 64) / nb, splits};
+  return {2, 64, op == OP_BF16 ? 64 : 64 / nb, splits};
 }
 // The choice: the least time by a model of the chip's 256 CUs.  per_it[w - 1]: a k stage with w workgroups on the CU (the large tile's
 // 8 waves fill it; two middle or two to three small ones share it), fixed: a tile's first loads and its epilogue -- microseconds,
 // measured on 5003 x 1001 x 2731 (bf16) and 32768 x 128 x 512 (fp32) with every kind in turn: e.g. X^T dG, 344 middle tiles of 79
 // stages 84 us, 172 large ones in two splits 82 + 17, small ones 105; A^T dY, 176 middle tiles 70 us, in two splits 54 + 9.
 // Splits cost their fp32 tiles' way to memory and back (4 MB a microsecond; half that through the gates' epilogues).
-Config choose(int64_t M, int64_t N, int nb, int planes, int64_t iters, bool gates) {
+Config choose(int64_t M, int64_t N, int nb, int op, int64_t iters, bool gates) {
   struct Cost { float per_it[3], fixed; int at_once, most; };
   static const Cost kBf16[3] = {{{2.0f, 0.f, 0.f}, 8.f, 1, 4}, {{0.82f, 1.08f, 0.f}, 6.f, 2, 8}, {{0.45f, 0.65f, 0.86f}, 4.f, 3, 64}};
   static const Cost kF32[3] = {{{2.8f, 0.f, 0.f}, 8.f, 1, 4}, {{1.0f, 1.6f, 0.f}, 5.f, 2, 8}, {{0.6f, 0.9f, 0.f}, 4.f, 2, 64}};
-  Config best = tile_of(2, planes, nb, 1);
+  static const Cost kWhole = {{0.6f, 0.8f, 1.0f}, 4.f, 3, 64};
+  Config best = tile_of(2, op, nb, 1);
   float least = 1e30f;
-  for (int kind = 0; kind < 3; ++kind) {
-    const Cost& k = planes == 1 ? kBf16[kind] : kF32[kind];
-    const int at_once = kind == 2 && nb == 2 ? 2 : k.at_once;            // (the LDS of two B matrices: two workgroups)
-    const Config c = tile_of(kind, planes, nb, 1);
+  for (int kind = op == OP_FP32 ? 2 : 0; kind < 3; ++kind) {              // (fp32 operands: the small tile alone)
+    const Cost& k = op == OP_BF16 ? kBf16[kind] : op == OP_FP32 ? kWhole : kF32[kind];
+    const int at_once = kind == 2 && nb == 2 && op == OP_BF16 ? 2 : k.at_once;            // (the LDS of two B matrices: two workgroups)
+    const Config c = tile_of(kind, op, nb, 1);
     const int64_t tiles = std::max<int64_t>(1, cdiv(M, c.bm) * cdiv(N, c.bn));     // (size queries come here with no rows, too)
     for (int s = 1; s <= k.most && s <= std::max<int64_t>(1, iters / 2); s += s < 8 ? 1 : 4) {
       const int64_t per_cu = cdiv(tiles * s, 256), its = cdiv(iters, s);
@@ -701,7 +764,7 @@ Config choose(int64_t M, int64_t N, int nb, int planes, int64_t iters, bool gate
       if (s > 1) t += 4.f + (float)s * nb * M * N * 8.f / (gates ? 2e6f : 4e6f);
       if (t < least) {
         least = t;
-        best = tile_of(kind, planes, nb, s);
+        best = tile_of(kind, op, nb, s);
       }
     }
   }
@@ -711,34 +774,34 @@ Config choose(int64_t M, int64_t N, int nb, int planes, int64_t iters, bool gate
 size_t part_bytes(const Config& c, int64_t M, int64_t N, int nb) {
   return c.splits > 1 ? (size_t)c.splits * nb * M * ((N + 7) & ~7ll) * sizeof(float) : 0;
 }
-int planes_of(const AgcnFfnDesc& d) { return d.dtype == AGCN_DTYPE_F32 ? 3 : 1; }
 int64_t ktiles_of(const AgcnFfnDesc& d, int64_t K) { return cdiv(K, d.dtype == AGCN_DTYPE_F32 ? 32 : 64); }
 
-template <int P, int BM, int BN, int WGM, int WGN, bool AT, bool BT, int NB, int EPI, int S>
+template <int OP, int BM, int BN, int WGM, int WGN, bool AT, bool BT, int NB, int EPI, int S>
 void launch_tile(const GemmArgs& g, hipStream_t s) {
   const int64_t total = (int64_t)g.tiles_m * g.tiles_n * g.splits;
-  hipLaunchKernelGGL((ffn_gemm_kernel<P, BM, BN, WGM, WGN, AT, BT, NB, EPI, S>), dim3((unsigned)(cdiv(total, 8) * 8)), dim3(64 * WGM * WGN), 0, s, g);
+  hipLaunchKernelGGL((ffn_gemm_kernel<OP, BM, BN, WGM, WGN, AT, BT, NB, EPI, S>), dim3((unsigned)(cdiv(total, 8) * 8)), dim3(64 * WGM * WGN), 0, s, g);
 }
 
 template <bool AT, bool BT, int NB, int EPI>
 void product(GemmArgs& g, void* part, hipStream_t s) {
-  const int planes = g.f32 ? 3 : 1;
   g.ktiles = (int)cdiv(g.K, g.f32 ? 32 : 64);
   const int n_all = EPI == EPI_STORE ? g.N : g.ldh;         // columns that the epilogue has to reach
-  const Config c = choose(g.M, n_all, NB, planes, (int64_t)g.nseg * g.ktiles, EPI != EPI_STORE);
+  const Config c = choose(g.M, n_all, NB, g.op, (int64_t)g.nseg * g.ktiles, EPI != EPI_STORE);
   g.tiles_m = (int)cdiv(g.M, c.bm); g.tiles_n = (int)cdiv(n_all, c.bn); g.splits = c.splits;
   g.part = static_cast<float*>(part); g.ldp = (n_all + 7) & ~7;
-  if (planes == 1) {
-    if (c.kind == 0) launch_tile<1, 256, 256 / NB, 2, 4, AT, BT, NB, EPI, 2>(g, s);
-    else if (c.kind == 1) launch_tile<1, 128, 128 / NB, 2, 2, AT, BT, NB, EPI, 2>(g, s);
-    else launch_tile<1, 64, 64, 2, 2, AT, BT, NB, EPI, 3>(g, s);
+  if (g.op == OP_BF16) {
+    if (c.kind == 0) launch_tile<OP_BF16, 256, 256 / NB, 2, 4, AT, BT, NB, EPI, 2>(g, s);
+    else if (c.kind == 1) launch_tile<OP_BF16, 128, 128 / NB, 2, 2, AT, BT, NB, EPI, 2>(g, s);
+    else launch_tile<OP_BF16, 64, 64, 2, 2, AT, BT, NB, EPI, 3>(g, s);
+  } else if (g.op == OP_PLANES) {
+    if (c.kind == 0) launch_tile<OP_PLANES, 256, 128 / NB, 4, 2, AT, BT, NB, EPI, 2>(g, s);
+    else if (c.kind == 1) launch_tile<OP_PLANES, 128, 64 / NB, 2, 2, AT, BT, NB, EPI, 2>(g, s);
+    else launch_tile<OP_PLANES, 64, 64 / NB, 2, 2, AT, BT, NB, EPI, 3>(g, s);
   } else {
-    if (c.kind == 0) launch_tile<3, 256, 128 / NB, 4, 2, AT, BT, NB, EPI, 2>(g, s);
-    else if (c.kind == 1) launch_tile<3, 128, 64 / NB, 2, 2, AT, BT, NB, EPI, 2>(g, s);
-    else launch_tile<3, 64, 64 / NB, 2, 2, AT, BT, NB, EPI, 3>(g, s);
+    launch_tile<OP_FP32, 64, 64 / NB, 2, 2, AT, BT, NB, EPI, 3>(g, s);
   }
   const dim3 rg((unsigned)cdiv((int64_t)g.M * (g.ldp / 8), 32));
-  if (g.splits > 1 && planes == 1) hipLaunchKernelGGL((ffn_reduce_kernel<NB, EPI, false>), rg, dim3(256), 0, s, g);
+  if (g.splits > 1 && !g.f32) hipLaunchKernelGGL((ffn_reduce_kernel<NB, EPI, false>), rg, dim3(256), 0, s, g);
   else if (g.splits > 1) hipLaunchKernelGGL((ffn_reduce_kernel<NB, EPI, true>), rg, dim3(256), 0, s, g);
 }
 
@@ -761,49 +824,56 @@ int check_ffn(const AgcnFfnDesc* d, const char* who) {
   return AGCN_OK;
 }
 
+// which operands are read in place; both projections or neither: they have one leading dimension
+struct InPlace {
+  bool x, w, wd;
+  InPlace(const AgcnFfnDesc& d, const void* X, const void* Wg, const void* Wu, const void* Wd)
+      : x(direct(d, X, d.Fin, d.ldx)), w(direct(d, Wg, d.H, d.H) && direct(d, Wu, d.H, d.H)), wd(direct(d, Wd, d.Fout, d.Fout)) {}
+};
+
 struct ImageList {
   ImageArgs a;
   ImageList() { std::memset(&a, 0, sizeof(a)); }
-  Mat add(const AgcnFfnDesc& d, const void* src, int64_t rows, int cols, int ld, uint16_t* dst) {
-    if (direct(d, src, cols, ld)) return {static_cast<const uint16_t*>(src), ld, 0};
-    const bool f32 = d.dtype == AGCN_DTYPE_F32;
-    const int lp = pad8(cols);
+  Mat add(const AgcnFfnDesc& d, const void* src, int64_t rows, int cols, int ld, void* dst, bool in_place) {
+    if (in_place) return {src, ld, 0};
+    const int lp = pad8(cols), op = op_of(d);
     Image& im = a.im[a.n++];
-    im = {src, dst, rows, rows * lp, a.chunks, cols, ld, lp, f32 ? 1 : 0};
+    im = {src, dst, rows, rows * lp, a.chunks, cols, ld, lp, op == OP_BF16 ? 0 : op == OP_FP32 ? 2 : 1};
     a.chunks += rows * (lp >> 3);
-    return {dst, lp, f32 ? im.plane : 0};
+    return {dst, lp, op == OP_PLANES ? im.plane : 0};
   }
   void launch(hipStream_t s) const {
     if (a.chunks) hipLaunchKernelGGL(ffn_image_kernel, dim3((unsigned)cdiv(a.chunks, 256)), dim3(256), 0, s, a);
   }
 };
 // the same matrix in the backward, whose image the forward has left
-Mat same(const AgcnFfnDesc& d, const void* src, int64_t rows, int cols, int ld, uint16_t* img) {
-  if (direct(d, src, cols, ld)) return {static_cast<const uint16_t*>(src), ld, 0};
-  return {img, pad8(cols), d.dtype == AGCN_DTYPE_F32 ? rows * pad8(cols) : 0};
+Mat same(const AgcnFfnDesc& d, const void* src, int64_t rows, int cols, int ld, const void* img, bool in_place) {
+  if (in_place) return {src, ld, 0};
+  return {img, pad8(cols), op_of(d) == OP_PLANES ? rows * pad8(cols) : 0};
 }
 
 GemmArgs base_args(const AgcnFfnDesc& d) {
   GemmArgs g;
   std::memset(&g, 0, sizeof(g));
-  g.act = d.activation; g.f32 = d.dtype == AGCN_DTYPE_F32;
+  g.act = d.activation; g.f32 = d.dtype == AGCN_DTYPE_F32; g.op = op_of(d);
   g.ldh = pad8(d.H); g.plane = (int64_t)d.rows * g.ldh;
   return g;
 }
 
 size_t product_part(const AgcnFfnDesc& d, int64_t M, int64_t N, int nb, int64_t K, int nseg, bool gates) {
-  return part_bytes(choose(M, N, nb, planes_of(d), nseg * ktiles_of(d, K), gates), M, N, nb);
+  return part_bytes(choose(M, N, nb, op_of(d), nseg * ktiles_of(d, K), gates), M, N, nb);
 }
 size_t forward_part(const AgcnFfnDesc& d) {
   return std::max(product_part(d, d.rows, pad8(d.H), 2, d.Fin, 1, true), product_part(d, d.rows, d.Fout, 1, d.H, 1, false));
 }
-struct BackWs { uint16_t *dy, *dg, *du; void* part; };
+struct BackWs { void *dy, *dg, *du, *part; };
 size_t carve_backward(const AgcnFfnDesc& d, void* mem, BackWs* w) {
-  const int P = planes_of(d), Hp = pad8(d.H);
+  const int op = op_of(d), Hp = pad8(d.H);
+  const size_t e = op == OP_BF16 ? 2 : op == OP_FP32 ? 4 : 6;
   Carve c{static_cast<char*>(mem), 0};
-  w->dy = static_cast<uint16_t*>(c.take((size_t)P * d.rows * pad8(d.Fout) * 2));
-  w->dg = static_cast<uint16_t*>(c.take((size_t)P * d.rows * Hp * 2));
-  w->du = static_cast<uint16_t*>(c.take((size_t)P * d.rows * Hp * 2));
+  w->dy = c.take(e * d.rows * pad8(d.Fout));
+  w->dg = c.take(e * d.rows * Hp);
+  w->du = c.take(e * d.rows * Hp);
   w->part = c.take(std::max(std::max(product_part(d, d.rows, Hp, 1, d.Fout, 1, true), product_part(d, d.rows, d.Fin, 1, d.H, 2, false)),
                             std::max(product_part(d, d.Fin, d.H, 2, d.rows, 1, false), product_part(d, d.H, d.Fout, 1, d.rows, 1, false))));
   return c.off;
@@ -849,17 +919,16 @@ extern "C" int agcn_gated_ffn_forward(const AgcnFfnDesc* desc, const void* X, co
     return fail(AGCN_ENOSPACE, "%s: workspace too small or not at 256 bytes (%zu < %zu)", who, workspace_bytes, wneed);
   hipStream_t s = static_cast<hipStream_t>(hip_stream);
   ImageList list;
-  const Mat x = list.add(d, X, d.rows, d.Fin, d.ldx, r.x), wg = list.add(d, Wg, d.Fin, d.H, d.H, r.wg);
-  // (read in place or as an image, both projections have one leading dimension: in place only if H is a multiple of eight)
-  const Mat wu = list.add(d, Wu, d.Fin, d.H, d.H, r.wu);
-  const Mat wd = list.add(d, Wd, d.H, d.Fout, d.Fout, r.wd);
+  const InPlace in(d, X, Wg, Wu, Wd);
+  const Mat x = list.add(d, X, d.rows, d.Fin, d.ldx, r.x, in.x), wg = list.add(d, Wg, d.Fin, d.H, d.H, r.wg, in.w),
+            wu = list.add(d, Wu, d.Fin, d.H, d.H, r.wu, in.w), wd = list.add(d, Wd, d.H, d.Fout, d.Fout, r.wd, in.wd);
   list.launch(s);
   GemmArgs g = base_args(d);
   operands(&g, x, wg, &wu);
   g.M = (int)d.rows; g.N = d.H; g.K = d.Fin;
   g.p = r.p; g.q = r.q; g.hid = r.hid;
   product<false, true, 2, EPI_GATED>(g, workspace, s);
-  const Mat hid = {r.hid, g.ldh, g.f32 ? g.plane : 0};
+  const Mat hid = {r.hid, g.ldh, g.op == OP_PLANES ? g.plane : 0};
   GemmArgs q = base_args(d);
   operands(&q, hid, wd, nullptr);
   q.M = (int)d.rows; q.N = d.Fout; q.K = d.H;
@@ -896,13 +965,14 @@ extern "C" int agcn_gated_ffn_backward(const AgcnFfnDesc* desc, const void* X, c
     return fail(AGCN_ENOSPACE, "%s: reserve too small or not at 256 bytes (%zu < %zu)", who, reserve_bytes, need);
   if (!workspace || ((uintptr_t)workspace & 255) || workspace_bytes < wneed)
     return fail(AGCN_ENOSPACE, "%s: workspace too small or not at 256 bytes (%zu < %zu)", who, workspace_bytes, wneed);
-  const Mat x = same(d, X, d.rows, d.Fin, d.ldx, r.x), wg = same(d, Wg, d.Fin, d.H, d.H, r.wg), wu = same(d, Wu, d.Fin, d.H, d.H, r.wu),
-            wd = same(d, Wd, d.H, d.Fout, d.Fout, r.wd);
+  const InPlace in(d, X, Wg, Wu, Wd);
+  const Mat x = same(d, X, d.rows, d.Fin, d.ldx, r.x, in.x), wg = same(d, Wg, d.Fin, d.H, d.H, r.wg, in.w),
+            wu = same(d, Wu, d.Fin, d.H, d.H, r.wu, in.w), wd = same(d, Wd, d.H, d.Fout, d.Fout, r.wd, in.wd);
   ImageList list;
-  const Mat dy = list.add(d, dY, d.rows, d.Fout, d.Fout, w.dy);
+  const Mat dy = list.add(d, dY, d.rows, d.Fout, d.Fout, w.dy, direct(d, dY, d.Fout, d.Fout));
   list.launch(s);
   GemmArgs base = base_args(d);
-  const int64_t pl = base.f32 ? base.plane : 0;
+  const int64_t pl = base.op == OP_PLANES ? base.plane : 0;
   const Mat hid = {r.hid, base.ldh, pl}, dg = {w.dg, base.ldh, pl}, du = {w.du, base.ldh, pl};
   if (dX || dWg) {
     GemmArgs g = base;                        // dA = dY Wd^T, and from it dG and dU

@@ -116,8 +116,8 @@ def check_exact(amd, args, dtype):
 
 
 # rows, F, H, F_out: one of everything, odd sizes, sizes around the tiles' edges, and (last) each of the kernel's tile shapes
-SMALL = [(1, 1, 1, 1), (1, 64, 128, 64), (7, 75, 33, 12), (18, 64, 256, 64), (63, 65, 66, 67), (65, 8, 7, 9), (130, 200, 129, 257), (300, 128, 512, 128)]
-LARGE = [(4608, 64, 256, 64), (4100, 257, 1000, 250), (8200, 1500, 4200, 1500), (5003, 1001, 2731, 1001), (1, 2048, 8192, 2048), (40000, 30, 50, 20)]
+SMALL = [(1, 1, 1, 1), (1, 64, 128, 64), (7, 75, 33, 12), (18, 64, 256, 64), (63, 65, 66, 67), (65, 8, 7, 9), (130, 200, 129, 257), (300, 128, 512, 128), (100, 36, 44, 28)]
+LARGE = [(4608, 64, 256, 64), (4100, 257, 1000, 250), (8200, 1500, 4200, 1500), (5003, 1001, 2731, 1001), (1, 2048, 8192, 2048), (40000, 30, 50, 20), (128, 516, 2052, 260), (129, 1024, 2052, 512)]
 
 
 @pytest.mark.gpu
@@ -176,8 +176,9 @@ def test_a_row_that_is_not_finite_stays_alone(amd):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [f32, bf16])
-def test_strides_alignment_and_what_lies_around(amd, dtype):
-    M, F, H, O = 70, 64, 96, 72
+@pytest.mark.parametrize("size", [(70, 64, 96, 72), (70, 68, 100, 76), (1500, 68, 1100, 76)])
+def test_strides_alignment_and_what_lies_around(amd, dtype, size):
+    M, F, H, O = size
     X, Wg, Wu, Wd, dY = integers(11, M, F, H, O, dtype)
     out, _, _ = reference(X, Wg, Wu, Wd, dY, "relu", dtype)
     wide = torch.full((M, F + 9), float("nan"), dtype=dtype, device="cuda")
