@@ -41,7 +41,8 @@ enum { EPI_GATED = 0, EPI_STORE = 1, EPI_DH = 2 };
 
 // How operands lie in memory: bf16 matrices, three bf16 planes of an fp32 one, or fp32 matrices that are split on the way to the
 // matrix pipe (few rows or little work: no launch for the planes, and a third of the bytes that they cost)
-enum { OP_BF16 = 1, OP_FP32 = 2, OP_PLANES = 3 };
+// (OP_WORDS: OP_FP32 whose rows do not start at 16 bytes or end in whole chunks; it is loaded into LDS four bytes a lane)
+enum { OP_BF16 = 1, OP_FP32 = 2, OP_PLANES = 3, OP_WORDS = 4 };
 
 struct Seg { const void *a, *b, *b2; };
 
@@ -55,7 +56,7 @@ struct GemmArgs {
   float* part;                       // splits > 1: [split][B matrix][M][ldp] fp32
   int32_t ldp;
   // epilogue
-  int32_t act, f32, op;
+  int32_t act, f32, op, words;       // words: OP_FP32 as OP_WORDS
   int32_t ldh;                       // leading dimension of P, Q, A, dG, dU
   int64_t plane;                     // elements between the planes of A, dG, dU
   void *out, *out2;                  // EPI_STORE: [M, ldo]
@@ -276,15 +277,15 @@ __device__ __forceinline__ void epilogue(const GemmArgs& g, int m, int n, const 
 
 #ifdef __HIP_DEVICE_COMPILE__      // (address spaces and builtins that the host pass does not know)
 // The tiles of one operand in a stage: NMAT matrices of PL planes, each ROWS rows of the operand (m or n) by BK, ES bytes an element.
-// T (transposed): the operand's matrix is [k][rows].  Every wave issues kSlots loads of 64 chunks.
-template <int ROWS, bool T, int BK, int PL, int ES, int NMAT, int WAVES>
+// T (transposed): the operand's matrix is [k][rows].  Every wave issues kSlots loads of 64 x LB bytes.
+template <int ROWS, bool T, int BK, int PL, int ES, int LB, int NMAT, int WAVES>
 struct Tiles {
   static constexpr int kEpc = 16 / ES;                         // elements of a chunk
   static constexpr int kRowBytes = (T ? ROWS : BK) * ES, kRowChunks = kRowBytes / 16;
   static constexpr int kBytes = ROWS * BK * ES;                // of one tile
-  static constexpr int kPerTile = kBytes / 1024;               // loads of a wave (1 KB) for one tile
+  static constexpr int kPerTile = kBytes / (64 * LB);          // loads of a wave for one tile
   static constexpr int kSlots = kPerTile * PL * NMAT / WAVES;
-  static_assert(kPerTile * PL * NMAT % WAVES == 0 && kBytes % 1024 == 0, "whole loads per wave");
+  static_assert(kPerTile * PL * NMAT % WAVES == 0 && kBytes % (64 * LB) == 0, "whole loads per wave");
   int voff[kSlots], kl[kSlots];
 
   // Which chunk of row r lies where (an xor).  Rows along k: sixteen rows of one chunk in different 16-byte columns of the 256-byte
@@ -300,8 +301,9 @@ struct Tiles {
   __device__ __forceinline__ void init(int row0, int rows, int ld, int wave, int lane) {
 #pragma unroll
     for (int i = 0; i < kSlots; ++i) {
-      const int ci = ((wave * kSlots + i) % kPerTile) * 64 + lane, tr = ci / kRowChunks, c = (ci % kRowChunks) ^ perm(tr);
-      const int r = T ? c * kEpc : tr, k = T ? tr : c * kEpc;
+      const int byte = (((wave * kSlots + i) % kPerTile) * 64 + lane) * LB, ci = byte >> 4, tr = ci / kRowChunks;
+      const int e = ((ci % kRowChunks) ^ perm(tr)) * kEpc + (byte & 15) / ES;      // place in the tile's row
+      const int r = T ? e : tr, k = T ? tr : e;
       voff[i] = (T ? k * ld + r : r * ld + k) * ES;
       kl[i] = row0 + r < rows ? k : 0x7fffffff;
     }
@@ -314,7 +316,7 @@ struct Tiles {
       const int t = wave * kSlots + i, tile = t / kPerTile;    // tile: matrix * PL + plane
       const char* base = static_cast<const char*>(NMAT == 2 && tile >= PL ? p1 : p0) + (PL == 1 ? 0 : (tile % PL) * plane * ES) + at;
       const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, 0x7fffffff, 0x00020000);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (AGCN_LDS void*)(dst + t * 1024), 16, kl[i] < left ? voff[i] : (int)0x80000000, 0, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (AGCN_LDS void*)(dst + t * (64 * LB)), LB, kl[i] < left ? voff[i] : (int)0x80000000, 0, 0, 0);
     }
   }
   // Fragment f, k step kk (32 k) of tile `tile`: sixteen rows, lane (r = lane & 15, q = lane / 16) gets k = 8 q .. 8 q + 7 of row r.
@@ -373,10 +375,11 @@ template <int OP, int BM, int BN, int WGM, int WGN, bool AT, bool BT, int NB, in
 __global__ __launch_bounds__(64 * WGM * WGN) void ffn_gemm_kernel(GemmArgs g) {
 #ifdef __HIP_DEVICE_COMPILE__
   constexpr int WAVES = WGM * WGN, FM = BM / WGM / 16, FN = BN / WGN / 16, BK = OP == OP_BF16 ? 64 : 32;
-  constexpr int PL = OP == OP_PLANES ? 3 : 1, ES = OP == OP_FP32 ? 4 : 2, P = OP == OP_BF16 ? 1 : 3;      // planes; element's bytes; pieces
+  constexpr bool WHOLE = OP == OP_FP32 || OP == OP_WORDS;      // fp32 operands, split here
+  constexpr int PL = OP == OP_PLANES ? 3 : 1, ES = WHOLE ? 4 : 2, P = OP == OP_BF16 ? 1 : 3, LB = OP == OP_WORDS ? 4 : 16;      // planes; bytes of an element; pieces; bytes of a load
   constexpr bool F32 = OP != OP_BF16;
-  typedef Tiles<BM, AT, BK, PL, ES, 1, WAVES> TA;
-  typedef Tiles<BN, BT, BK, PL, ES, NB, WAVES> TB;
+  typedef Tiles<BM, AT, BK, PL, ES, LB, 1, WAVES> TA;
+  typedef Tiles<BN, BT, BK, PL, ES, LB, NB, WAVES> TB;
   constexpr int SA = PL * TA::kBytes, SB = NB * PL * TB::kBytes;
   // (arrays of their own for every stage and operand: the compiler then sees that the loads into one do not touch the reads of
   // another; it would wait for all loads in flight otherwise)
@@ -430,7 +433,7 @@ __global__ __launch_bounds__(64 * WGM * WGN) void ffn_gemm_kernel(GemmArgs g) {
 #pragma unroll
     for (int kk = 0; kk < BK / 32; ++kk) {
       u32x4 fa[P][FM], fb[P][NB][FN];
-      if constexpr (OP == OP_FP32) {
+      if constexpr (WHOLE) {
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
           const Pieces x = ra.pieces(a, 0, i);
@@ -627,7 +630,7 @@ __global__ __launch_bounds__(256) void ffn_reduce_kernel(GemmArgs g) {
 
 // Operand images: bf16 matrices whose rows do not start at 16 bytes or end at eights, padded with zeros; fp32 ones as three planes of
 // bf16 pieces.  One launch for all matrices of a call; a thread makes eight columns.
-struct Image { const void* src; void* dst; int64_t rows, plane, chunk0; int32_t cols, ld_src, ld_dst, f32; /* 1: as planes, 2: as it is */ };
+struct Image { const void* src; void* dst; int64_t rows, plane, chunk0; int32_t cols, ld_src, ld_dst, f32; };
 struct ImageArgs { Image im[4]; int32_t n; int64_t chunks; };
 __global__ __launch_bounds__(256) void ffn_image_kernel(ImageArgs a) {
   const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -648,12 +651,6 @@ __global__ __launch_bounds__(256) void ffn_image_kernel(ImageArgs a) {
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = c + i < im.cols ? p[i] : 0.f;
-    }
-    if (im.f32 == 2) {          // (as they are: rows that do not start at 16 bytes)
-      float* d = static_cast<float*>(im.dst) + r * im.ld_dst + c;
-      *reinterpret_cast<f32x4*>(d) = (f32x4){v[0], v[1], v[2], v[3]};
-      *reinterpret_cast<f32x4*>(d + 4) = (f32x4){v[4], v[5], v[6], v[7]};
-      return;
     }
     u32x4 h, m, l;
 #pragma unroll
@@ -689,7 +686,7 @@ inline int pad8(int v) { return (v + 7) & ~7; }
 inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // A matrix as the products read it: its own memory, or an image of it
-struct Mat { const void* p; int32_t ld; int64_t plane; };
+struct Mat { const void* p; int32_t ld; int64_t plane; bool chunks; };      // chunks: rows at 16 bytes, of whole 16-byte chunks
 
 struct Carve {
   char* base;
@@ -701,17 +698,20 @@ struct Carve {
   }
 };
 
-// How an fp32 call lays its operands out, by its sizes alone (the backward has to come to the same answer): as they are while few
-// rows meet many weights -- the planes of 2048 x 8001 weights cost 150 us, more than 16 rows' whole pass over them -- or the work is
-// little; as planes otherwise, which the matrix pipe reads faster.
+// How an fp32 call lays its operands out, by its sizes alone (the backward has to come to the same answer).  Measured, planes / as
+// they are, forward: 16 rows through 2048 x 8192 188 / 77 us, 256 rows 292 / 226, 400 rows 329 / 379 (training pass: 128 rows 487 / 404, 200
+// rows 595 / 654); 5000 rows through 128 x 512 39 / 38, 10000 rows 54 / 60; 700 rows through 1024 x 1024 62 / 66.
 int op_of(const AgcnFfnDesc& d) {
   if (d.dtype == AGCN_DTYPE_BF16) return OP_BF16;
-  return d.rows <= 128 || d.rows * (int64_t)d.H * (d.Fin + d.Fout) <= (int64_t)160 << 20 ? OP_FP32 : OP_PLANES;
+  return d.rows <= (d.training ? 160 : 320) || d.rows * (int64_t)d.H * (d.Fin + d.Fout) <= (int64_t)640 << 20 ? OP_FP32 : OP_PLANES;
 }
-// read in place: rows at 16 bytes, whole chunks
-bool direct(const AgcnFfnDesc& d, const void* p, int cols, int ld) {
+bool whole_chunks(const AgcnFfnDesc& d, const void* p, int cols, int ld) {
   const int epc = d.dtype == AGCN_DTYPE_BF16 ? 8 : 4;
-  return op_of(d) != OP_PLANES && cols % epc == 0 && ld % epc == 0 && ((uintptr_t)p & 15) == 0;
+  return cols % epc == 0 && ld % epc == 0 && ((uintptr_t)p & 15) == 0;
+}
+// read in place: whole fp32 matrices always, bf16 ones in whole chunks
+bool direct(const AgcnFfnDesc& d, const void* p, int cols, int ld) {
+  return op_of(d) == OP_FP32 || (op_of(d) == OP_BF16 && whole_chunks(d, p, cols, ld));
 }
 
 // What the forward leaves for the backward.  The images are there only where a matrix cannot be read as it is; room is kept for
@@ -720,11 +720,11 @@ struct Reserve { void *x, *wg, *wu, *wd, *hid, *p, *q; };
 size_t carve_reserve(const AgcnFfnDesc& d, void* mem, Reserve* r) {
   Carve c{static_cast<char*>(mem), 0};
   const int op = op_of(d), Hp = pad8(d.H), Fp = pad8(d.Fin), Op = pad8(d.Fout);
-  const size_t e = op == OP_BF16 ? 2 : op == OP_FP32 ? 4 : 6, kept = d.dtype == AGCN_DTYPE_F32 ? 4 : 3;
-  r->x = c.take(e * d.rows * Fp);
-  r->wg = c.take(e * d.Fin * Hp);
-  r->wu = c.take(e * d.Fin * Hp);
-  r->wd = c.take(e * d.H * Op);
+  const size_t e = op == OP_BF16 ? 2 : op == OP_FP32 ? 4 : 6, image = op == OP_FP32 ? 0 : e, kept = d.dtype == AGCN_DTYPE_F32 ? 4 : 3;
+  r->x = c.take(image * d.rows * Fp);
+  r->wg = c.take(image * d.Fin * Hp);
+  r->wu = c.take(image * d.Fin * Hp);
+  r->wd = c.take(image * d.H * Op);
   r->hid = c.take(e * d.rows * Hp);
   r->p = d.training ? c.take(kept * d.rows * Hp) : nullptr;
   r->q = d.training ? c.take(kept * d.rows * Hp) : nullptr;
@@ -798,7 +798,8 @@ void product(GemmArgs& g, void* part, hipStream_t s) {
     else if (c.kind == 1) launch_tile<OP_PLANES, 128, 64 / NB, 2, 2, AT, BT, NB, EPI, 2>(g, s);
     else launch_tile<OP_PLANES, 64, 64 / NB, 2, 2, AT, BT, NB, EPI, 3>(g, s);
   } else {
-    launch_tile<OP_FP32, 64, 64 / NB, 2, 2, AT, BT, NB, EPI, 3>(g, s);
+    if (g.words) launch_tile<OP_WORDS, 64, 64 / NB, 2, 2, AT, BT, NB, EPI, 3>(g, s);
+    else launch_tile<OP_FP32, 64, 64 / NB, 2, 2, AT, BT, NB, EPI, 3>(g, s);
   }
   const dim3 rg((unsigned)cdiv((int64_t)g.M * (g.ldp / 8), 32));
   if (g.splits > 1 && !g.f32) hipLaunchKernelGGL((ffn_reduce_kernel<NB, EPI, false>), rg, dim3(256), 0, s, g);
@@ -810,6 +811,7 @@ void operands(GemmArgs* g, const Mat& a, const Mat& b, const Mat* b2) {
   g->seg[g->nseg++] = {a.p, b.p, b2 ? b2->p : nullptr};
   g->a_plane = a.plane; g->b_plane = b.plane;
   g->lda = a.ld; g->ldb = b.ld;
+  g->words |= !a.chunks || !b.chunks || (b2 && !b2->chunks);
 }
 
 int check_ffn(const AgcnFfnDesc* d, const char* who) {
@@ -835,12 +837,12 @@ struct ImageList {
   ImageArgs a;
   ImageList() { std::memset(&a, 0, sizeof(a)); }
   Mat add(const AgcnFfnDesc& d, const void* src, int64_t rows, int cols, int ld, void* dst, bool in_place) {
-    if (in_place) return {src, ld, 0};
+    if (in_place) return {src, ld, 0, whole_chunks(d, src, cols, ld)};
     const int lp = pad8(cols), op = op_of(d);
     Image& im = a.im[a.n++];
-    im = {src, dst, rows, rows * lp, a.chunks, cols, ld, lp, op == OP_BF16 ? 0 : op == OP_FP32 ? 2 : 1};
+    im = {src, dst, rows, rows * lp, a.chunks, cols, ld, lp, op == OP_PLANES};
     a.chunks += rows * (lp >> 3);
-    return {dst, lp, op == OP_PLANES ? im.plane : 0};
+    return {dst, lp, op == OP_PLANES ? im.plane : 0, true};
   }
   void launch(hipStream_t s) const {
     if (a.chunks) hipLaunchKernelGGL(ffn_image_kernel, dim3((unsigned)cdiv(a.chunks, 256)), dim3(256), 0, s, a);
@@ -848,8 +850,8 @@ struct ImageList {
 };
 // the same matrix in the backward, whose image the forward has left
 Mat same(const AgcnFfnDesc& d, const void* src, int64_t rows, int cols, int ld, const void* img, bool in_place) {
-  if (in_place) return {src, ld, 0};
-  return {img, pad8(cols), op_of(d) == OP_PLANES ? rows * pad8(cols) : 0};
+  if (in_place) return {src, ld, 0, whole_chunks(d, src, cols, ld)};
+  return {img, pad8(cols), op_of(d) == OP_PLANES ? rows * pad8(cols) : 0, true};
 }
 
 GemmArgs base_args(const AgcnFfnDesc& d) {
@@ -871,7 +873,7 @@ size_t carve_backward(const AgcnFfnDesc& d, void* mem, BackWs* w) {
   const int op = op_of(d), Hp = pad8(d.H);
   const size_t e = op == OP_BF16 ? 2 : op == OP_FP32 ? 4 : 6;
   Carve c{static_cast<char*>(mem), 0};
-  w->dy = c.take(e * d.rows * pad8(d.Fout));
+  w->dy = c.take(op == OP_FP32 ? 0 : e * d.rows * pad8(d.Fout));
   w->dg = c.take(e * d.rows * Hp);
   w->du = c.take(e * d.rows * Hp);
   w->part = c.take(std::max(std::max(product_part(d, d.rows, Hp, 1, d.Fout, 1, true), product_part(d, d.rows, d.Fin, 1, d.H, 2, false)),
@@ -928,7 +930,7 @@ extern "C" int agcn_gated_ffn_forward(const AgcnFfnDesc* desc, const void* X, co
   g.M = (int)d.rows; g.N = d.H; g.K = d.Fin;
   g.p = r.p; g.q = r.q; g.hid = r.hid;
   product<false, true, 2, EPI_GATED>(g, workspace, s);
-  const Mat hid = {r.hid, g.ldh, g.op == OP_PLANES ? g.plane : 0};
+  const Mat hid = {r.hid, g.ldh, g.op == OP_PLANES ? g.plane : 0, true};
   GemmArgs q = base_args(d);
   operands(&q, hid, wd, nullptr);
   q.M = (int)d.rows; q.N = d.Fout; q.K = d.H;
@@ -973,7 +975,7 @@ extern "C" int agcn_gated_ffn_backward(const AgcnFfnDesc* desc, const void* X, c
   list.launch(s);
   GemmArgs base = base_args(d);
   const int64_t pl = base.op == OP_PLANES ? base.plane : 0;
-  const Mat hid = {r.hid, base.ldh, pl}, dg = {w.dg, base.ldh, pl}, du = {w.du, base.ldh, pl};
+  const Mat hid = {r.hid, base.ldh, pl, true}, dg = {w.dg, base.ldh, pl, true}, du = {w.du, base.ldh, pl, true};
   if (dX || dWg) {
     GemmArgs g = base;                        // dA = dY Wd^T, and from it dG and dU
     operands(&g, dy, wd, nullptr);
