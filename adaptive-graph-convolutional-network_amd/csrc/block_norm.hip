@@ -509,8 +509,8 @@ __global__ __launch_bounds__(1024) void norm_params_kernel(ReduceArgs p) {
     else if (a.z && a.dh) add_parts<true, true, false>(t, rl, a.units, step, F, q);
     else if (a.z && two) add_parts<true, false, true>(t, rl, a.units, step, F, q);
     else if (a.z) add_parts<true, false, false>(t, rl, a.units, step, F, q);
-    else if (two) add_parts<false, true, true>(t, rl, a.units, step, F, q);
-    else add_parts<false, true, false>(t, rl, a.units, step, F, q);
+    else if (a.dh && two) add_parts<false, true, true>(t, rl, a.units, step, F, q);
+    else if (a.dh) add_parts<false, true, false>(t, rl, a.units, step, F, q);
   }
 #pragma unroll
   for (int j = 0; j < 4; ++j) s[j][rl][cl] = q[j];
@@ -648,7 +648,8 @@ int check_norm(const AgcnNormDesc* d, const void* plan_host, const void* plan_de
     a->B = host.info.B;
     a->pads = host.info.rows != host.info.N1;
     int32_t most = 0;                       // rows of the largest graph, its pad rows counted
-    for (int32_t g = 0; g < host.info.B; ++g) most = std::max(most, host.row_off[g + 1] - host.row_off[g]);
+    if (d->gate == AGCN_GATE_GRAPH)
+      for (int32_t g = 0; g < host.info.B; ++g) most = std::max(most, host.row_off[g + 1] - host.row_off[g]);
     // rows of a graph per workgroup: few enough for a thousand workgroups, up to 64 (each leaves four sums per column)
     const int R = rows_at_once(shape_for(d->F));
     a->graph_rows = R;

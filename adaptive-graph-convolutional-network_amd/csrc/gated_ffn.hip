@@ -633,52 +633,51 @@ __global__ __launch_bounds__(256) void ffn_reduce_kernel(GemmArgs g) {
 struct Image { const void* src; void* dst; int64_t rows, plane, chunk0; int32_t cols, ld_src, ld_dst, f32; };
 struct ImageArgs { Image im[4]; int32_t n; int64_t chunks; };
 __global__ __launch_bounds__(256) void ffn_image_kernel(ImageArgs a) {
-  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (e >= a.chunks) return;
-  int k = 0;
-  while (k + 1 < a.n && a.im[k + 1].chunk0 <= e) ++k;
-  const Image& im = a.im[k];
-  const int64_t at = e - im.chunk0, per = im.ld_dst >> 3, r = at / per;
-  const int c = (int)(at - r * per) * 8;
-  uint16_t* dst = static_cast<uint16_t*>(im.dst) + r * im.ld_dst + c;
-  if (im.f32) {
-    const float* p = static_cast<const float*>(im.src) + r * im.ld_src + c;
-    float v[8];
-    if (c + 8 <= im.cols) {
-      const u32x4u lo = *reinterpret_cast<const u32x4u*>(p), hi = *reinterpret_cast<const u32x4u*>(p + 4);
+  for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < a.chunks; e += (int64_t)gridDim.x * 256) {
+    int k = 0;
+    while (k + 1 < a.n && a.im[k + 1].chunk0 <= e) ++k;
+    const Image& im = a.im[k];
+    const int64_t at = e - im.chunk0, per = im.ld_dst >> 3, r = at / per;
+    const int c = (int)(at - r * per) * 8;
+    uint16_t* dst = static_cast<uint16_t*>(im.dst) + r * im.ld_dst + c;
+    if (im.f32) {
+      const float* p = static_cast<const float*>(im.src) + r * im.ld_src + c;
+      float v[8];
+      if (c + 8 <= im.cols) {
+        const u32x4u lo = *reinterpret_cast<const u32x4u*>(p), hi = *reinterpret_cast<const u32x4u*>(p + 4);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) { v[i] = __uint_as_float(lo[i]); v[4 + i] = __uint_as_float(hi[i]); }
+        for (int i = 0; i < 4; ++i) { v[i] = __uint_as_float(lo[i]); v[4 + i] = __uint_as_float(hi[i]); }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = c + i < im.cols ? p[i] : 0.f;
+      }
+      u32x4 h, m, l;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t x, y, z;
+        split3(v[2 * i], v[2 * i + 1], x, y, z);
+        h[i] = x; m[i] = y; l[i] = z;
+      }
+      *reinterpret_cast<u32x4*>(dst) = h;
+      *reinterpret_cast<u32x4*>(dst + im.plane) = m;
+      *reinterpret_cast<u32x4*>(dst + 2 * im.plane) = l;
     } else {
+      const uint16_t* p = static_cast<const uint16_t*>(im.src) + r * im.ld_src + c;
+      u32x4 v;
+      if (c + 8 <= im.cols) {
+        v = *reinterpret_cast<const u32x4h*>(p);
+      } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = c + i < im.cols ? p[i] : 0.f;
+        for (int i = 0; i < 4; ++i)
+          v[i] = (c + 2 * i < im.cols ? (uint32_t)p[2 * i] : 0u) | (c + 2 * i + 1 < im.cols ? (uint32_t)p[2 * i + 1] << 16 : 0u);
+      }
+      *reinterpret_cast<u32x4*>(dst) = v;
     }
-    u32x4 h, m, l;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      uint32_t x, y, z;
-      split3(v[2 * i], v[2 * i + 1], x, y, z);
-      h[i] = x; m[i] = y; l[i] = z;
-    }
-    *reinterpret_cast<u32x4*>(dst) = h;
-    *reinterpret_cast<u32x4*>(dst + im.plane) = m;
-    *reinterpret_cast<u32x4*>(dst + 2 * im.plane) = l;
-  } else {
-    const uint16_t* p = static_cast<const uint16_t*>(im.src) + r * im.ld_src + c;
-    u32x4 v;
-    if (c + 8 <= im.cols) {
-      v = *reinterpret_cast<const u32x4h*>(p);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        v[i] = (c + 2 * i < im.cols ? (uint32_t)p[2 * i] : 0u) | (c + 2 * i + 1 < im.cols ? (uint32_t)p[2 * i + 1] << 16 : 0u);
-    }
-    *reinterpret_cast<u32x4*>(dst) = v;
   }
 }
 
 __global__ __launch_bounds__(256) void ffn_zero_kernel(void* p, int64_t bytes) {
-  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (e < bytes >> 1) static_cast<uint16_t*>(p)[e] = 0;
+  for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < bytes >> 1; e += (int64_t)gridDim.x * 256) static_cast<uint16_t*>(p)[e] = 0;
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------------
@@ -845,7 +844,7 @@ struct ImageList {
     return {dst, lp, op == OP_PLANES ? im.plane : 0, true};
   }
   void launch(hipStream_t s) const {
-    if (a.chunks) hipLaunchKernelGGL(ffn_image_kernel, dim3((unsigned)cdiv(a.chunks, 256)), dim3(256), 0, s, a);
+    if (a.chunks) hipLaunchKernelGGL(ffn_image_kernel, dim3((unsigned)std::min<int64_t>(cdiv(a.chunks, 256), 1 << 20)), dim3(256), 0, s, a);
   }
 };
 // the same matrix in the backward, whose image the forward has left
@@ -881,7 +880,7 @@ size_t carve_backward(const AgcnFfnDesc& d, void* mem, BackWs* w) {
   return c.off;
 }
 void zero(void* p, int64_t bytes, hipStream_t s) {
-  hipLaunchKernelGGL(ffn_zero_kernel, dim3((unsigned)cdiv(bytes / 2, 256)), dim3(256), 0, s, p, bytes);
+  hipLaunchKernelGGL(ffn_zero_kernel, dim3((unsigned)std::min<int64_t>(cdiv(bytes / 2, 256), 1 << 16)), dim3(256), 0, s, p, bytes);
 }
 }  // namespace
 }  // namespace agcn

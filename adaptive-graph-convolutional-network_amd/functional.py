@@ -6,6 +6,7 @@ import functools
 import threading
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _ffi
 
@@ -858,6 +859,7 @@ class NormGateResidualFunction(torch.autograd.Function):
         return y, h
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy, dh):
         if dy is None and dh is None:
             return (None,) * 12
@@ -957,6 +959,7 @@ class GatedFfnFunction(torch.autograd.Function):
         return Y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dY):
         return _on_device_of(dY, GatedFfnFunction._backward, ctx.desc, ctx.saved_tensors, dY, ctx.needs_input_grad)
 

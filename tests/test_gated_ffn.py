@@ -281,6 +281,14 @@ def test_other_stream_and_replayed_graph(amd, dtype):
             assert torch.equal(r, out[k].to(dtype)), k
 
 
+@pytest.mark.gpu
+def test_a_second_derivative_is_refused(amd):
+    ts = [t.requires_grad_(True) for t in real(1, 6, 8, 16, 8, f32)[:4]]
+    (g,) = torch.autograd.grad(amd.gated_ffn(*ts).sum(), ts[:1], create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable|twice|differentiat"):
+        g.sum().backward()
+
+
 def test_refusals(amd):
     lib = amd._ffi.lib()
     z = torch.zeros
