@@ -294,7 +294,7 @@ __global__ __launch_bounds__(threads_of<L>()) void norm_forward_kernel(NormArgs 
 // y is formed again from x, z and the gate, which have to be read anyway (x in y's place): the stored y may be rounded to
 // bf16, and a row whose features differ by less than that rounding would get a wrong yh.
 // AHEAD: the next row's operands are fetched while a row is worked on.  It pays where it costs few registers (bf16 rows, no gate, no
-// means: 32768 x 4096 463 -> AHEADUS us); with more it spills.
+// means: 32768 x 4096 463 -> 395 us); with more it spills.
 template <typename TX, typename TZ, int L, int NV, bool LAYER, bool GATED>
 __global__ __launch_bounds__(threads_of<L>(), LAYER || GATED ? 3 : 4) void norm_backward_kernel(NormArgs a) {
   constexpr bool AHEAD = !LAYER && !GATED && NV == 1 && sizeof(TX) == 2;

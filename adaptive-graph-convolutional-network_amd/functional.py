@@ -6,7 +6,6 @@ import functools
 import threading
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _ffi
 
@@ -846,6 +845,31 @@ def _norm_forward(z, x, gate, scale, post_weight, post_bias, pre_weight, pre_bia
     return y, h, (z, x, gate, scale, post_weight, post_bias, pre_weight, pre_bias, stats), desc
 
 
+class _NoSecondDerivative(torch.autograd.Function):
+    """A gradient that may be used, but not differentiated: without it, a penalty on a gradient would silently lose the terms
+    that a kernel's backward does not carry on."""
+
+    @staticmethod
+    def forward(ctx, grad, mark):
+        return grad.view_as(grad)
+
+    @staticmethod
+    def backward(ctx, grad):
+        raise _ffi.AgcnError("this operator's gradient cannot be differentiated again")
+
+
+def _first_order(backward):
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        if not torch.is_grad_enabled():                       # the usual case: no graph of the backward pass is wanted
+            return backward(ctx, *grads)
+        with torch.no_grad():
+            out = backward(ctx, *grads)
+            mark = torch.empty(0, requires_grad=True)
+        return tuple(None if g is None else _NoSecondDerivative.apply(g, mark) for g in out)
+    return run
+
+
 class NormGateResidualFunction(torch.autograd.Function):
     """(y, h) = (x + scale * a(gate) * N(z), N'(y)); see norm_gate_residual."""
 
@@ -859,7 +883,7 @@ class NormGateResidualFunction(torch.autograd.Function):
         return y, h
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dy, dh):
         if dy is None and dh is None:
             return (None,) * 12
@@ -959,7 +983,7 @@ class GatedFfnFunction(torch.autograd.Function):
         return Y
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dY):
         return _on_device_of(dY, GatedFfnFunction._backward, ctx.desc, ctx.saved_tensors, dY, ctx.needs_input_grad)
 

@@ -361,6 +361,34 @@ def test_other_stream_and_replayed_graph(amd):
             assert torch.equal(o, eager[k]), k
 
 
+@pytest.mark.gpu
+def test_a_second_derivative_is_refused(amd):
+    d = make(30, 6, 32)
+    x = d["x"].requires_grad_(True)
+    y, h = amd.norm_gate_residual(d["z"], x, post_weight=d["post_weight"], pre_weight=d["pre_weight"])
+    loss = y.sum() + h.sum()
+    (g,) = torch.autograd.grad(loss, [x], create_graph=True)
+    with pytest.raises(amd.AgcnError, match="differentiated again"):
+        (loss + (g * g).sum()).backward()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gate", ["none", "row", "graph"])
+def test_two_backward_passes_of_one_forward(amd, gate):
+    ns = [18, 5, 48, 1]
+    plan = amd.Plan(ns, device="cuda") if gate == "graph" else None
+    d = make(31, sum(ns), 96, gate=gate, ns=ns)
+    names = [k for k in ("z", "x", "gate", "scale", "post_weight", "pre_weight") if k in d]
+    ts = [d[k].requires_grad_(True) for k in names]
+    out = amd.norm_gate_residual(**{k: d[k] for k in names}, gate_activation="tanh", plan=plan)
+    first = torch.autograd.grad(out, ts, (d["dy"], d["dh"]), retain_graph=True)
+    other = torch.autograd.grad(out, ts, (-2 * d["dy"], -2 * d["dh"]), retain_graph=True)
+    again = torch.autograd.grad(out, ts, (d["dy"], d["dh"]))
+    for a, b, c in zip(first, other, again):
+        assert torch.equal(a, c)
+        assert torch.equal(-2 * a, b)
+
+
 def test_refusals(amd):
     """Before any launch: shapes, types, combinations (CPU; the C entries see addresses only)."""
     lib = amd._ffi.lib()

@@ -287,6 +287,27 @@ def test_a_second_derivative_is_refused(amd):
     (g,) = torch.autograd.grad(amd.gated_ffn(*ts).sum(), ts[:1], create_graph=True)
     with pytest.raises(RuntimeError, match="once_differentiable|twice|differentiat"):
         g.sum().backward()
+    loss = amd.gated_ffn(*ts).sum()                           # ... nor dropped next to a loss that has a derivative
+    (g,) = torch.autograd.grad(loss, ts[:1], create_graph=True)
+    with pytest.raises(amd.AgcnError, match="differentiated again"):
+        (loss + (g * g).sum()).backward()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [5, 700])
+@pytest.mark.parametrize("dtype", [f32, bf16])
+def test_two_backward_passes_of_one_forward(amd, rows, dtype):
+    X, Wg, Wu, Wd, dY = real(2, rows, 40, 72, 24, dtype)
+    ts = [t.requires_grad_(True) for t in (X, Wg, Wu, Wd)]
+    Y = amd.gated_ffn(*ts)
+    first = torch.autograd.grad(Y, ts, dY, retain_graph=True)
+    other = torch.autograd.grad(Y, ts, -2 * dY, retain_graph=True)
+    again = torch.autograd.grad(Y, ts, dY)
+    for a, b, c in zip(first, other, again):
+        assert torch.equal(a, c)
+    fresh = torch.autograd.grad(amd.gated_ffn(*ts), ts, -2 * dY)
+    for b, f in zip(other, fresh):                            # (not -2 x the first: the matrix instruction's sums need not be
+        assert torch.equal(b, f)                              # rounded the same way for both signs)
 
 
 def test_refusals(amd):
