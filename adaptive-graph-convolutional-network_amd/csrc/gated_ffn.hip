@@ -20,13 +20,16 @@
 //     one small loop of epilogue code instead of one copy per fragment.
 //   * Few tiles for the chip: the k loop is cut into splits whose fp32 tiles a second kernel adds in order (no atomics) and
 //     puts through the same epilogue.
-// Roundings of bf16 calls: A, dG, dU are stored in bf16 for the products that read them (the matrix pipe takes bf16); P and Q, which
+//   * One to four rows while serving are bound by the weights' bytes: kernels of their own on the vector unit (ffn_rows_kernel).
+// Roundings of bf16 calls: A, dG, dU are stored in bf16 for the products that read them (the matrix pipe takes bf16; calls with few
+// elements of A keep a second piece); P and Q, which
 // are only multiplied element by element, keep 24 bits (sign, exponent, 15 bits of the mantissa: in bf16 they would add as
 // much error to every gradient as dG's own rounding); sums, activations and their slopes are fp32.
 #include <hip/hip_bf16.h>
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "bf16_split.h"
 #include "sgc_kernels.h"
@@ -47,7 +50,7 @@ enum { OP_BF16 = 1, OP_FP32 = 2, OP_PLANES = 3, OP_WORDS = 4 };
 struct Seg { const void *a, *b, *b2; };
 
 struct GemmArgs {
-  Seg seg[2];                        // the k loop runs over one or two products of the same sizes
+  Seg seg[4];                        // the k loop runs over one to four products of the same sizes
   int32_t nseg;
   int32_t M, N, K;                   // N: columns of one B matrix (two B matrices: of each)
   int32_t lda, ldb;
@@ -57,6 +60,7 @@ struct GemmArgs {
   int32_t ldp;
   // epilogue
   int32_t act, f32, op, words;       // words: OP_FP32 as OP_WORDS
+  int32_t two;                       // A, dG, dU in two bf16 pieces
   int32_t ldh;                       // leading dimension of P, Q, A, dG, dU
   int64_t plane;                     // elements between the planes of A, dG, dU
   void *out, *out2;                  // EPI_STORE: [M, ldo]
@@ -164,6 +168,16 @@ __device__ __forceinline__ void store8_kept(const GemmArgs& g, void* p, int64_t 
   }
 }
 template <bool F32>
+__device__ __forceinline__ void store_kept(void* p, int64_t plane, int64_t at, float x) {
+  if constexpr (F32) {
+    static_cast<float*>(p)[at] = x;
+  } else {
+    const uint32_t r = __float_as_uint(x) + 0x80u;
+    static_cast<uint16_t*>(p)[at] = (uint16_t)(r >> 16);
+    reinterpret_cast<uint8_t*>(static_cast<uint16_t*>(p) + plane)[at] = (uint8_t)(r >> 8);
+  }
+}
+template <bool F32>
 __device__ __forceinline__ void fetch8_kept(const GemmArgs& g, const void* p, int64_t at, Kept8<F32>& k) {
   if constexpr (F32) {
     const float* q = static_cast<const float*>(p) + at;
@@ -187,12 +201,21 @@ __device__ __forceinline__ F8 kept8(const Kept8<F32>& k) {
   }
   return x;
 }
+// what bf16 leaves of x (nothing, where the leading piece is infinite: the products would make NaN of inf - inf)
+__device__ __forceinline__ float rest_of(float x, float lead) { return fabsf(lead) < __builtin_inff() ? x - lead : 0.f; }
 // eight values of a matrix that a later product reads
 template <bool F32>
 __device__ __forceinline__ void store8_operand(const GemmArgs& g, void* dst, int64_t at, const F8& x) {
   uint16_t* p = static_cast<uint16_t*>(dst);
   if constexpr (!F32) {
-    *reinterpret_cast<u32x4*>(p + at) = bf8(x);
+    const u32x4 h = bf8(x);
+    *reinterpret_cast<u32x4*>(p + at) = h;
+    if (g.two) {
+      F8 rest;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) rest.v[i] = rest_of(x.v[i], __uint_as_float(i & 1 ? h[i >> 1] & 0xffff0000u : h[i >> 1] << 16));
+      *reinterpret_cast<u32x4*>(p + g.plane + at) = bf8(rest);
+    }
   } else if (g.op == OP_FP32) {
     store8_f32(static_cast<float*>(dst) + at, x);
   } else {
@@ -413,7 +436,7 @@ __global__ __launch_bounds__(64 * WGM * WGN) void ffn_gemm_kernel(GemmArgs g) {
   // waits below expect.  Two stages: no load, and the branch keeps the scheduler from spreading the loads over the products, which
   // costs it more registers than there are)
   auto load = [&](AGCN_LDS char* a, AGCN_LDS char* b) {
-    const Seg s = g.seg[seg < 2 ? seg : 1];
+    const Seg s = g.seg[seg < 4 ? seg : 3];
     const int left = lit < it1 ? g.K - kt * BK : 0;
     ta.load(s.a, nullptr, m0, g.a_plane, g.lda, kt, left, a, wave);
     tb.load(s.b, s.b2, n0, g.b_plane, g.ldb, kt, left, b, wave);
@@ -628,6 +651,173 @@ __global__ __launch_bounds__(256) void ffn_reduce_kernel(GemmArgs g) {
   epilogue<EPI, NB, F32>(g, m, n, o[0], o[NB - 1], kp, kq);
 }
 
+// Few rows (single tokens while serving): bound by the weights' bytes, nothing else is worth waiting for.  A workgroup takes a strip of
+// 128 bytes of the weights' columns, eight lanes a row, eight rows in flight per lane; products and sums in fp32 on the vector unit.
+// The lanes' sums meet by halving exchanges in the wave, then in LDS.  The first product's workgroups take one projection each and
+// leave fp32 sums (of a part of k each, where the strips alone do not fill the chip); the second product's lanes add the
+// parts, apply the gate to the eight k they need (one per lane, handed round by shuffles), and multiply: no launch in between, and A is
+// rounded nowhere.
+template <typename T> struct Cols;
+template <> struct Cols<float> {
+  static constexpr int n = 4;
+  static __device__ __forceinline__ u32x4 load(const float* p, int left) {
+    if (left >= 4) { const u32x4u v = *reinterpret_cast<const u32x4u*>(p); return (u32x4){v.x, v.y, v.z, v.w}; }
+    u32x4 v = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 3; ++i) if (i < left) v[i] = __float_as_uint(p[i]);
+    return v;
+  }
+  static __device__ __forceinline__ float at(const u32x4& v, int i) { return __uint_as_float(v[i]); }
+};
+template <> struct Cols<uint16_t> {
+  static constexpr int n = 8;
+  static __device__ __forceinline__ u32x4 load(const uint16_t* p, int left) {
+    if (left >= 8) { const u32x4h v = *reinterpret_cast<const u32x4h*>(p); return (u32x4){v.x, v.y, v.z, v.w}; }
+    u32x4 v = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 7; ++i) if (i < left) v[i >> 1] |= (uint32_t)p[i] << (16 * (i & 1));
+    return v;
+  }
+  static __device__ __forceinline__ float at(const u32x4& v, int i) { return __uint_as_float(i & 1 ? v[i >> 1] & 0xffff0000u : v[i >> 1] << 16); }
+};
+
+// Sums of N values over the lanes whose numbers differ in the bits from M down to LX: a lane gives away half of its values at every
+// step and adds what it gets to the other half (`first`: which are left to it); with one value left, both lanes add.
+template <int N, int M, int LX>
+constexpr int halved() { if constexpr (M < LX) return N; else return halved<(N > 1 ? N / 2 : 1), M / 2, LX>(); }
+template <int N, int M, int LX>
+__device__ __forceinline__ void halve(float* v, int lane, int& first, bool& mine) {
+  if constexpr (M >= LX) {
+    const bool up = lane & M;
+    if constexpr (N > 1) {
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) {
+        const float keep = up ? v[i + N / 2] : v[i], give = up ? v[i] : v[i + N / 2];
+        v[i] = keep + __shfl_xor(give, M);
+      }
+      first += up ? N / 2 : 0;
+    } else {
+      v[0] += __shfl_xor(v[0], M);
+      mine = mine && !up;
+    }
+    halve<(N > 1 ? N / 2 : 1), M / 2, LX>(v, lane, first, mine);
+  }
+}
+
+struct FewArgs {
+  const void *x, *w[2];              // GATE: w[0] alone
+  const float* sums;                 // GATE: the first product's, [split][G, U][M][ld_sums]
+  float* part;                       // [split][matrix][M][ldp]
+  void* out;                         // GATE, one split: [M, N]
+  void *p, *q, *hid;                 // GATE, training: [M, ld of the sums], as the matrix pipe's path leaves them
+  int32_t M, N, K, ldx, ldw, ld_sums, ldp, act, strips, splits, in_splits, two;
+};
+constexpr int kFewLanes = 8;         // of a weight row
+
+template <typename TW, int R, bool GATE>
+__global__ __launch_bounds__(512) void ffn_rows_kernel(FewArgs g) {
+  typedef Cols<TW> CW;
+  constexpr bool F32 = sizeof(TW) == 4;
+  constexpr int LX = kFewLanes, N0 = R * CW::n, COLS = LX * CW::n, GROUPS = 512 / LX, MATS = GATE ? 1 : 2;
+  __shared__ float sums[8][LX * N0];
+  const int total = g.strips * MATS * g.splits, run = (total + 7) >> 3;
+  const int id = (blockIdx.x & 7) * run + (blockIdx.x >> 3);        // neighbouring strips on one die
+  if ((int)(blockIdx.x >> 3) >= run || id >= total) return;
+  const int sm = id / g.strips, split = sm / MATS, n_wg = (id - sm * g.strips) * COLS;
+  const int lane = threadIdx.x & 63, lx = threadIdx.x % LX, n = n_wg + lx * CW::n;
+  const TW* x = static_cast<const TW*>(g.x);
+  const TW* w = static_cast<const TW*>(g.w[sm % MATS]);
+  float acc[R][CW::n];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int i = 0; i < CW::n; ++i) acc[r][i] = 0.f;
+  const int blocks = (g.K + 7) >> 3;
+  const int b1 = (int)((int64_t)blocks * (split + 1) / g.splits);
+  for (int b = (int)((int64_t)blocks * split / g.splits) + threadIdx.x / LX; b < b1; b += GROUPS) {
+    const int k = b * 8;
+    u32x4 wv[8];
+    if (k + 8 <= g.K && n + CW::n <= g.N) {                         // (loads without branches: they all fly together)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) wv[i] = CW::load(w + (int64_t)(k + i) * g.ldw + n, CW::n);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) wv[i] = CW::load(w + (int64_t)(k + i) * g.ldw + n, k + i < g.K ? g.N - n : 0);
+    }
+    if constexpr (GATE) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        float a = 0.f, da = 0.f, U = 0.f;
+        if (k + lx < g.K && r < g.M) {
+          float G = 0.f;
+          for (int q = 0; q < g.in_splits; ++q) {
+            const float* p = g.sums + ((int64_t)q * 2 * g.M + r) * g.ld_sums + k + lx;
+            G += p[0];
+            U += p[(int64_t)g.M * g.ld_sums];
+          }
+          if (F32) gate_of(g.act, G, a, da);
+          else gate_of_bf16(g.act, G, a, da);
+        }
+        if (g.p && n_wg == 0 && r < g.M) {                          // (pads included: zeros)
+          const int64_t at = (int64_t)r * g.ld_sums + k + lx;
+          store_kept<F32>(g.p, (int64_t)g.M * g.ld_sums, at, da * U);
+          store_kept<F32>(g.q, (int64_t)g.M * g.ld_sums, at, a);
+          if (F32) static_cast<float*>(g.hid)[at] = a * U;
+          else {
+            const __bf16 h = (__bf16)(a * U);
+            static_cast<__bf16*>(g.hid)[at] = h;
+            if (g.two) static_cast<__bf16*>(g.hid)[(int64_t)g.M * g.ld_sums + at] = (__bf16)rest_of(a * U, (float)h);
+          }
+        }
+        a *= U;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float ai = __shfl(a, (lane & ~(LX - 1)) + i);
+#pragma unroll
+          for (int e = 0; e < CW::n; ++e) acc[r][e] = fmaf(ai, CW::at(wv[i], e), acc[r][e]);
+        }
+      }
+    } else {
+      u32x4 xv[R][8 / CW::n];
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int i = 0; i < 8 / CW::n; ++i) xv[r][i] = CW::load(x + (int64_t)(r < g.M ? r : 0) * g.ldx + k + i * CW::n, g.K - k - i * CW::n);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int e = 0; e < CW::n; ++e)
+#pragma unroll
+          for (int r = 0; r < R; ++r) acc[r][e] = fmaf(CW::at(xv[r][i / CW::n], i % CW::n), CW::at(wv[i], e), acc[r][e]);
+    }
+  }
+  float v[N0];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int e = 0; e < CW::n; ++e) v[r * CW::n + e] = acc[r][e];
+  int first = 0;
+  bool mine = true;
+  constexpr int have = halved<N0, 32, LX>();
+  halve<N0, 32, LX>(v, lane, first, mine);
+  if (mine) {
+#pragma unroll
+    for (int i = 0; i < have; ++i) sums[threadIdx.x >> 6][lx * N0 + first + i] = v[i];
+  }
+  __syncthreads();
+  // a thread: one column of one row
+  for (int j = threadIdx.x; j < R * COLS; j += 512) {
+    const int m = j / COLS, c = j % COLS, at = c / CW::n * N0 + m * CW::n + c % CW::n;
+    if (m >= g.M || n_wg + c >= g.N) continue;
+    float s = sums[0][at];
+#pragma unroll
+    for (int q = 1; q < 8; ++q) s += sums[q][at];
+    if (!GATE || g.splits > 1) g.part[((int64_t)sm * g.M + m) * g.ldp + n_wg + c] = s;
+    else if (F32) static_cast<float*>(g.out)[(int64_t)m * g.N + n_wg + c] = s;
+    else static_cast<__bf16*>(g.out)[(int64_t)m * g.N + n_wg + c] = (__bf16)s;
+  }
+}
+
 // Operand images: bf16 matrices whose rows do not start at 16 bytes or end at eights, padded with zeros; fp32 ones as three planes of
 // bf16 pieces.  One launch for all matrices of a call; a thread makes eight columns.
 struct Image { const void* src; void* dst; int64_t rows, plane, chunk0; int32_t cols, ld_src, ld_dst, f32; };
@@ -704,6 +894,10 @@ int op_of(const AgcnFfnDesc& d) {
   if (d.dtype == AGCN_DTYPE_BF16) return OP_BF16;
   return d.rows <= (d.training ? 160 : 320) || d.rows * (int64_t)d.H * (d.Fin + d.Fout) <= (int64_t)640 << 20 ? OP_FP32 : OP_PLANES;
 }
+// bf16 calls whose A has few elements: A, dG and dU go on in two bf16 pieces.  One rounding of each is as much error as the rounding of
+// the result on the average, but where few roundings meet in a result row the average does not hold (6 rows through 1617 x 270: 1.56
+// times the error of an unrounded A).  The second piece's products cost 0.3 to 1.2 us of a forward's 11 to 22 at that size.
+bool two_pieces(const AgcnFfnDesc& d) { return d.dtype == AGCN_DTYPE_BF16 && d.rows * d.H <= 16384; }
 bool whole_chunks(const AgcnFfnDesc& d, const void* p, int cols, int ld) {
   const int epc = d.dtype == AGCN_DTYPE_BF16 ? 8 : 4;
   return cols % epc == 0 && ld % epc == 0 && ((uintptr_t)p & 15) == 0;
@@ -713,13 +907,18 @@ bool direct(const AgcnFfnDesc& d, const void* p, int cols, int ld) {
   return op_of(d) == OP_FP32 || (op_of(d) == OP_BF16 && whole_chunks(d, p, cols, ld));
 }
 
+// Which forwards the few-row kernels serve.  Measured with them / on the matrix pipe, 1 row and 4 rows: 2048 x 8192 bf16 29.5 / 36.3 us and
+// 35.5 / 36.1, 2000 x 8001 bf16 (no images of the weights) 30 / 59 and 36 / 58, 2048 x 8192 f32 50 / 79 and 56 / 71, 1024 x 4096 f32 20.5 / 30
+// and 20.5 / 31, 128 x 512 17.5 / 17.5 us; 8 rows 43 / 36, 54 / 59, 70 / 72.
+bool few_rows(const AgcnFfnDesc& d) { return d.rows <= 4; }
+
 // What the forward leaves for the backward.  The images are there only where a matrix cannot be read as it is; room is kept for
 // them whenever the SIZES alone would not rule them out (an address can be odd).
 struct Reserve { void *x, *wg, *wu, *wd, *hid, *p, *q; };
 size_t carve_reserve(const AgcnFfnDesc& d, void* mem, Reserve* r) {
   Carve c{static_cast<char*>(mem), 0};
   const int op = op_of(d), Hp = pad8(d.H), Fp = pad8(d.Fin), Op = pad8(d.Fout);
-  const size_t e = op == OP_BF16 ? 2 : op == OP_FP32 ? 4 : 6, image = op == OP_FP32 ? 0 : e, kept = d.dtype == AGCN_DTYPE_F32 ? 4 : 3;
+  const size_t image = op == OP_BF16 ? 2 : op == OP_FP32 ? 0 : 6, e = two_pieces(d) || op == OP_FP32 ? 4 : image, kept = d.dtype == AGCN_DTYPE_F32 ? 4 : 3;
   r->x = c.take(image * d.rows * Fp);
   r->wg = c.take(image * d.Fin * Hp);
   r->wu = c.take(image * d.Fin * Hp);
@@ -805,6 +1004,43 @@ void product(GemmArgs& g, void* part, hipStream_t s) {
   else if (g.splits > 1) hipLaunchKernelGGL((ffn_reduce_kernel<NB, EPI, true>), rg, dim3(256), 0, s, g);
 }
 
+// The few-row products: strips of 128 bytes, and k cut until 256 workgroups are there (a workgroup has 512 k in flight; 512 of them: 2048
+// x 8192 bf16 30 -> 31.5 us).  The second product's parts cost a launch that adds them: from 2048 k on (1 row through 512 x 2048 17.6 us
+// whole, 20.7 in parts; 2 rows through 1024 x 4096 24.8 whole, 21.5 in parts).
+struct Few { int strips, splits; size_t part; int ldp; };
+Few few_of(const AgcnFfnDesc& d, int64_t N, int64_t K, int mats) {
+  Few c;
+  c.strips = (int)cdiv(N, kFewLanes * (d.dtype == AGCN_DTYPE_F32 ? 4 : 8));
+  c.splits = (int)std::max<int64_t>(1, std::min<int64_t>(16, std::min(cdiv(256, c.strips * mats), K / 512)));
+  if (mats == 1 && K <= 2048) c.splits = 1;
+  c.ldp = pad8((int)N);
+  c.part = mats == 2 || c.splits > 1 ? align256((size_t)c.splits * mats * d.rows * c.ldp * sizeof(float)) : 0;
+  return c;
+}
+template <typename TW, bool GATE>
+void few_launch(const FewArgs& g, hipStream_t s) {
+  const dim3 grid((unsigned)(cdiv((int64_t)g.strips * g.splits * (GATE ? 1 : 2), 8) * 8)), block(512);
+  if (g.M == 1) hipLaunchKernelGGL((ffn_rows_kernel<TW, 1, GATE>), grid, block, 0, s, g);
+  else if (g.M == 2) hipLaunchKernelGGL((ffn_rows_kernel<TW, 2, GATE>), grid, block, 0, s, g);
+  else hipLaunchKernelGGL((ffn_rows_kernel<TW, 4, GATE>), grid, block, 0, s, g);
+}
+void few_forward(const AgcnFfnDesc& d, const void* X, const void* Wg, const void* Wu, const void* Wd, void* Y, const Reserve& r, void* workspace, hipStream_t s) {
+  const Few a = few_of(d, d.H, d.Fin, 2), b = few_of(d, d.Fout, d.H, 1);
+  const bool f32 = d.dtype == AGCN_DTYPE_F32;
+  float *sums = static_cast<float*>(workspace), *part = reinterpret_cast<float*>(static_cast<char*>(workspace) + a.part);
+  const FewArgs up = {X, {Wg, Wu}, nullptr, sums, nullptr, nullptr, nullptr, nullptr, (int)d.rows, d.H, d.Fin, d.ldx, d.H, 0, a.ldp, d.activation, a.strips, a.splits, 0, 0};
+  const FewArgs down = {nullptr, {Wd, nullptr}, sums, part, Y, r.p, r.q, r.hid, (int)d.rows, d.Fout, d.H, 0, d.Fout, a.ldp, b.ldp, d.activation, b.strips, b.splits, a.splits, two_pieces(d)};
+  if (f32) few_launch<float, false>(up, s), few_launch<float, true>(down, s);
+  else few_launch<uint16_t, false>(up, s), few_launch<uint16_t, true>(down, s);
+  if (b.splits == 1) return;
+  GemmArgs g;
+  std::memset(&g, 0, sizeof(g));
+  g.part = part; g.ldp = b.ldp; g.splits = b.splits; g.M = (int)d.rows; g.N = g.ldo = d.Fout; g.out = Y;
+  const dim3 grid((unsigned)cdiv((int64_t)g.M * (g.ldp / 8), 32));
+  if (f32) hipLaunchKernelGGL((ffn_reduce_kernel<1, EPI_STORE, true>), grid, dim3(256), 0, s, g);
+  else hipLaunchKernelGGL((ffn_reduce_kernel<1, EPI_STORE, false>), grid, dim3(256), 0, s, g);
+}
+
 // the operands of a product: one or two pairs of matrices
 void operands(GemmArgs* g, const Mat& a, const Mat& b, const Mat* b2) {
   g->seg[g->nseg++] = {a.p, b.p, b2 ? b2->p : nullptr};
@@ -812,6 +1048,9 @@ void operands(GemmArgs* g, const Mat& a, const Mat& b, const Mat* b2) {
   g->lda = a.ld; g->ldb = b.ld;
   g->words |= !a.chunks || !b.chunks || (b2 && !b2->chunks);
 }
+
+// the lower pieces of A, dG, dU: products of their own, added first
+Mat rest(const GemmArgs& g, const Mat& m) { return {static_cast<const uint16_t*>(m.p) + g.plane, m.ld, 0, true}; }
 
 int check_ffn(const AgcnFfnDesc* d, const char* who) {
   if (!d) return fail(AGCN_EINVAL, "%s: null descriptor", who);
@@ -856,27 +1095,29 @@ Mat same(const AgcnFfnDesc& d, const void* src, int64_t rows, int cols, int ld, 
 GemmArgs base_args(const AgcnFfnDesc& d) {
   GemmArgs g;
   std::memset(&g, 0, sizeof(g));
-  g.act = d.activation; g.f32 = d.dtype == AGCN_DTYPE_F32; g.op = op_of(d);
+  g.act = d.activation; g.f32 = d.dtype == AGCN_DTYPE_F32; g.op = op_of(d); g.two = two_pieces(d);
   g.ldh = pad8(d.H); g.plane = (int64_t)d.rows * g.ldh;
   return g;
 }
 
+int pieces_of(const AgcnFfnDesc& d) { return two_pieces(d) ? 2 : 1; }
 size_t product_part(const AgcnFfnDesc& d, int64_t M, int64_t N, int nb, int64_t K, int nseg, bool gates) {
   return part_bytes(choose(M, N, nb, op_of(d), nseg * ktiles_of(d, K), gates), M, N, nb);
 }
 size_t forward_part(const AgcnFfnDesc& d) {
-  return std::max(product_part(d, d.rows, pad8(d.H), 2, d.Fin, 1, true), product_part(d, d.rows, d.Fout, 1, d.H, 1, false));
+  if (few_rows(d)) return few_of(d, d.H, d.Fin, 2).part + few_of(d, d.Fout, d.H, 1).part;
+  return std::max(product_part(d, d.rows, pad8(d.H), 2, d.Fin, 1, true), product_part(d, d.rows, d.Fout, 1, d.H, pieces_of(d), false));
 }
 struct BackWs { void *dy, *dg, *du, *part; };
 size_t carve_backward(const AgcnFfnDesc& d, void* mem, BackWs* w) {
-  const int op = op_of(d), Hp = pad8(d.H);
-  const size_t e = op == OP_BF16 ? 2 : op == OP_FP32 ? 4 : 6;
+  const int op = op_of(d), Hp = pad8(d.H), pc = pieces_of(d);
+  const size_t image = op == OP_BF16 ? 2 : op == OP_FP32 ? 0 : 6, e = two_pieces(d) || op == OP_FP32 ? 4 : image;
   Carve c{static_cast<char*>(mem), 0};
-  w->dy = c.take(op == OP_FP32 ? 0 : e * d.rows * pad8(d.Fout));
+  w->dy = c.take(image * d.rows * pad8(d.Fout));
   w->dg = c.take(e * d.rows * Hp);
   w->du = c.take(e * d.rows * Hp);
-  w->part = c.take(std::max(std::max(product_part(d, d.rows, Hp, 1, d.Fout, 1, true), product_part(d, d.rows, d.Fin, 1, d.H, 2, false)),
-                            std::max(product_part(d, d.Fin, d.H, 2, d.rows, 1, false), product_part(d, d.H, d.Fout, 1, d.rows, 1, false))));
+  w->part = c.take(std::max(std::max(product_part(d, d.rows, Hp, 1, d.Fout, 1, true), product_part(d, d.rows, d.Fin, 1, d.H, 2 * pc, false)),
+                            std::max(product_part(d, d.Fin, d.H, 2, d.rows, pc, false), product_part(d, d.H, d.Fout, 1, d.rows, pc, false))));
   return c.off;
 }
 void zero(void* p, int64_t bytes, hipStream_t s) {
@@ -923,6 +1164,13 @@ extern "C" int agcn_gated_ffn_forward(const AgcnFfnDesc* desc, const void* X, co
   const InPlace in(d, X, Wg, Wu, Wd);
   const Mat x = list.add(d, X, d.rows, d.Fin, d.ldx, r.x, in.x), wg = list.add(d, Wg, d.Fin, d.H, d.H, r.wg, in.w),
             wu = list.add(d, Wu, d.Fin, d.H, d.H, r.wu, in.w), wd = list.add(d, Wd, d.H, d.Fout, d.Fout, r.wd, in.wd);
+  if (few_rows(d)) {
+    if (d.training) list.launch(s);                           // (the backward reads them)
+    few_forward(d, X, Wg, Wu, Wd, Y, r, workspace, s);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return fail(AGCN_EDEVICE, "%s: %s", who, hipGetErrorString(e));
+    return AGCN_OK;
+  }
   list.launch(s);
   GemmArgs g = base_args(d);
   operands(&g, x, wg, &wu);
@@ -931,6 +1179,7 @@ extern "C" int agcn_gated_ffn_forward(const AgcnFfnDesc* desc, const void* X, co
   product<false, true, 2, EPI_GATED>(g, workspace, s);
   const Mat hid = {r.hid, g.ldh, g.op == OP_PLANES ? g.plane : 0, true};
   GemmArgs q = base_args(d);
+  if (q.two) operands(&q, rest(q, hid), wd, nullptr);
   operands(&q, hid, wd, nullptr);
   q.M = (int)d.rows; q.N = d.Fout; q.K = d.H;
   q.out = Y; q.ldo = d.Fout;
@@ -984,6 +1233,7 @@ extern "C" int agcn_gated_ffn_backward(const AgcnFfnDesc* desc, const void* X, c
   }
   if (dX) {
     GemmArgs g = base;
+    if (g.two) operands(&g, rest(g, dg), wg, nullptr), operands(&g, rest(g, du), wu, nullptr);
     operands(&g, dg, wg, nullptr);
     operands(&g, du, wu, nullptr);
     g.M = (int)d.rows; g.N = d.Fin; g.K = d.H;
@@ -992,6 +1242,8 @@ extern "C" int agcn_gated_ffn_backward(const AgcnFfnDesc* desc, const void* X, c
   }
   if (dWg) {
     GemmArgs g = base;
+    const Mat du_rest = rest(g, du);
+    if (g.two) operands(&g, x, rest(g, dg), &du_rest);
     operands(&g, x, dg, &du);
     g.M = d.Fin; g.N = d.H; g.K = (int)d.rows;
     g.out = dWg; g.out2 = dWu; g.ldo = d.H;
@@ -999,6 +1251,7 @@ extern "C" int agcn_gated_ffn_backward(const AgcnFfnDesc* desc, const void* X, c
   }
   if (dWd) {
     GemmArgs g = base;
+    if (g.two) operands(&g, rest(g, hid), dy, nullptr);
     operands(&g, hid, dy, nullptr);
     g.M = d.H; g.N = d.Fout; g.K = (int)d.rows;
     g.out = dWd; g.ldo = d.Fout;

@@ -37,9 +37,10 @@ def act64(name, g):
     return g * c, c + g * torch.exp(-0.5 * g * g) / math.sqrt(2 * math.pi)
 
 
-def reference(X, Wg, Wu, Wd, dY, act, dtype):
+def reference(X, Wg, Wu, Wd, dY, act, dtype, b=None, act_err=16 * E):
     X, Wg, Wu, Wd, dY = (t.double() for t in (X, Wg, Wu, Wd, dY))
-    b = B8 if dtype == bf16 else 0.0
+    if b is None:
+        b = B8 if dtype == bf16 else 0.0
     M, F = X.shape
     H, O = Wd.shape
     G, U = X @ Wg, X @ Wu
@@ -47,16 +48,16 @@ def reference(X, Wg, Wu, Wd, dY, act, dtype):
     A = a * U
     aX, aWg, aWu, aWd = X.abs(), Wg.abs(), Wu.abs(), Wd.abs()
     eG, eU = (F + 8) * E * (aX @ aWg), (F + 8) * E * (aX @ aWu)
-    ea = 1.2 * eG + 16 * E * a.abs()
+    ea = 1.2 * eG + act_err * a.abs()
     eA = U.abs() * ea + a.abs() * eU + (b + 2 * E) * A.abs()
     out, err = {"Y": A @ Wd}, {"Y": eA @ aWd + (H + 8) * E * (A.abs() @ aWd)}
     dA = dY @ Wd.t()
     eDA = (O + 8) * E * (dY.abs() @ aWd.t())
     eGs, eUs = eG + b * G.abs(), eU + b * U.abs()
-    eda = ((G.abs() <= eGs).double() if act == "relu" else 0.8 * eGs) + 16 * E * da.abs()
+    eda = ((G.abs() <= eGs).double() if act == "relu" else 0.8 * eGs) + act_err * da.abs()
     dG, dU = dA * U * da, dA * a
     eDG = (dA * U).abs() * eda + (dA * da).abs() * eUs + (U * da).abs() * eDA + (b + 4 * E) * dG.abs()
-    eDU = dA.abs() * (1.2 * eGs + 16 * E * a.abs()) + a.abs() * eDA + (b + 2 * E) * dU.abs()
+    eDU = dA.abs() * (1.2 * eGs + act_err * a.abs()) + a.abs() * eDA + (b + 2 * E) * dU.abs()
     out["dX"] = dG @ Wg.t() + dU @ Wu.t()
     err["dX"] = eDG @ aWg.t() + eDU @ aWu.t() + (2 * H + 8) * E * (dG.abs() @ aWg.t() + dU.abs() @ aWu.t())
     out["dWg"], out["dWu"], out["dWd"] = X.t() @ dG, X.t() @ dU, A.t() @ dY
@@ -279,6 +280,64 @@ def test_other_stream_and_replayed_graph(amd, dtype):
         torch.cuda.synchronize()
         for r, k in zip(res, ("Y", "dX", "dWg", "dWu", "dWd")):
             assert torch.equal(r, out[k].to(dtype)), k
+
+
+# few rows have kernels of their own; the sizes cut k in parts in neither, one or both of their products, strips end inside a chunk
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [f32, bf16])
+@pytest.mark.parametrize("size", [(9, 5, 3), (64, 40, 24), (520, 4104, 1000), (1030, 2057, 90), (1100, 1500, 70)])
+@pytest.mark.parametrize("rows", [1, 2, 3, 4, 5])
+def test_few_rows(amd, rows, size, dtype):
+    check_exact(amd, integers(rows + sum(size), rows, *size, dtype), dtype)
+    args = real(rows * sum(size), rows, *size, dtype)
+    out, err, _ = reference(*args, "silu", dtype)
+    check(run(amd, *args, "silu"), out, err, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [f32, bf16])
+@pytest.mark.parametrize("rows", [1, 3])
+def test_few_rows_at_any_address(amd, rows, dtype):
+    F, H, O = 75, 1101, 130
+    X, Wg, Wu, Wd, dY = real(5, rows, F, H, O, dtype)
+    want = amd.gated_ffn(X, Wg, Wu, Wd)
+    wide = torch.full((rows, F + 9), float("nan"), dtype=dtype, device="cuda")          # what is around the operands is not read as one
+    wide[:, 3:3 + F] = X
+    moved = []
+    for w in (Wg, Wu, Wd):
+        flat = torch.full((w.numel() + 12,), float("nan"), dtype=dtype, device="cuda")
+        flat[1:1 + w.numel()] = w.reshape(-1)
+        moved.append(flat[1:1 + w.numel()].view(w.shape))
+    assert torch.equal(amd.gated_ffn(wide[:, 3:3 + F], *moved), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [f32, bf16])
+def test_few_rows_do_not_touch_each_other(amd, dtype):
+    X, Wg, Wu, Wd, _ = real(6, 3, 70, 2600, 90, dtype)
+    want = amd.gated_ffn(X, Wg, Wu, Wd)
+    X[1] = float("nan")
+    got = amd.gated_ffn(X, Wg, Wu, Wd)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[2], want[2]) and bool(got[1].isnan().all())
+
+
+# bf16 calls of up to 16384 elements of A keep it, dG and dU in two pieces (2^-16), P and Q in 24 bits (2^-16): b = 2^-15.  Their
+# activations: the fit of the normal distribution is within 3e-5 < 2^-15 of its tail, exp2 within (1 + |g|) 2^-23: 2^-14.
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["silu", "gelu", "sigmoid"])
+@pytest.mark.parametrize("size", [(2, 40, 72, 24), (6, 40, 72, 24), (9, 33, 130, 50), (60, 100, 272, 64), (300, 20, 50, 30)])
+def test_small_bf16_calls_round_their_results_alone(amd, size, act):
+    args = real(sum(size), *size, bf16)
+    out, err, _ = reference(*args, act, bf16, b=2.0 ** -15, act_err=2.0 ** -14)
+    check(run(amd, *args, act), out, err, bf16)
+
+
+@pytest.mark.gpu
+def test_a_value_beyond_bf16_stays_infinite(amd):
+    X = torch.full((6, 8), 2.0 ** 60, device="cuda", dtype=bf16)
+    W = torch.full((8, 16), 2.0 ** 4, device="cuda", dtype=bf16)
+    Y = amd.gated_ffn(X, W, W, torch.ones(16, 4, device="cuda", dtype=bf16), activation="relu")      # A = (2^67)^2 > 2^128
+    assert bool((Y == float("inf")).all())
 
 
 @pytest.mark.gpu
