@@ -20,16 +20,15 @@
 //     one small loop of epilogue code instead of one copy per fragment.
 //   * Few tiles for the chip: the k loop is cut into splits whose fp32 tiles a second kernel adds in order (no atomics) and
 //     puts through the same epilogue.
-//   * One to four rows while serving are bound by the weights' bytes: kernels of their own on the vector unit (ffn_rows_kernel).
+//   * One to four rows are bound by the weights' bytes: kernels of their own on the vector unit (ffn_rows_kernel).
+//   * Features of at most 128, forward only: both products in one kernel, A stays in registers (ffn_fused_kernel).
 // Roundings of bf16 calls: A, dG, dU are stored in bf16 for the products that read them (the matrix pipe takes bf16; calls with few
-// elements of A keep a second piece); P and Q, which
-// are only multiplied element by element, keep 24 bits (sign, exponent, 15 bits of the mantissa: in bf16 they would add as
-// much error to every gradient as dG's own rounding); sums, activations and their slopes are fp32.
+// elements of A keep a second piece); P and Q, which are only multiplied element by element, keep 24 bits (sign, exponent, 15
+// bits of the mantissa: in bf16 they would add as much error to every gradient as dG's own rounding); sums, activations and their slopes are fp32.
 #include <hip/hip_bf16.h>
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
-#include <type_traits>
 
 #include "bf16_split.h"
 #include "sgc_kernels.h"
@@ -73,35 +72,23 @@ __device__ __forceinline__ uint32_t pk_bf(float a, float b) {
   return __builtin_bit_cast(uint32_t, (bf16x2){(__bf16)a, (__bf16)b});
 }
 
-// act(g) and act'(g).  The slopes are formed from e^-|g| (no 1 - s where s is near 1).
-__device__ __forceinline__ void gate_of(int act, float g, float& a, float& da) {
-  if (act == AGCN_ACT_RELU) {
+// act(g) and act'(g).  The slopes are formed from e^-|g| (no 1 - s where s is near 1).  F32: within a few 2^-24: the exponent's product
+// with log2 e is carried in two parts, the reciprocal gets one Newton step (silu and sigmoid; with gates() below 115 -> 93 us for a
+// 32768 x 128 x 512 forward that called the library and branched for every value).  bf16 calls, whose results are rounded to eight
+// bits: the hardware's exp2 and reciprocal as they are (a few 2^-24, and |g| 2^-23 from the exponent's rounding), and for the normal
+// distribution function the five-term fit of Abramowitz and Stegun, 7.1.26 (1.4e-7; relative to the tail 3e-5 at g = -2.8,
+// beyond which the library function takes over).
+template <int ACT, bool F32>
+__device__ __forceinline__ void gate(float g, float& a, float& da) {
+  if constexpr (ACT == AGCN_ACT_RELU) {
     a = g > 0.f ? g : 0.f;
     da = g > 0.f ? 1.f : 0.f;
     if (g != g) a = da = g;
-  } else if (act == AGCN_ACT_GELU) {
+  } else if constexpr (ACT == AGCN_ACT_GELU && F32) {
     const float c = 0.5f * erfcf(-0.70710678f * g);
     a = g * c;
     da = fmaf(g, 0.39894228f * expf(-0.5f * g * g), c);
-  } else {
-    const float e = expf(-fabsf(g)), d = 1.f / (1.f + e);
-    const float s = g >= 0.f ? d : e * d, ns = g >= 0.f ? e * d : d;    // sigmoid(g), sigmoid(-g)
-    if (act == AGCN_ACT_SIGMOID) {
-      a = s;
-      da = s * ns;
-    } else {
-      a = g * s;
-      da = s * fmaf(g, ns, 1.f);
-    }
-  }
-}
-// The same for bf16 calls, whose results are rounded to eight bits: the hardware's exp2 and reciprocal (a few 2^-24, and
-// |g| 2^-23 from the exponent's rounding), and for the normal distribution function the five-term fit of Abramowitz and Stegun,
-// 7.1.26 (1.4e-7; relative to the tail 3e-5 at g = -2.8, beyond which the library function takes over).
-__device__ __forceinline__ void gate_of_bf16(int act, float g, float& a, float& da) {
-  if (act == AGCN_ACT_RELU) {
-    gate_of(AGCN_ACT_RELU, g, a, da);
-  } else if (act == AGCN_ACT_GELU) {
+  } else if constexpr (ACT == AGCN_ACT_GELU) {
     const float x = 0.70710678f * fabsf(g), t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.f));
     const float e = __builtin_amdgcn_exp2f(-0.72134752f * g * g);       // e^(-g^2 / 2)
     float q = fmaf(fmaf(fmaf(fmaf(1.061405429f, t, -1.453152027f), t, 1.421413741f), t, -0.284496736f), t, 0.254829592f) * t * e;
@@ -110,15 +97,43 @@ __device__ __forceinline__ void gate_of_bf16(int act, float g, float& a, float& 
     a = g * c;
     da = fmaf(g, 0.39894228f * e, c);
   } else {
-    const float e = __builtin_amdgcn_exp2f(-1.44269504f * fabsf(g)), d = __builtin_amdgcn_rcpf(1.f + e);
-    const float s = g >= 0.f ? d : e * d, ns = g >= 0.f ? e * d : d;
-    if (act == AGCN_ACT_SIGMOID) {
+    float e, d;
+    if constexpr (F32) {
+      const float x = fabsf(g) > 128.f ? -128.f : -fabsf(g);            // (a NaN stays; e^-128 is below every normal number)
+      const float hi = x * 1.44269504f, lo = fmaf(x, 1.925963033e-8f, fmaf(x, 1.44269504f, -hi));
+      e = __builtin_amdgcn_exp2f(hi);
+      e = fmaf(e, lo * 0.69314718f, e);
+      d = __builtin_amdgcn_rcpf(1.f + e);
+      d = fmaf(d, fmaf(-(1.f + e), d, 1.f), d);
+    } else {
+      e = __builtin_amdgcn_exp2f(-1.44269504f * fabsf(g));
+      d = __builtin_amdgcn_rcpf(1.f + e);
+    }
+    const float s = g >= 0.f ? d : e * d, ns = g >= 0.f ? e * d : d;    // sigmoid(g), sigmoid(-g)
+    if constexpr (ACT == AGCN_ACT_SIGMOID) {
       a = s;
       da = s * ns;
     } else {
       a = g * s;
       da = s * fmaf(g, ns, 1.f);
     }
+  }
+}
+// the same for N values: one branch for all, so that their chains run side by side
+template <bool F32, int N>
+__device__ __forceinline__ void gates(int act, const float (&g)[N], float (&a)[N], float (&da)[N]) {
+  if (act == AGCN_ACT_SILU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) gate<AGCN_ACT_SILU, F32>(g[i], a[i], da[i]);
+  } else if (act == AGCN_ACT_GELU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) gate<AGCN_ACT_GELU, F32>(g[i], a[i], da[i]);
+  } else if (act == AGCN_ACT_SIGMOID) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) gate<AGCN_ACT_SIGMOID, F32>(g[i], a[i], da[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) gate<AGCN_ACT_RELU, F32>(g[i], a[i], da[i]);
   }
 }
 
@@ -271,14 +286,13 @@ __device__ __forceinline__ void epilogue(const GemmArgs& g, int m, int n, const 
   const int64_t at = (int64_t)m * g.ldh + n;
   if (EPI == EPI_GATED) {
     F8 hv, pv, qv;
+    float a[8], da[8];
+    gates<F32, 8>(g.act, v0.v, a, da);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      float a, da;
-      if (F32) gate_of(g.act, v0.v[i], a, da);
-      else gate_of_bf16(g.act, v0.v[i], a, da);
-      qv.v[i] = n + i < g.N ? a : 0.f;
-      hv.v[i] = n + i < g.N ? a * v1.v[i] : 0.f;
-      pv.v[i] = n + i < g.N ? da * v1.v[i] : 0.f;
+      qv.v[i] = n + i < g.N ? a[i] : 0.f;
+      hv.v[i] = n + i < g.N ? a[i] * v1.v[i] : 0.f;
+      pv.v[i] = n + i < g.N ? da[i] * v1.v[i] : 0.f;
     }
     if (g.p) {
       store8_kept<F32>(g, g.p, at, pv);
@@ -301,7 +315,9 @@ __device__ __forceinline__ void epilogue(const GemmArgs& g, int m, int n, const 
 #ifdef __HIP_DEVICE_COMPILE__      // (address spaces and builtins that the host pass does not know)
 // The tiles of one operand in a stage: NMAT matrices of PL planes, each ROWS rows of the operand (m or n) by BK, ES bytes an element.
 // T (transposed): the operand's matrix is [k][rows].  Every wave issues kSlots loads of 64 x LB bytes.
-template <int ROWS, bool T, int BK, int PL, int ES, int LB, int NMAT, int WAVES>
+// INTER (transposed bf16): a fragment's lanes q = lane / 16 hold k = 4 q .. 4 q + 3 and 16 + 4 q .. 16 + 4 q + 3 of its 32 (as the
+// accumulators of two neighbouring fragments lie), in place of 8 q .. 8 q + 7.
+template <int ROWS, bool T, int BK, int PL, int ES, int LB, int NMAT, int WAVES, bool INTER = false>
 struct Tiles {
   static constexpr int kEpc = 16 / ES;                         // elements of a chunk
   static constexpr int kRowBytes = (T ? ROWS : BK) * ES, kRowChunks = kRowBytes / 16;
@@ -317,8 +333,9 @@ struct Tiles {
   static __device__ __forceinline__ int perm(int r) {
     if (!T) return kRowBytes == 128 ? (r >> 1) & 7 : (r >> 2) & 3;
     if (ES == 4) return ((r >> 3) & 3) << 2 & (kRowChunks - 1);
-    if (kRowChunks >= 16) return ((r & 3) | ((r >> 3) & 1) << 2) << 1;
-    if (kRowChunks == 8) return (((r >> 1) & 1) | ((r >> 3) & 1) << 1) << 1;
+    constexpr int hb = INTER ? 2 : 3;
+    if (kRowChunks >= 16) return ((r & 3) | ((r >> hb) & 1) << 2) << 1;
+    if (kRowChunks == 8) return (((r >> 1) & 1) | ((r >> hb) & 1) << 1) << 1;
     return ((r >> 3) & 1) << 1;
   }
   __device__ __forceinline__ void init(int row0, int rows, int ld, int wave, int lane) {
@@ -349,7 +366,7 @@ struct Tiles {
   struct Reader {
     int at[T ? FR : 1], lane, row0;
     __device__ __forceinline__ Reader(int row, int lane_) : lane(lane_), row0(row) {
-      const int l = lane & 15, q = lane >> 4, k = ES == 4 ? q * 8 : q * 8 + (l >> 2);
+      const int l = lane & 15, q = lane >> 4, k = ES == 4 ? q * 8 : q * (INTER ? 4 : 8) + (l >> 2);
 #pragma unroll
       for (int f = 0; f < (T ? FR : 0); ++f) {
         // (fp32: a column's 32 bits; bf16: where the transposing read wants this lane to point, four columns of one k)
@@ -366,7 +383,7 @@ struct Tiles {
       } else {
         const AGCN_LDS char* p = s + at[f] + (tile * BK + kk * 32) * kRowBytes;
         const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((AGCN_LDS s16x4*)p);
-        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((AGCN_LDS s16x4*)(p + 4 * kRowBytes));
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((AGCN_LDS s16x4*)(p + (INTER ? 16 : 4) * kRowBytes));
         const u32x2 a = __builtin_bit_cast(u32x2, lo), b = __builtin_bit_cast(u32x2, hi);
         return (u32x4){a.x, a.y, b.x, b.y};
       }
@@ -651,6 +668,220 @@ __global__ __launch_bounds__(256) void ffn_reduce_kernel(GemmArgs g) {
   epilogue<EPI, NB, F32>(g, m, n, o[0], o[NB - 1], kp, kq);
 }
 
+// ---- both products in one kernel: forwards that keep nothing, features of at most 128 -----------------------------------------------------------
+struct FusedArgs {
+  GemmArgs g;                        // seg[0]: X, Wg, Wu with lda, ldb, b_plane; M, N = H, act, two, out, ldo, part, ldp, splits
+  const void* wd;
+  int64_t d_plane;
+  int32_t ldd, Fin, Fout;
+};
+
+// A wave owns 16 rows: their X stays in its registers (as the pieces that the matrix pipe takes), Y's accumulators too, and H is walked
+// in chunks of 32 columns: G and U of the chunk, the gate, and at once the chunk's 32 k of Y.  The gate's results already lie as the
+// next product's operand wants them but for the order of k, and Wd is read in that order: A needs neither memory nor LDS.  The
+// chunk's weights (three matrices, 144 KB of LDS for two stages of fp32 pieces at 128 features) are all that is loaded.
+// A chunk's gate is worked out among the next chunk's first products: the vector unit's work (as much as the matrix pipe's) is
+// hidden there (93 -> 75 us; two dependent products in a row in place of four accumulators in turn: 74 -> 70 us).  32768 x 128 x 512
+// fp32: the call 108 us as two products (80 + 31: the first has four k stages between filling and emptying its tiles, and A's planes
+// are 100 MB each way), 69 here: 1.2 PFLOP/s of bf16 products; bound by the matrix pipe and what is left of the vector unit.
+template <int P, int D, int WV, int ACT>
+__global__ __launch_bounds__(64 * WV) void ffn_fused_kernel(FusedArgs f) {
+#ifdef __HIP_DEVICE_COMPILE__
+  constexpr bool F32 = P == 3;
+  constexpr int KK = D / 32, FO = D / 16, MID = P == 3 ? 1 : 0, LOW = P - 1;
+  typedef Tiles<32, true, D, P, 2, 16, 2, WV> TW;
+  typedef Tiles<D, true, 32, P, 2, 16, 1, WV, true> TD;
+  __shared__ __attribute__((aligned(1024))) char sw0[2 * P * TW::kBytes], sw1[2 * P * TW::kBytes], sd0[P * TD::kBytes], sd1[P * TD::kBytes];
+  AGCN_LDS char *const w0 = (AGCN_LDS char*)sw0, *const w1 = (AGCN_LDS char*)sw1, *const d0 = (AGCN_LDS char*)sd0, *const d1 = (AGCN_LDS char*)sd1;
+  const GemmArgs& g = f.g;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, q = lane >> 4;
+  const int split = blockIdx.x % g.splits, m = (int)(blockIdx.x / g.splits) * (16 * WV) + wave * 16 + r;
+  const int chunks = (g.N + 31) >> 5;
+  const int c0 = (int)((int64_t)chunks * split / g.splits), c1 = (int)((int64_t)chunks * (split + 1) / g.splits);
+  TW tw;
+  TD td;
+  td.init(0, f.Fout, f.ldd, wave, lane);
+  auto load_w = [&](int c, AGCN_LDS char* w) {
+    tw.init(c * 32, g.N, g.ldb, wave, lane);
+    tw.load(g.seg[0].b, g.seg[0].b2, c * 32, g.b_plane, g.ldb, 0, f.Fin, w, wave);
+  };
+  auto load_d = [&](int c, AGCN_LDS char* d) { td.load(f.wd, nullptr, 0, f.d_plane, f.ldd, c, g.N - c * 32, d, wave); };
+  load_w(c0, w0);
+
+  u32x4 xa[P][KK];
+#pragma unroll
+  for (int kk = 0; kk < KK; ++kk) {
+    const int k = kk * 32 + q * 8, left = m < g.M ? f.Fin - k : 0;
+    const int64_t at = (int64_t)m * g.lda + k;
+    if constexpr (F32) {
+      const float* x = static_cast<const float*>(g.seg[0].a) + at;
+      f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
+      if (left >= 8) {
+        const u32x4u a = *reinterpret_cast<const u32x4u*>(x), b = *reinterpret_cast<const u32x4u*>(x + 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { lo[e] = __uint_as_float(a[e]); hi[e] = __uint_as_float(b[e]); }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (e < left) lo[e] = x[e];
+          if (4 + e < left) hi[e] = x[4 + e];
+        }
+      }
+      const Pieces s = split3x8(lo, hi);
+      xa[0][kk] = s.h; xa[MID][kk] = s.m; xa[LOW][kk] = s.l;
+    } else {
+      const uint16_t* x = static_cast<const uint16_t*>(g.seg[0].a) + at;
+      u32x4 v = {0, 0, 0, 0};
+      if (left >= 8) {
+        const u32x4h a = *reinterpret_cast<const u32x4h*>(x);
+        v = (u32x4){a.x, a.y, a.z, a.w};
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) if (e < left) v[e >> 1] |= (uint32_t)x[e] << (16 * (e & 1));
+      }
+      xa[0][kk] = v;
+    }
+  }
+  f32x4 y[FO];
+#pragma unroll
+  for (int j = 0; j < FO; ++j) y[j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  const typename TW::template Reader<2> rw(0, lane);
+  const typename TD::template Reader<FO> rd(0, lane);
+  // (pieces: small terms first)
+  constexpr int NP = P == 1 ? 1 : 6;
+  constexpr int pa[6] = {LOW, 0, MID, MID, 0, 0}, pb[6] = {0, LOW, MID, 0, MID, 0};
+  struct Chunk { f32x4 v[2][2]; };                          // G and U: 16 columns, 16 columns
+  auto first = [&](const AGCN_LDS char* w, Chunk& gu) {
+#pragma unroll
+    for (int b = 0; b < 2; ++b) gu.v[b][0] = gu.v[b][1] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      u32x4 fb[P][2][2];
+#pragma unroll
+      for (int p = 0; p < P; ++p)
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) fb[p][b][j] = rw(w, b * P + p, j, kk);
+#pragma unroll
+      for (int t = 0; t < NP; ++t)
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) gu.v[b][j] = mfma_bf(fb[pb[t]][b][j], xa[pa[t]][kk], gu.v[b][j]);
+    }
+  };
+  struct Gated { float a[8]; u32x4 fa[P]; };
+  auto gated = [&](const Chunk& gu, Gated& o) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float slope;
+      gate<ACT, F32>(gu.v[0][e >> 2][e & 3], o.a[e], slope);
+    }
+    const f32x4 lo = {o.a[0] * gu.v[1][0][0], o.a[1] * gu.v[1][0][1], o.a[2] * gu.v[1][0][2], o.a[3] * gu.v[1][0][3]};
+    const f32x4 hi = {o.a[4] * gu.v[1][1][0], o.a[5] * gu.v[1][1][1], o.a[6] * gu.v[1][1][2], o.a[7] * gu.v[1][1][3]};
+    if constexpr (F32) {
+      const Pieces s = split3x8(lo, hi);
+      o.fa[0] = s.h; o.fa[MID] = s.m; o.fa[LOW] = s.l;
+    } else {
+      o.fa[0] = (u32x4){pk_bf(lo[0], lo[1]), pk_bf(lo[2], lo[3]), pk_bf(hi[0], hi[1]), pk_bf(hi[2], hi[3])};
+    }
+  };
+  auto second = [&](const AGCN_LDS char* d, const Chunk& gu, const Gated& o) {
+    u32x4 low = {0, 0, 0, 0};
+    if constexpr (!F32) {
+      if (g.two) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          x[e] = rest_of(o.a[e] * gu.v[1][e >> 2][e & 3], __uint_as_float(e & 1 ? o.fa[0][e >> 1] & 0xffff0000u : o.fa[0][e >> 1] << 16));
+        low = (u32x4){pk_bf(x[0], x[1]), pk_bf(x[2], x[3]), pk_bf(x[4], x[5]), pk_bf(x[6], x[7])};
+      }
+    }
+#pragma unroll
+    for (int j0 = 0; j0 < FO; j0 += 4) {                    // (four accumulators in turn: one product waits for its last)
+      u32x4 fd[P][4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int p = 0; p < P; ++p) fd[p][j] = rd(d, p, j0 + j, 0);
+      if constexpr (!F32) {
+        if (g.two) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) y[j0 + j] = mfma_bf(fd[0][j], low, y[j0 + j]);
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < NP; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j0 + j] = mfma_bf(fd[pb[t]][j], o.fa[pa[t]], y[j0 + j]);
+    }
+  };
+  // (a stage is there when every wave's loads of it are and all have said so; by then the other stage has been read)
+  auto ready = [] {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(7 << 4);                     // vmcnt(0) lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  auto both = [&](const AGCN_LDS char* w, Chunk& next, const AGCN_LDS char* d, const Chunk& gu) {
+    Gated o;
+    first(w, next);
+    gated(gu, o);
+    second(d, gu, o);
+  };
+  Chunk ga, gb;
+  ready();
+  load_d(c0, d0);
+  if (c0 + 1 < c1) load_w(c0 + 1, w1);
+  first(w0, ga);
+  int c = c0;
+  for (; c + 2 < c1; c += 2) {
+    ready();
+    load_d(c + 1, d1);
+    load_w(c + 2, w0);
+    both(w1, gb, d0, ga);
+    ready();
+    load_d(c + 2, d0);
+    if (c + 3 < c1) load_w(c + 3, w1);
+    both(w0, ga, d1, gb);
+  }
+  ready();
+  Gated o;
+  if (c + 1 < c1) {
+    load_d(c + 1, d1);
+    both(w1, gb, d0, ga);
+    ready();
+    gated(gb, o);
+    second(d1, gb, o);
+  } else {
+    gated(ga, o);
+    second(d0, ga, o);
+  }
+#pragma unroll
+  for (int j = 0; j < FO; ++j) {
+    const int n = j * 16 + q * 4;
+    if (m >= g.M || n >= f.Fout) continue;
+    const f32x4 v = y[j];
+    if (g.splits > 1) {
+      *reinterpret_cast<f32x4*>(g.part + ((int64_t)split * g.M + m) * g.ldp + n) = v;
+    } else if constexpr (F32) {
+      float* o = static_cast<float*>(g.out) + (int64_t)m * g.ldo + n;
+      if (n + 4 <= f.Fout) {
+        *reinterpret_cast<u32x4u*>(o) = (u32x4u){__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) if (n + e < f.Fout) o[e] = v[e];
+      }
+    } else {
+      __bf16* o = static_cast<__bf16*>(g.out) + (int64_t)m * g.ldo + n;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) if (n + e < f.Fout) o[e] = (__bf16)v[e];
+    }
+  }
+#endif
+}
+
 // Few rows (single tokens while serving): bound by the weights' bytes, nothing else is worth waiting for.  A workgroup takes a strip of
 // 128 bytes of the weights' columns, eight lanes a row, eight rows in flight per lane; products and sums in fp32 on the vector unit.
 // The lanes' sums meet by halving exchanges in the wave, then in LDS.  The first product's workgroups take one projection each and
@@ -755,8 +986,10 @@ __global__ __launch_bounds__(512) void ffn_rows_kernel(FewArgs g) {
             G += p[0];
             U += p[(int64_t)g.M * g.ld_sums];
           }
-          if (F32) gate_of(g.act, G, a, da);
-          else gate_of_bf16(g.act, G, a, da);
+          const float one[1] = {G};
+          float oa[1], oda[1];
+          gates<F32, 1>(g.act, one, oa, oda);
+          a = oa[0]; da = oda[0];
         }
         if (g.p && n_wg == 0 && r < g.M) {                          // (pads included: zeros)
           const int64_t at = (int64_t)r * g.ld_sums + k + lx;
@@ -911,6 +1144,17 @@ bool direct(const AgcnFfnDesc& d, const void* p, int cols, int ld) {
 // 35.5 / 36.1, 2000 x 8001 bf16 (no images of the weights) 30 / 59 and 36 / 58, 2048 x 8192 f32 50 / 79 and 56 / 71, 1024 x 4096 f32 20.5 / 30
 // and 20.5 / 31, 128 x 512 17.5 / 17.5 us; 8 rows 43 / 36, 54 / 59, 70 / 72.
 bool few_rows(const AgcnFfnDesc& d) { return d.rows <= 4; }
+
+// Which forwards the fused kernel serves: those that keep nothing (written from its registers, P, Q and A leave in pieces of 16 bytes: 100000
+// x 64 x 4096 bf16 training forward 2250 us, 970 as two products).  Measured as two products / fused, in a captured graph: 4608 x 64 x 256
+// f32 19 / 15 us, bf16 11 / 9; 5 x 64 x 256 f32 15 / 10; 1000 x 64 x 4096 38 / 25; 5 x 64 x 4096 13 / 16; up to 128 features 4608 x 512 f32 35 / 30,
+// bf16 15.8 / 15.4; 10000 x 512 f32 53 / 40; 32768 x 128 45 / 26; but 1000 x 1000 f32 24 / 27, 4608 x 128 17 / 23 (a chunk of 128 features
+// takes a workgroup 3 us, whatever its neighbours do).
+bool wide(const AgcnFfnDesc& d) { return d.Fin > 64 || d.Fout > 64; }
+bool fused(const AgcnFfnDesc& d) {
+  if (d.training || few_rows(d) || d.Fin > 128 || d.Fout > 128) return false;
+  return !wide(d) || d.rows * d.H >= 1 << 21;
+}
 
 // What the forward leaves for the backward.  The images are there only where a matrix cannot be read as it is; room is kept for
 // them whenever the SIZES alone would not rule them out (an address can be odd).
@@ -1076,7 +1320,10 @@ struct ImageList {
   ImageList() { std::memset(&a, 0, sizeof(a)); }
   Mat add(const AgcnFfnDesc& d, const void* src, int64_t rows, int cols, int ld, void* dst, bool in_place) {
     if (in_place) return {src, ld, 0, whole_chunks(d, src, cols, ld)};
-    const int lp = pad8(cols), op = op_of(d);
+    return image(op_of(d), src, rows, cols, ld, dst);
+  }
+  Mat image(int op, const void* src, int64_t rows, int cols, int ld, void* dst) {
+    const int lp = pad8(cols);
     Image& im = a.im[a.n++];
     im = {src, dst, rows, rows * lp, a.chunks, cols, ld, lp, op == OP_PLANES};
     a.chunks += rows * (lp >> 3);
@@ -1104,7 +1351,65 @@ int pieces_of(const AgcnFfnDesc& d) { return two_pieces(d) ? 2 : 1; }
 size_t product_part(const AgcnFfnDesc& d, int64_t M, int64_t N, int nb, int64_t K, int nseg, bool gates) {
   return part_bytes(choose(M, N, nb, op_of(d), nseg * ktiles_of(d, K), gates), M, N, nb);
 }
+// The fused kernel: workgroups, splits of H, and the weights' planes.  The splits by a model like choose()'s: a chunk takes a workgroup
+// t_chunk on a CU of its own (microseconds, measured), workgroups that share a CU overlap (not those of fp32 pieces of 128 features: they
+// fill its LDS), and parts cost a launch and their way to memory and back: 10000 x 64 x 256 fp32 18.4 us whole, 22.7 in two
+// parts; 10000 x 64 x 4096 193 whole, 107 in three.
+struct Fused { int waves, blocks, splits, ldp; size_t planes, part; };
+Fused fused_of(const AgcnFfnDesc& d) {
+  const bool f32 = d.dtype == AGCN_DTYPE_F32;
+  Fused c;
+  c.waves = f32 && wide(d) ? 8 : 4;
+  c.blocks = (int)cdiv(std::max<int64_t>(1, d.rows), 16 * c.waves);
+  c.splits = 1;
+  const float t_chunk = f32 ? (wide(d) ? 3.2f : 1.5f) : (wide(d) ? 1.0f : 0.6f);
+  const int64_t chunks = cdiv(d.H, 32);
+  float least = 1e30f;
+  for (int s = 1; s <= 32 && s <= chunks; ++s) {
+    const int64_t per_cu = cdiv((int64_t)c.blocks * s, 256);
+    float t = cdiv(chunks, s) * t_chunk * (per_cu == 1 || c.waves == 8 ? per_cu : 0.7f * per_cu);
+    if (s > 1) t += 3.5f + (float)s * d.rows * pad8(d.Fout) * 2e-6f;
+    if (t < least) {
+      least = t;
+      c.splits = s;
+    }
+  }
+  c.ldp = pad8(d.Fout);
+  c.planes = f32 ? align256((size_t)6 * (2 * (size_t)d.Fin * pad8(d.H) + (size_t)d.H * pad8(d.Fout))) : 0;
+  c.part = c.splits > 1 ? align256((size_t)c.splits * d.rows * c.ldp * sizeof(float)) : 0;
+  return c;
+}
+template <int P, int D, int WV>
+void fused_launch(const FusedArgs& f, const Fused& c, hipStream_t s) {
+  const dim3 grid((unsigned)((int64_t)c.blocks * c.splits)), block(64 * WV);
+  if (f.g.act == AGCN_ACT_SILU) hipLaunchKernelGGL((ffn_fused_kernel<P, D, WV, AGCN_ACT_SILU>), grid, block, 0, s, f);
+  else if (f.g.act == AGCN_ACT_GELU) hipLaunchKernelGGL((ffn_fused_kernel<P, D, WV, AGCN_ACT_GELU>), grid, block, 0, s, f);
+  else if (f.g.act == AGCN_ACT_SIGMOID) hipLaunchKernelGGL((ffn_fused_kernel<P, D, WV, AGCN_ACT_SIGMOID>), grid, block, 0, s, f);
+  else hipLaunchKernelGGL((ffn_fused_kernel<P, D, WV, AGCN_ACT_RELU>), grid, block, 0, s, f);
+}
+void fused_forward(const AgcnFfnDesc& d, const void* X, const Mat& wg, const Mat& wu, const Mat& wd, void* Y, float* part, hipStream_t s) {
+  const Fused c = fused_of(d);
+  FusedArgs f;
+  std::memset(&f, 0, sizeof(f));
+  GemmArgs& g = f.g;
+  g = base_args(d);
+  g.seg[0] = {X, wg.p, wu.p};
+  g.lda = d.ldx; g.ldb = wg.ld; g.b_plane = wg.plane;
+  g.M = (int)d.rows; g.N = d.H;
+  g.out = Y; g.ldo = d.Fout; g.part = part; g.ldp = c.ldp; g.splits = c.splits;
+  f.wd = wd.p; f.d_plane = wd.plane; f.ldd = wd.ld; f.Fin = d.Fin; f.Fout = d.Fout;
+  if (g.f32) wide(d) ? fused_launch<3, 128, 8>(f, c, s) : fused_launch<3, 64, 4>(f, c, s);
+  else wide(d) ? fused_launch<1, 128, 4>(f, c, s) : fused_launch<1, 64, 4>(f, c, s);
+  if (c.splits == 1) return;
+  GemmArgs q = g;
+  q.N = d.Fout;
+  const dim3 grid((unsigned)cdiv((int64_t)q.M * (q.ldp / 8), 32));
+  if (g.f32) hipLaunchKernelGGL((ffn_reduce_kernel<1, EPI_STORE, true>), grid, dim3(256), 0, s, q);
+  else hipLaunchKernelGGL((ffn_reduce_kernel<1, EPI_STORE, false>), grid, dim3(256), 0, s, q);
+}
+
 size_t forward_part(const AgcnFfnDesc& d) {
+  if (fused(d)) return fused_of(d).planes + fused_of(d).part;
   if (few_rows(d)) return few_of(d, d.H, d.Fin, 2).part + few_of(d, d.Fout, d.H, 1).part;
   return std::max(product_part(d, d.rows, pad8(d.H), 2, d.Fin, 1, true), product_part(d, d.rows, d.Fout, 1, d.H, pieces_of(d), false));
 }
@@ -1162,6 +1467,26 @@ extern "C" int agcn_gated_ffn_forward(const AgcnFfnDesc* desc, const void* X, co
   hipStream_t s = static_cast<hipStream_t>(hip_stream);
   ImageList list;
   const InPlace in(d, X, Wg, Wu, Wd);
+  if (fused(d)) {
+    const Fused c = fused_of(d);
+    Mat w[3];
+    if (c.planes) {
+      char* at = static_cast<char*>(workspace);
+      const size_t one = (size_t)6 * d.Fin * pad8(d.H);
+      w[0] = list.image(OP_PLANES, Wg, d.Fin, d.H, d.H, at);
+      w[1] = list.image(OP_PLANES, Wu, d.Fin, d.H, d.H, at + one);
+      w[2] = list.image(OP_PLANES, Wd, d.H, d.Fout, d.Fout, at + 2 * one);
+    } else {
+      w[0] = list.add(d, Wg, d.Fin, d.H, d.H, r.wg, in.w);
+      w[1] = list.add(d, Wu, d.Fin, d.H, d.H, r.wu, in.w);
+      w[2] = list.add(d, Wd, d.H, d.Fout, d.Fout, r.wd, in.wd);
+    }
+    list.launch(s);
+    fused_forward(d, X, w[0], w[1], w[2], Y, reinterpret_cast<float*>(static_cast<char*>(workspace) + c.planes), s);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return fail(AGCN_EDEVICE, "%s: %s", who, hipGetErrorString(e));
+    return AGCN_OK;
+  }
   const Mat x = list.add(d, X, d.rows, d.Fin, d.ldx, r.x, in.x), wg = list.add(d, Wg, d.Fin, d.H, d.H, r.wg, in.w),
             wu = list.add(d, Wu, d.Fin, d.H, d.H, r.wu, in.w), wd = list.add(d, Wd, d.H, d.Fout, d.Fout, r.wd, in.wd);
   if (few_rows(d)) {

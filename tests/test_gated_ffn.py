@@ -73,11 +73,12 @@ def run(amd, X, Wg, Wu, Wd, dY, act):
     Y = amd.gated_ffn(*ts, activation=act)
     g = torch.autograd.grad(Y, ts, dY)
     with torch.no_grad():
-        assert torch.equal(amd.gated_ffn(X, Wg, Wu, Wd, activation=act), Y)      # the form that keeps nothing
-    return dict(zip(("Y", "dX", "dWg", "dWu", "dWd"), (Y.detach(),) + g))
+        serving = amd.gated_ffn(X, Wg, Wu, Wd, activation=act)                   # the form that keeps nothing
+    return dict(zip(("Y", "dX", "dWg", "dWu", "dWd", "serving"), (Y.detach(),) + g + (serving,)))
 
 
 def check(got, out, err, dtype):
+    out, err = dict(out, serving=out["Y"]), dict(err, serving=err["Y"])
     b = B8 if dtype == bf16 else E
     for k in out:
         assert got[k].shape == out[k].shape and got[k].dtype == dtype
@@ -111,6 +112,7 @@ def check_exact(amd, args, dtype):
     got = run(amd, *args, "relu")
     out, _, inner = reference(*args, "relu", dtype)
     assert inner <= 256
+    out["serving"] = out["Y"]
     for k in out:
         assert float(out[k].abs().max()) < 2 ** 24
         assert torch.equal(got[k], out[k].to(dtype)), k
@@ -292,6 +294,40 @@ def test_few_rows(amd, rows, size, dtype):
     args = real(rows * sum(size), rows, *size, dtype)
     out, err, _ = reference(*args, "silu", dtype)
     check(run(amd, *args, "silu"), out, err, dtype)
+
+
+# features of at most 128 have a forward of their own that keeps nothing: both widths of it, rows and chunks of H that end inside a tile, H
+# in one part and in several, odd numbers of chunks
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [f32, bf16])
+@pytest.mark.parametrize("size", [(5, 64, 32, 64), (70, 33, 97, 17), (1500, 64, 1000, 50), (20000, 16, 40, 64), (33, 8, 1, 1), (4200, 100, 520, 128), (17000, 65, 130, 9), (33000, 128, 70, 128), (2100, 7, 1100, 127)])
+def test_narrow_features(amd, size, dtype):
+    check_exact(amd, integers(sum(size), *size, dtype), dtype)
+    args = real(sum(size) + 1, *size, dtype)
+    for act in ("gelu", "sigmoid"):
+        out, err, _ = reference(*args, act, dtype)
+        check(run(amd, *args, act), out, err, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [f32, bf16])
+@pytest.mark.parametrize("size", [(700, 50, 330, 30), (17000, 90, 130, 70)])
+def test_narrow_features_at_any_address(amd, size, dtype):
+    rows, F, H, O = size
+    X, Wg, Wu, Wd, _ = real(7, *size, dtype)
+    want = amd.gated_ffn(X, Wg, Wu, Wd)
+    wide = torch.full((rows + 1, F + 9), float("nan"), dtype=dtype, device="cuda")
+    wide[:rows, 3:3 + F] = X
+    moved = []
+    for w in (Wg, Wu, Wd):
+        flat = torch.full((w.numel() + 12,), float("nan"), dtype=dtype, device="cuda")
+        flat[1:1 + w.numel()] = w.reshape(-1)
+        moved.append(flat[1:1 + w.numel()].view(w.shape))
+    assert torch.equal(amd.gated_ffn(wide[:rows, 3:3 + F], *moved), want)
+    X[rows // 2] = float("nan")                               # a row is a row of its own
+    got = amd.gated_ffn(X, Wg, Wu, Wd)
+    keep = torch.arange(rows, device="cuda") != rows // 2
+    assert torch.equal(got[keep], want[keep]) and bool(got[rows // 2].isnan().all())
 
 
 @pytest.mark.gpu
