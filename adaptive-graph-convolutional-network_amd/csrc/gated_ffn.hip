@@ -670,7 +670,7 @@ __global__ __launch_bounds__(256) void ffn_reduce_kernel(GemmArgs g) {
 
 // ---- both products in one kernel: forwards that keep nothing, features of at most 128 -----------------------------------------------------------
 struct FusedArgs {
-  GemmArgs g;                        // seg[0]: X, Wg, Wu with lda, ldb, b_plane; M, N = H, act, two, out, ldo, part, ldp, splits
+  GemmArgs g;                        // seg[0]: X, Wg, Wu with lda, ldb, b_plane; M, N = H, act, out, ldo, part, ldp, splits
   const void* wd;
   int64_t d_plane;
   int32_t ldd, Fin, Fout;
@@ -683,7 +683,9 @@ struct FusedArgs {
 // A chunk's gate is worked out among the next chunk's first products: the vector unit's work (as much as the matrix pipe's) is
 // hidden there (93 -> 75 us; two dependent products in a row in place of four accumulators in turn: 74 -> 70 us).  32768 x 128 x 512
 // fp32: the call 108 us as two products (80 + 31: the first has four k stages between filling and emptying its tiles, and A's planes
-// are 100 MB each way), 69 here: 1.2 PFLOP/s of bf16 products; bound by the matrix pipe and what is left of the vector unit.
+// are 100 MB each way), 70 here: 1.2 PFLOP/s of bf16 products; bound by the matrix pipe and what is left of the vector unit.
+// bf16 calls give A to the second product in two pieces (851 x 16 x 5656, one piece: 1.5 times the error of an unrounded A; 32768 x 64 x 256
+// 12.8 -> 14.7 us, as two products 21.5).
 template <int P, int D, int WV, int ACT>
 __global__ __launch_bounds__(64 * WV) void ffn_fused_kernel(FusedArgs f) {
 #ifdef __HIP_DEVICE_COMPILE__
@@ -771,33 +773,27 @@ __global__ __launch_bounds__(64 * WV) void ffn_fused_kernel(FusedArgs f) {
           for (int j = 0; j < 2; ++j) gu.v[b][j] = mfma_bf(fb[pb[t]][b][j], xa[pa[t]][kk], gu.v[b][j]);
     }
   };
-  struct Gated { float a[8]; u32x4 fa[P]; };
+  struct Gated { u32x4 fa[F32 ? 3 : 2]; };                  // A's pieces (bf16 calls: two, so that it is rounded nowhere that shows)
   auto gated = [&](const Chunk& gu, Gated& o) {
+    f32x4 A[2];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      float slope;
-      gate<ACT, F32>(gu.v[0][e >> 2][e & 3], o.a[e], slope);
+      float a, slope;
+      gate<ACT, F32>(gu.v[0][e >> 2][e & 3], a, slope);
+      A[e >> 2][e & 3] = a * gu.v[1][e >> 2][e & 3];
     }
-    const f32x4 lo = {o.a[0] * gu.v[1][0][0], o.a[1] * gu.v[1][0][1], o.a[2] * gu.v[1][0][2], o.a[3] * gu.v[1][0][3]};
-    const f32x4 hi = {o.a[4] * gu.v[1][1][0], o.a[5] * gu.v[1][1][1], o.a[6] * gu.v[1][1][2], o.a[7] * gu.v[1][1][3]};
     if constexpr (F32) {
-      const Pieces s = split3x8(lo, hi);
+      const Pieces s = split3x8(A[0], A[1]);
       o.fa[0] = s.h; o.fa[MID] = s.m; o.fa[LOW] = s.l;
     } else {
-      o.fa[0] = (u32x4){pk_bf(lo[0], lo[1]), pk_bf(lo[2], lo[3]), pk_bf(hi[0], hi[1]), pk_bf(hi[2], hi[3])};
+      const u32x4 h = {pk_bf(A[0][0], A[0][1]), pk_bf(A[0][2], A[0][3]), pk_bf(A[1][0], A[1][1]), pk_bf(A[1][2], A[1][3])};
+      o.fa[0] = h;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) A[e >> 2][e & 3] = rest_of(A[e >> 2][e & 3], __uint_as_float(e & 1 ? h[e >> 1] & 0xffff0000u : h[e >> 1] << 16));
+      o.fa[1] = (u32x4){pk_bf(A[0][0], A[0][1]), pk_bf(A[0][2], A[0][3]), pk_bf(A[1][0], A[1][1]), pk_bf(A[1][2], A[1][3])};
     }
   };
-  auto second = [&](const AGCN_LDS char* d, const Chunk& gu, const Gated& o) {
-    u32x4 low = {0, 0, 0, 0};
-    if constexpr (!F32) {
-      if (g.two) {
-        float x[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          x[e] = rest_of(o.a[e] * gu.v[1][e >> 2][e & 3], __uint_as_float(e & 1 ? o.fa[0][e >> 1] & 0xffff0000u : o.fa[0][e >> 1] << 16));
-        low = (u32x4){pk_bf(x[0], x[1]), pk_bf(x[2], x[3]), pk_bf(x[4], x[5]), pk_bf(x[6], x[7])};
-      }
-    }
+  auto second = [&](const AGCN_LDS char* d, const Gated& o) {
 #pragma unroll
     for (int j0 = 0; j0 < FO; j0 += 4) {                    // (four accumulators in turn: one product waits for its last)
       u32x4 fd[P][4];
@@ -806,10 +802,8 @@ __global__ __launch_bounds__(64 * WV) void ffn_fused_kernel(FusedArgs f) {
 #pragma unroll
         for (int p = 0; p < P; ++p) fd[p][j] = rd(d, p, j0 + j, 0);
       if constexpr (!F32) {
-        if (g.two) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) y[j0 + j] = mfma_bf(fd[0][j], low, y[j0 + j]);
-        }
+        for (int j = 0; j < 4; ++j) y[j0 + j] = mfma_bf(fd[0][j], o.fa[1], y[j0 + j]);
       }
 #pragma unroll
       for (int t = 0; t < NP; ++t)
@@ -828,7 +822,7 @@ __global__ __launch_bounds__(64 * WV) void ffn_fused_kernel(FusedArgs f) {
     Gated o;
     first(w, next);
     gated(gu, o);
-    second(d, gu, o);
+    second(d, o);
   };
   Chunk ga, gb;
   ready();
@@ -853,10 +847,10 @@ __global__ __launch_bounds__(64 * WV) void ffn_fused_kernel(FusedArgs f) {
     both(w1, gb, d0, ga);
     ready();
     gated(gb, o);
-    second(d1, gb, o);
+    second(d1, o);
   } else {
     gated(ga, o);
-    second(d0, ga, o);
+    second(d0, o);
   }
 #pragma unroll
   for (int j = 0; j < FO; ++j) {
@@ -1147,8 +1141,8 @@ bool few_rows(const AgcnFfnDesc& d) { return d.rows <= 4; }
 
 // Which forwards the fused kernel serves: those that keep nothing (written from its registers, P, Q and A leave in pieces of 16 bytes: 100000
 // x 64 x 4096 bf16 training forward 2250 us, 970 as two products).  Measured as two products / fused, in a captured graph: 4608 x 64 x 256
-// f32 19 / 15 us, bf16 11 / 9; 5 x 64 x 256 f32 15 / 10; 1000 x 64 x 4096 38 / 25; 5 x 64 x 4096 13 / 16; up to 128 features 4608 x 512 f32 35 / 30,
-// bf16 15.8 / 15.4; 10000 x 512 f32 53 / 40; 32768 x 128 45 / 26; but 1000 x 1000 f32 24 / 27, 4608 x 128 17 / 23 (a chunk of 128 features
+// f32 19 / 15 us, bf16 11 / 10; 5 x 64 x 256 f32 15 / 10; 1000 x 64 x 4096 38 / 25; 5 x 64 x 4096 13 / 16; up to 128 features 4608 x 512 f32 35 / 30,
+// bf16 15.8 / 16.1; 10000 x 512 f32 53 / 40; 32768 x 128 45 / 26; but 1000 x 1000 f32 24 / 27, 4608 x 128 17 / 23 (a chunk of 128 features
 // takes a workgroup 3 us, whatever its neighbours do).
 bool wide(const AgcnFfnDesc& d) { return d.Fin > 64 || d.Fout > 64; }
 bool fused(const AgcnFfnDesc& d) {
