@@ -1157,11 +1157,13 @@ size_t carve_reserve(const AgcnFfnDesc& d, void* mem, Reserve* r) {
   Carve c{static_cast<char*>(mem), 0};
   const int op = op_of(d), Hp = pad8(d.H), Fp = pad8(d.Fin), Op = pad8(d.Fout);
   const size_t image = op == OP_BF16 ? 2 : op == OP_FP32 ? 0 : 6, e = two_pieces(d) || op == OP_FP32 ? 4 : image, kept = d.dtype == AGCN_DTYPE_F32 ? 4 : 3;
-  r->x = c.take(image * d.rows * Fp);
-  r->wg = c.take(image * d.Fin * Hp);
-  r->wu = c.take(image * d.Fin * Hp);
-  r->wd = c.take(image * d.H * Op);
-  r->hid = c.take(e * d.rows * Hp);
+  const bool served = !d.training && few_rows(d), one = fused(d);        // (neither reads images nor A; fp32 planes lie in the workspace)
+  const size_t weights = served || (one && d.dtype == AGCN_DTYPE_F32) ? 0 : image;
+  r->x = c.take(served || one ? 0 : image * d.rows * Fp);
+  r->wg = c.take(weights * d.Fin * Hp);
+  r->wu = c.take(weights * d.Fin * Hp);
+  r->wd = c.take(weights * d.H * Op);
+  r->hid = c.take(served || one ? 0 : e * d.rows * Hp);
   r->p = d.training ? c.take(kept * d.rows * Hp) : nullptr;
   r->q = d.training ? c.take(kept * d.rows * Hp) : nullptr;
   return c.off;

@@ -1007,7 +1007,8 @@ class GatedFfnFunction(torch.autograd.Function):
 def gated_ffn(X, w_gate, w_up, w_down, activation="silu"):
     """Gated feed-forward block over node rows: (act(X w_gate) * (X w_up)) w_down.  X [rows, F], w_gate and w_up [F, H], w_down
     [H, F_out], all float32 or all bfloat16; activation: 'silu', 'gelu' (the erf form), 'relu' or 'sigmoid'.  Every row is a
-    row of its own: pad rows that are zero come out zero."""
+    row of its own: pad rows that are zero come out zero.  The kernels are chosen by the sizes and by whether a gradient is wanted: a
+    row's last bits may differ between batch sizes, and between serving and training."""
     if activation not in _ffi.FFN_ACT:
         raise ValueError("activation must be one of %s" % ", ".join(sorted(_ffi.FFN_ACT)))
     if _wants_grad((X, w_gate, w_up, w_down)):

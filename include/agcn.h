@@ -418,7 +418,8 @@ AGCN_API int agcn_cast_rows(const void* src, int32_t src_dtype, void* dst, int32
  *   Y = (act(X Wg) (.) (X Wu)) Wd          X [rows, ldx] (Fin used), Wg, Wu [Fin, H], Wd [H, Fout], Y [rows, Fout]
  * All matrices are of one type (f32 | bf16).  f32 products run on the bf16 matrix pipe at fp32 accuracy (csrc/bf16_split.h: a row that
  * holds an infinity or a NaN comes out non-finite, but an infinity may come out as NaN); bf16 calls round the block's inner
- * matrices to bf16, sums are fp32.  reserve (256-byte aligned, agcn_gated_ffn_reserve_bytes): scratch of the forward; with
+ * matrices to bf16 (small calls keep a second piece), sums are fp32.  The kernels are chosen by the sizes, the type and `training`:
+ * a row's result may differ in its last bits with the number of rows beside it, and between training = 0 and 1.  reserve (256-byte aligned, agcn_gated_ffn_reserve_bytes): scratch of the forward; with
  * training = 1 the backward needs it as the forward left it, and X, Wg, Wu, Wd unchanged at the same addresses.
  * Backward: dX [rows, Fin], dWg, dWu (together), dWd are each nullable. Fixed-order sums: bit-reproducible.
  * rows = 0: the forward does nothing, the backward writes zeros. */
