@@ -13,9 +13,9 @@
 // memory's latency where a row after another would not.  Sums, means and column sums are fp32 (a column sum's partials, one per
 // workgroup, are added in a fixed order: no atomics); rounding happens where a result is stored, and h is taken from the unrounded
 // y.  Pad rows give zeros and take part in no sum.
-// Measured, forward / backward: 32768 x 4096 bf16 190 / 357 us (1074 MB: 5.6 TB/s; 1611 MB: 4.5 TB/s, registers leave half of the
-// forward's waves); 19978 x 1001, fp32 rows, bf16 z and a gate per element 71 / 134 us (3.9 and 3.3 TB/s: rows at odd addresses, sigmoids);
-// 4600 x 256 fp32 with a gate per graph 8.5 / 30 us in three launches.
+// Measured, forward / backward: 32916 x 4096 bf16 190 / 357 us (1074 MB: 5.6 TB/s; 1611 MB: 4.5 TB/s, registers leave half of the
+// forward's waves); 19202 x 1001, fp32 rows, bf16 z and a gate per element 71 / 134 us (3.9 and 3.3 TB/s: rows at odd addresses, sigmoids);
+// 4071 x 256 fp32 with a gate per graph 8.5 / 30 us in three launches.
 #include <hip/hip_bf16.h>
 #include <hip/hip_runtime.h>
 
@@ -297,7 +297,7 @@ __global__ __launch_bounds__(threads_of<L>()) void norm_forward_kernel(NormArgs 
 // y is formed again from x, z and the gate, which have to be read anyway (x in y's place): the stored y may be rounded to
 // bf16, and a row whose features differ by less than that rounding would get a wrong yh.
 // AHEAD: the next row's operands are fetched while a row is worked on.  It pays where it costs few registers (bf16 rows, no gate, no
-// means: 32768 x 4096 463 -> 395 us); with more it spills.
+// means: 32916 x 4096 463 -> 395 us); with more it spills.
 template <typename TX, typename TZ, int L, int NV, bool LAYER, bool GATED>
 __global__ __launch_bounds__(threads_of<L>(), LAYER || GATED ? 3 : 4) void norm_backward_kernel(NormArgs a) {
   constexpr bool AHEAD = !LAYER && !GATED && NV == 1 && sizeof(TX) == 2;
