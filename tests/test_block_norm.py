@@ -362,6 +362,26 @@ def test_other_stream_and_replayed_graph(amd):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind,gate", [("rms", "none"), ("layer", "row")])
+def test_offsets_beyond_32_bits(amd, kind, gate):
+    """more than 2^31 elements: the last rows' results are those of a call on the last rows alone"""
+    rows, F, last = 132000, 16384, 7
+    g = torch.Generator(device="cuda").manual_seed(1)
+    t = {k: torch.randn(rows, F, generator=g, device="cuda", dtype=torch.bfloat16) for k in ("z", "x") + (("gate",) if gate == "row" else ())}
+    v = {k: 1 + 0.1 * torch.randn(F, generator=g, device="cuda") for k in ("scale", "post_weight", "pre_weight")}
+    if kind == "layer":
+        v.update({k: 0.1 * torch.randn(F, generator=g, device="cuda") for k in ("post_bias", "pre_bias")})
+    dy, dh = t["x"].flip(1), t["z"].flip(1)
+
+    def call(cut):
+        ts = {k: a[cut].detach().requires_grad_(True) for k, a in t.items()}
+        out = amd.norm_gate_residual(**ts, **v, norm=kind, gate_activation="tanh" if gate == "row" else "linear")
+        return out + torch.autograd.grad(out, list(ts.values()), (dy[cut], dh[cut]))
+    for a, b in zip(call(slice(None)), call(slice(rows - last, rows))):
+        assert torch.equal(a[rows - last:], b)
+
+
+@pytest.mark.gpu
 def test_a_second_derivative_is_refused(amd):
     d = make(30, 6, 32)
     x = d["x"].requires_grad_(True)

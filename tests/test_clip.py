@@ -124,6 +124,17 @@ def test_none_entries_strides_and_bucket(amd):
 
 
 @pytest.mark.gpu
+def test_a_tensor_of_more_than_2_to_the_31_elements(amd):
+    n = (1 << 31) + 1003
+    t = torch.ones(n, device="cuda", dtype=torch.bfloat16)
+    t[-5:] = 3.0
+    norm64_ = float(np.sqrt((n - 5) + 45.0))
+    (out,), norm = amd.clip_by_global_norm([t], norm64_ / 2)
+    assert abs(float(norm) - norm64_) <= 2 * E * norm64_
+    assert bool((out[:-5] == 0.5).all()) and bool((out[-5:] == 1.5).all())      # (k = 0.5 within 2 E: a bf16 rounds to the same)
+
+
+@pytest.mark.gpu
 def test_clip_in_a_replayed_graph_and_on_another_stream(amd):
     ts = tensors(2, [5000, 3, 70001], [f32, bf16, f32])
     s = torch.cuda.Stream()

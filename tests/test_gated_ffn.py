@@ -284,6 +284,52 @@ def test_other_stream_and_replayed_graph(amd, dtype):
             assert torch.equal(r, out[k].to(dtype)), k
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [f32, bf16])
+@pytest.mark.parametrize("size", [(1, 600, 2100, 80), (3, 40, 64, 24), (500, 64, 1000, 60), (17000, 96, 160, 100), (90, 300, 200, 150)])
+def test_replayed_serving_calls(amd, size, dtype):
+    """Two calls in one graph, so that the second's scratch may lie where the first's was; replayed between eager calls."""
+    a, b = integers(80, *size, dtype)[:4], integers(81, *size, dtype)[:4]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        amd.gated_ffn(*a, activation="relu")
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ya = amd.gated_ffn(*a, activation="relu")
+        yb = amd.gated_ffn(*b, activation="relu")
+    for seed in range(3):
+        for args, off in ((a, 0), (b, 50)):
+            for t, v in zip(args, integers(90 + seed + off, *size, dtype)):
+                t.copy_(v)
+        graph.replay()
+        eager = amd.gated_ffn(*a, activation="relu")
+        torch.cuda.synchronize()
+        for args, y in ((a, ya), (b, yb), (a, eager)):
+            X, Wg, Wu, Wd = (t.double() for t in args)
+            assert torch.equal(y, (((X @ Wg).clamp(min=0) * (X @ Wu)) @ Wd).to(dtype))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [f32, bf16])
+@pytest.mark.parametrize("size", [(2300, 32, 40, 16), (2300, 200, 40, 16), (2300, 200, 3000, 160)])
+def test_offsets_beyond_32_bits(amd, size, dtype):
+    """rows 2^20 elements apart: the last ones lie more than 2^31 elements behind the first"""
+    X, Wg, Wu, Wd, dY = real(9, *size, dtype)
+    far = torch.empty((size[0], 1 << 20), dtype=dtype, device="cuda")[:, :size[1]]
+    far.copy_(X)
+    assert torch.equal(amd.gated_ffn(far, Wg, Wu, Wd), amd.gated_ffn(X, Wg, Wu, Wd))
+    both = []
+    for x in (far, X):
+        ts = [t.detach().requires_grad_(True) for t in (x, Wg, Wu, Wd)]
+        Y = amd.gated_ffn(*ts)
+        both.append((Y,) + torch.autograd.grad(Y, ts, dY))
+    for a, b in zip(*both):
+        assert torch.equal(a, b)
+
+
 # few rows have kernels of their own; the sizes cut k in parts in neither, one or both of their products, strips end inside a chunk
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [f32, bf16])
