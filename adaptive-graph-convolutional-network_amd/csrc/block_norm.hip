@@ -14,14 +14,15 @@
 // workgroup, are added in a fixed order: no atomics); rounding happens where a result is stored, and h is taken from the unrounded
 // y.  Pad rows give zeros and take part in no sum.
 // Measured, forward / backward: 32916 x 4096 bf16 190 / 357 us (1074 MB: 5.6 TB/s; 1611 MB: 4.5 TB/s, registers leave half of the
-// forward's waves); 19202 x 1001, fp32 rows, bf16 z and a gate per element 71 / 134 us (3.9 and 3.3 TB/s: rows at odd addresses, sigmoids);
-// 4071 x 256 fp32 with a gate per graph 8.5 / 30 us in three launches.
+// forward's waves); 19202 x 1001, fp32 rows, bf16 z and a gate per element 66 / 120 us (4.1 and 3.5 TB/s: rows at odd addresses, sigmoids);
+// 4071 x 256 fp32 with a gate per graph 8 / 26 us in three launches.
 #include <hip/hip_bf16.h>
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
 
 #include "agcn_device.h"
+#include "gate_math.h"
 #include "sgc_kernels.h"
 
 namespace agcn {
@@ -118,16 +119,37 @@ __device__ __forceinline__ void store8(__hip_bfloat16* p_, int c, int F, const f
   }
 }
 
-__device__ __forceinline__ float gate_act(int act, float g) {
-  if (act == AGCN_ACT_TANH) return tanhf(g);
-  if (act == AGCN_ACT_SIGMOID) return 1.f / (1.f + expf(-g));
-  return g;
+// The gate's activation and its slope, which is formed from e^-|g| (1 - a^2 and a (1 - a) lose their digits where the activation is flat).
+// tanh below 1/4: its series (1 - e^-2|g| loses digits there; the first term left out is 2^-26 of the sum).
+__device__ __forceinline__ float series_tanh(float g) {
+  const float t = g * g;
+  return fmaf(g * t, fmaf(t, fmaf(t, fmaf(t, 0.021869489f, -0.053968254f), 0.13333333f), -0.33333333f), g);
 }
-// a'(g), from g: 1 - a^2 and a (1 - a) lose their digits where the activation is flat (e^-2|g| and e^-|g| do not)
-__device__ __forceinline__ float gate_slope(int act, float g) {
-  if (act == AGCN_ACT_LINEAR) return 1.f;
-  const float e = expf(act == AGCN_ACT_TANH ? -2.f * fabsf(g) : -fabsf(g)), d = 1.f / (1.f + e);
-  return (act == AGCN_ACT_TANH ? 4.f : 1.f) * e * d * d;
+// N gates: one branch on the activation for all.  (Against the library's functions, called for each value where it was needed: 19202 x 1001
+// with sigmoids forward 71 -> 66, backward 134 -> 120 us.)
+template <int N>
+__device__ __forceinline__ void gates(int act, const float (&g)[N], float (&a)[N], float (&slope)[N]) {
+  if (act == AGCN_ACT_SIGMOID) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float e = exp_neg(fabsf(g[i])), d = recip_1p(e);
+      a[i] = g[i] >= 0.f ? d : e * d;
+      slope[i] = e * d * d;
+    }
+  } else if (act == AGCN_ACT_TANH) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float e = exp_neg(2.f * fabsf(g[i])), d = recip_1p(e);
+      a[i] = fabsf(g[i]) < 0.25f ? series_tanh(g[i]) : copysignf((1.f - e) * d, g[i]);
+      slope[i] = 4.f * e * d * d;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      a[i] = g[i];
+      slope[i] = 1.f;
+    }
+  }
 }
 
 // Sums of N values over the L lanes of a row; every lane gets them.  L > 64: over the row's waves through `red`
@@ -267,9 +289,17 @@ __global__ __launch_bounds__(threads_of<L>()) void norm_forward_kernel(NormArgs 
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
         const int c = (k * L + lane) * V;
+        float slope[V];
+        if (a.gate) {
+          const float (&gk)[V] = g[k];
+          float act[V];
+          gates<V>(a.d.gate_activation, gk, act, slope);
+#pragma unroll
+          for (int i = 0; i < V; ++i) g[k][i] = act[i];
+        }
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          const float ga = a.gate ? gate_act(a.d.gate_activation, g[k][i]) : 1.f;
+          const float ga = a.gate ? g[k][i] : 1.f;
           const float u = LAYER ? fmaf(zz[k][i], sw[k][i], sb[k][i]) : zz[k][i] * sw[k][i];
           y[k][i] = c + i < F && use ? fmaf(ga, u, y[k][i]) : 0.f;
         }
@@ -358,13 +388,17 @@ __global__ __launch_bounds__(threads_of<L>(), LAYER || GATED ? 3 : 4) void norm_
     if (!AHEAD) fetch(row);
     const bool live = nlive, use = nuse;
     const f32x4 st = nst;
-    // D: the gradient of y (dx); e: dh, then times w'; yh: y, then normalised; zh; g: the gate before its activation
-    float D[NV][V], e[NV][V], yh[NV][V], zh[NV][V], g[NV][V];
+    // D: the gradient of y (dx); e: dh, then times w'; yh: y, then normalised; zh; g: the gate's activation, its slope
+    float D[NV][V], e[NV][V], yh[NV][V], zh[NV][V], g[NV][V], slope[NV][V];
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       unpack8(nx[k], yh[k]);
       unpack8(nz[k], zh[k]);
-      unpack8(ng[k], g[k]);
+      if (GATED) {
+        float before[V];
+        unpack8(ng[k], before);
+        gates<V>(a.d.gate_activation, before, g[k], slope[k]);
+      }
       unpack8(ny[k], D[k]);
       unpack8(nh[k], e[k]);
     }
@@ -380,7 +414,7 @@ __global__ __launch_bounds__(threads_of<L>(), LAYER || GATED ? 3 : 4) void norm_
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           zh[k][i] = c + i < F && use ? (LAYER ? zh[k][i] - st.x : zh[k][i]) * st.y : 0.f;   // (no post norm: mean 0, deviation 1)
-          const float ga = GATED ? gate_act(a.d.gate_activation, g[k][i]) : 1.f;
+          const float ga = GATED ? g[k][i] : 1.f;
           const float sw = s[i] * w[i], u = LAYER ? fmaf(zh[k][i], sw, s[i] * b[i]) : zh[k][i] * sw;
           yh[k][i] = fmaf(ga, u, yh[k][i]);
         }
@@ -428,12 +462,12 @@ __global__ __launch_bounds__(threads_of<L>(), LAYER || GATED ? 3 : 4) void norm_
         if (LAYER) load_param(a.b, c, F, 0.f, b);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          const float ga = GATED ? gate_act(a.d.gate_activation, g[k][i]) : 1.f;
+          const float ga = GATED ? g[k][i] : 1.f;
           const float Dq = per_graph ? D[k][i] : D[k][i] * ga;
           q1[k][i] = fmaf(Dq, zh[k][i], q1[k][i]);
           if (LAYER) q2[k][i] += Dq;
           const float u = LAYER ? fmaf(zh[k][i], w[i], b[i]) : zh[k][i] * w[i];
-          dg[i] = GATED ? D[k][i] * s[i] * u * gate_slope(a.d.gate_activation, g[k][i]) : 0.f;
+          dg[i] = GATED ? D[k][i] * s[i] * u * slope[k][i] : 0.f;
           D[k][i] *= s[i] * ga * w[i];                                 // gradient of zh
           m[0] = fmaf(D[k][i], zh[k][i], m[0]);
           if (LAYER) m[1] += D[k][i];
@@ -562,7 +596,9 @@ __global__ __launch_bounds__(64) void norm_graph_gate_kernel(NormArgs a) {
   const bool bf = a.d.z_dtype == AGCN_DTYPE_BF16;
   const int64_t at = (int64_t)g * a.d.ldg + c;
   const float gv = bf ? __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(a.gate)[at] << 16) : static_cast<const float*>(a.gate)[at];
-  const float ga = gate_act(a.d.gate_activation, gv), da = gate_slope(a.d.gate_activation, gv);
+  float one[1] = {gv}, act[1], slope[1];
+  gates<1>(a.d.gate_activation, one, act, slope);
+  const float ga = act[0], da = slope[0];
   const float sc = a.scale ? a.scale[c] : 1.f, w = a.w ? a.w[c] : 1.f, b = a.b ? a.b[c] : 0.f;
   const float o = da * sc * fmaf(w, q[0], b * q[1]);
   if (bf) reinterpret_cast<uint16_t*>(a.dgate)[(int64_t)g * F + c] = (uint16_t)pk_bf(o, 0.f);

@@ -31,6 +31,7 @@
 #include <algorithm>
 
 #include "bf16_split.h"
+#include "gate_math.h"
 #include "sgc_kernels.h"
 
 namespace agcn {
@@ -72,10 +73,9 @@ __device__ __forceinline__ uint32_t pk_bf(float a, float b) {
   return __builtin_bit_cast(uint32_t, (bf16x2){(__bf16)a, (__bf16)b});
 }
 
-// act(g) and act'(g).  The slopes are formed from e^-|g| (no 1 - s where s is near 1).  F32: within a few 2^-24: the exponent's product
-// with log2 e is carried in two parts, the reciprocal gets one Newton step (silu and sigmoid; with gates() below 115 -> 93 us for a
-// 32768 x 128 x 512 forward that called the library and branched for every value).  bf16 calls, whose results are rounded to eight
-// bits: the hardware's exp2 and reciprocal as they are (a few 2^-24, and |g| 2^-23 from the exponent's rounding), and for the normal
+// act(g) and act'(g).  The slopes are formed from e^-|g| (no 1 - s where s is near 1).  F32: within a few 2^-24 (gate_math.h; with
+// gates() below 115 -> 93 us for a 32768 x 128 x 512 forward that called the library and branched for every value).  bf16 calls,
+// whose results are rounded to eight bits: the hardware's exp2 and reciprocal as they are (a few 2^-24, and |g| 2^-23 from the exponent's rounding), and for the normal
 // distribution function the five-term fit of Abramowitz and Stegun, 7.1.26 (1.4e-7; relative to the tail 3e-5 at g = -2.8,
 // beyond which the library function takes over).
 template <int ACT, bool F32>
@@ -99,12 +99,8 @@ __device__ __forceinline__ void gate(float g, float& a, float& da) {
   } else {
     float e, d;
     if constexpr (F32) {
-      const float x = fabsf(g) > 128.f ? -128.f : -fabsf(g);            // (a NaN stays; e^-128 is below every normal number)
-      const float hi = x * 1.44269504f, lo = fmaf(x, 1.925963033e-8f, fmaf(x, 1.44269504f, -hi));
-      e = __builtin_amdgcn_exp2f(hi);
-      e = fmaf(e, lo * 0.69314718f, e);
-      d = __builtin_amdgcn_rcpf(1.f + e);
-      d = fmaf(d, fmaf(-(1.f + e), d, 1.f), d);
+      e = exp_neg(fabsf(g));
+      d = recip_1p(e);
     } else {
       e = __builtin_amdgcn_exp2f(-1.44269504f * fabsf(g));
       d = __builtin_amdgcn_rcpf(1.f + e);
