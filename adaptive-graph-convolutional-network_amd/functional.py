@@ -45,6 +45,7 @@ def _f32c(t, what):
 
 
 _DT = {torch.float32: 0, torch.bfloat16: 1}
+_TYPES = {i: t for t, i in _DT.items()}
 
 
 class CastRowsFunction(torch.autograd.Function):
@@ -794,6 +795,18 @@ def _on_device_of(t, fn, *args):
         return fn(*args)
 
 
+def _saved(t, what, shape, dtype, index):
+    """A saved tensor for a backward on GPU `index`.  Saved-tensor hooks (save_on_cpu, a pack hook that clones) give back the
+    values, not the layout: sizes, type and device are held against the forward's, and leading dimensions are taken from the
+    tensor that is returned here."""
+    if t.shape != shape or t.dtype is not dtype or t.get_device() != index:
+        raise ValueError("%s: saved as %s %s on GPU %d, but came back as %s %s on %s" %
+                         (what, tuple(shape), dtype, index, tuple(t.shape), t.dtype, t.device))
+    if t.is_contiguous() or (t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= shape[1]):
+        return t
+    return t.contiguous()
+
+
 def _norm_forward(z, x, gate, scale, post_weight, post_bias, pre_weight, pre_bias, plan, norm, eps, gate_activation, keep):
     """-> (y, h, what a backward needs: the tensors as the kernel read them, its row statistics, the descriptor)"""
     x = _row_matrix(x, "residual rows")
@@ -888,13 +901,24 @@ class NormGateResidualFunction(torch.autograd.Function):
         if dy is None and dh is None:
             return (None,) * 12
         saved = ctx.saved_tensors
-        return _on_device_of(saved[-1], NormGateResidualFunction._backward, ctx.desc, ctx.plan, saved, dy, dh) + (None,) * 4
+        return _on_device_of(dh if dy is None else dy, NormGateResidualFunction._backward, ctx.desc, ctx.plan, saved, dy, dh) + (None,) * 4
 
     @staticmethod
     def _backward(desc, plan, saved, dy, dh):
         lib = _ffi.lib()
         z, x, gate, scale, post_weight, post_bias, pre_weight, pre_bias, stats = saved
-        dev, rows, F = stats.device, desc.rows, desc.F
+        rows, F = desc.rows, desc.F
+        dev = (dh if dy is None else dy).device
+        at, xt, zt = (dh if dy is None else dy).get_device(), _TYPES[desc.x_dtype], _TYPES[desc.z_dtype]
+        x = _saved(x, "residual rows", (rows, F), xt, at)
+        z = None if z is None else _saved(z, "block output", (rows, F), zt, at)
+        gate = None if gate is None else _saved(gate, "gate", (plan.B if desc.gate == 2 else rows, F), zt, at)
+        stats = _saved(stats, "row statistics", (rows, 4), torch.float32, at).contiguous()
+        scale, post_weight, post_bias, pre_weight, pre_bias = [
+            None if p is None else _saved(p, "a vector", (F,), torch.float32, at)
+            for p in (scale, post_weight, post_bias, pre_weight, pre_bias)]
+        desc = _ffi.NormDesc(rows, F, desc.norm, desc.gate, desc.gate_activation, desc.x_dtype, desc.z_dtype, _ld(x),
+                             0 if z is None else _ld(z), 0 if gate is None else _ld(gate), desc.eps)
         dy = None if dy is None else dy.contiguous()
         dh = None if dh is None else dh.contiguous()
         dx = torch.empty((rows, F), dtype=x.dtype, device=dev)

@@ -1,0 +1,147 @@
+"""What autograd may do with the calls of norm_gate_residual and gated_ffn between forward and backward: saved tensors that
+come back at other addresses and in other layouts.  The CPU tests put a recorder in the library's place: it holds every pointer that a call hands over
+against the tensor that lies there."""
+import ctypes as C
+
+import pytest
+import torch
+
+f32, bf16 = torch.float32, torch.bfloat16
+
+
+@pytest.fixture(scope="module")
+def amd():
+    import agcn_amd
+    if agcn_amd._build.is_stale():
+        agcn_amd._build.build()
+    return agcn_amd
+
+
+class Recorder(object):
+    """Answers every entry with success and keeps the arguments; size queries ask the library itself (they need no GPU)."""
+
+    def __init__(self, lib):
+        self.lib, self.calls = lib, {}
+
+    def __getattr__(self, name):
+        if name.endswith("_bytes") or name == "agcn_last_error":
+            return getattr(self.lib, name)
+
+        def entry(*args):
+            self.calls.setdefault(name, []).append([getattr(a, "_obj", a) for a in args])
+            return 0
+        return entry
+
+
+@pytest.fixture
+def recorder(amd, monkeypatch):
+    rec = Recorder(amd._ffi.lib())
+    f = amd.functional
+    monkeypatch.setattr(amd._ffi, "lib", lambda: rec)
+    monkeypatch.setattr(f, "_require_gpu", lambda t, what: None)
+    monkeypatch.setattr(f, "_stream", lambda dev: 0)
+    monkeypatch.setattr(f, "_on_device_of", lambda t, fn, *args: fn(*args))
+    return rec
+
+
+class Hook(object):
+    """A pack / unpack pair; `back` makes what a saved tensor comes back as, and `seen` keeps it, by address."""
+
+    def __init__(self, back):
+        self.back, self.seen = back, {}
+
+    def unpack(self, t):
+        t = self.back(t)
+        self.seen[t.data_ptr()] = t
+        return t
+
+    def __enter__(self):
+        self.ctx = torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach(), self.unpack)
+        self.ctx.__enter__()
+        return self
+
+    def __exit__(self, *exc):
+        self.ctx.__exit__(*exc)
+
+
+def odd(t):
+    """the same values, one element behind an allocation's start"""
+    flat = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)
+    return flat[1:].view(t.shape).copy_(t)
+
+
+def wider(t):
+    """the same values with more room between the rows"""
+    return t.new_empty(t.shape[0], t.shape[1] + 24)[:, :t.shape[1]].copy_(t) if t.dim() == 2 else t.clone()
+
+
+def turned(t):
+    """the same values, columns first"""
+    return t.t().contiguous().t() if t.dim() == 2 else t.clone()
+
+
+def dense(t):
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+BACK = {"dense": dense, "odd": odd, "wider": wider, "turned": turned}
+
+
+def cut(rows, cols, dtype, seed, device="cpu", at=64):
+    """columns of a wider matrix"""
+    g = torch.Generator().manual_seed(seed)
+    return torch.randn(rows, 2 * at + cols, generator=g).to(device=device, dtype=dtype)[:, at:at + cols]
+
+
+@pytest.mark.parametrize("back", sorted(BACK))
+@pytest.mark.parametrize("xt,zt", [(f32, f32), (f32, bf16), (bf16, bf16)])
+def test_norm_backward_reads_saved_tensors_as_they_come_back(amd, recorder, back, xt, zt):
+    rows, F = 7, 64
+    t = {"z": cut(rows, F, zt, 1), "x": cut(rows, F, xt, 2), "gate": cut(rows, F, zt, 3)}
+    v = {k: torch.ones(F) for k in ("scale", "post_weight", "pre_weight")}
+    leaves = [a.requires_grad_(True) for a in list(t.values()) + list(v.values())]
+    with Hook(BACK[back]) as hook:
+        y, h = amd.norm_gate_residual(**t, **v)
+        torch.autograd.grad((y, h), leaves, (torch.ones_like(y), torch.ones_like(h)))
+    (desc, _, _, inputs, stats, _, _, _, _, _, _), = recorder.calls["agcn_norm_gate_residual_backward"]
+    for name, ld, dt in (("x", desc.ldx, xt), ("z", desc.ldz, zt), ("gate", desc.ldg, zt)):
+        p = getattr(inputs, name)
+        if p in hook.seen:                                   # read as it came back: with ITS leading dimension
+            s = hook.seen[p]
+            assert s.dtype is dt and s.stride() == (ld, 1), name
+        else:                                                # or a copy of it
+            assert ld == F, name
+    forward = recorder.calls["agcn_norm_gate_residual_forward"][0][0]
+    assert (forward.ldx, forward.ldz, forward.ldg) == (F + 128,) * 3
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("back", sorted(BACK) + ["save_on_cpu"])
+@pytest.mark.parametrize("xt,zt", [(f32, f32), (f32, bf16), (bf16, bf16)])
+@pytest.mark.parametrize("gate", ["row", "graph"])
+def test_norm_gradients_under_saved_tensor_hooks(amd, gate, back, xt, zt):
+    ns, F = [18, 5, 48, 1], 64
+    plan = amd.Plan(ns, device="cuda") if gate == "graph" else None
+    rows = sum(ns)
+    t = {"z": cut(rows, F, zt, 1, "cuda"), "x": cut(rows, F, xt, 2, "cuda"), "gate": cut(len(ns) if plan else rows, F, zt, 3, "cuda")}
+    v = {k: 1 + 0.1 * cut(1, F, f32, 4 + i, "cuda")[0] for i, k in enumerate(("scale", "post_weight", "post_bias", "pre_weight", "pre_bias"))}
+    leaves = [a.requires_grad_(True) for a in list(t.values()) + list(v.values())]
+
+    def grads():
+        y, h = amd.norm_gate_residual(**t, **v, norm="layer", gate_activation="tanh", plan=plan)
+        return torch.autograd.grad((y, h), leaves, (cut(rows, F, xt, 8, "cuda"), cut(rows, F, zt, 9, "cuda")))
+    want = grads()
+    with torch.autograd.graph.save_on_cpu() if back == "save_on_cpu" else Hook(BACK[back]):
+        got = grads()
+    for a, b in zip(want, got):
+        assert torch.equal(a, b)
+
+
+def test_norm_refuses_a_saved_tensor_that_is_another(amd, recorder):
+    for back in (lambda t: t[:1], lambda t: t.double()):
+        x = cut(5, 16, f32, 1).requires_grad_(True)
+        with Hook(back):
+            y, h = amd.norm_gate_residual(cut(5, 16, f32, 2), x, pre_weight=torch.ones(16))
+            with pytest.raises((TypeError, ValueError), match="saved"):
+                (y.sum() + h.sum()).backward()
+    assert "agcn_norm_gate_residual_backward" not in recorder.calls
