@@ -997,6 +997,14 @@ def _ffn_forward(X, Wg, Wu, Wd, activation, keep):
     return Y, (X, Wg, Wu, Wd, reserve), desc
 
 
+def _read_again(t, was):
+    """Where the forward could read a bf16 matrix in place it left no aligned copy of it.  One that has moved since (saved-tensor
+    hooks) and whose rows no longer start at 16 bytes is copied to where they do."""
+    if t.dtype is torch.bfloat16 and (t.data_ptr(), _ld(t)) != was and (t.data_ptr() & 15 or _ld(t) & 7):
+        return t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
 class GatedFfnFunction(torch.autograd.Function):
     """Y = (act(X Wg) * (X Wu)) Wd; see gated_ffn."""
 
@@ -1004,18 +1012,28 @@ class GatedFfnFunction(torch.autograd.Function):
     def forward(ctx, X, Wg, Wu, Wd, activation):
         Y, saved, ctx.desc = _on_device_of(X, _ffn_forward, X, Wg, Wu, Wd, activation, True)
         ctx.save_for_backward(*saved)
+        ctx.read_at = [(t.data_ptr(), _ld(t)) for t in saved[:4]]
         return Y
 
     @staticmethod
     @_first_order
     def backward(ctx, dY):
-        return _on_device_of(dY, GatedFfnFunction._backward, ctx.desc, ctx.saved_tensors, dY, ctx.needs_input_grad)
+        return _on_device_of(dY, GatedFfnFunction._backward, ctx.desc, ctx.saved_tensors, ctx.read_at, dY, ctx.needs_input_grad)
 
     @staticmethod
-    def _backward(desc, saved, dY, need):
+    def _backward(desc, saved, read_at, dY, need):
         lib = _ffi.lib()
-        X, Wg, Wu, Wd, reserve = saved
-        dev = X.device
+        dev, at, dtype = dY.device, dY.get_device(), _TYPES[desc.dtype]
+        sizes = (("node features", (desc.rows, desc.Fin)), ("w_gate", (desc.Fin, desc.H)), ("w_up", (desc.Fin, desc.H)),
+                 ("w_down", (desc.H, desc.Fout)))
+        X, Wg, Wu, Wd = [_read_again(_saved(t, what, shape, dtype, at), was) for t, (what, shape), was in zip(saved, sizes, read_at)]
+        Wg, Wu, Wd = Wg.contiguous(), Wu.contiguous(), Wd.contiguous()
+        reserve = saved[4]
+        if reserve.get_device() != at:
+            raise ValueError("what the forward kept came back on %s" % reserve.device)
+        if not reserve.is_contiguous() or reserve.data_ptr() & 255:
+            reserve = reserve.clone(memory_format=torch.contiguous_format)
+        desc = _ffi.FfnDesc(desc.rows, desc.Fin, desc.H, desc.Fout, desc.activation, desc.dtype, _ld(X), desc.training, 0)
         dY = dY.contiguous()
         dX = torch.empty((desc.rows, desc.Fin), dtype=X.dtype, device=dev) if need[0] else None
         dWg, dWu = (torch.empty_like(Wg), torch.empty_like(Wu)) if need[1] or need[2] else (None, None)

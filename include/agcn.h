@@ -420,7 +420,9 @@ AGCN_API int agcn_cast_rows(const void* src, int32_t src_dtype, void* dst, int32
  * holds an infinity or a NaN comes out non-finite, but an infinity may come out as NaN); bf16 calls round the block's inner
  * matrices to bf16 (small calls keep a second piece), sums are fp32.  The kernels are chosen by the sizes, the type and `training`:
  * a row's result may differ in its last bits with the number of rows beside it, and between training = 0 and 1.  reserve (256-byte aligned, agcn_gated_ffn_reserve_bytes): scratch of the forward; with
- * training = 1 the backward needs it as the forward left it, and X, Wg, Wu, Wd unchanged at the same addresses.
+ * training = 1 the backward needs it as the forward left it, and X, Wg, Wu, Wd with the same values: at the same addresses with the
+ * same ldx, or elsewhere if each bf16 matrix whose columns are a multiple of eight then starts at 16 bytes and has a leading
+ * dimension that is one too (of the other bf16 matrices, and of large fp32 ones, the forward leaves a copy in the reserve).
  * Backward: dX [rows, Fin], dWg, dWu (together), dWd are each nullable. Fixed-order sums: bit-reproducible.
  * rows = 0: the forward does nothing, the backward writes zeros. */
 typedef struct AgcnFfnDesc {

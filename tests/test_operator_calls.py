@@ -145,3 +145,74 @@ def test_norm_refuses_a_saved_tensor_that_is_another(amd, recorder):
             with pytest.raises((TypeError, ValueError), match="saved"):
                 (y.sum() + h.sum()).backward()
     assert "agcn_norm_gate_residual_backward" not in recorder.calls
+
+
+@pytest.mark.parametrize("back", sorted(BACK))
+@pytest.mark.parametrize("dtype", [f32, bf16])
+def test_ffn_backward_reads_saved_tensors_as_they_come_back(amd, recorder, back, dtype):
+    """Features of whole 16-byte chunks: the forward reads such bf16 matrices in place, so the backward must find them so."""
+    rows, F, H, O = 50, 64, 96, 72
+    ts = [cut(rows, F, dtype, 1)] + [cut(a, b, dtype, 2 + i, at=0) for i, (a, b) in enumerate(((F, H), (F, H), (H, O)))]
+    ts = [t.requires_grad_(True) for t in ts]
+    with Hook(BACK[back]) as hook:
+        Y = amd.gated_ffn(*ts)
+        torch.autograd.grad(Y, ts, torch.ones_like(Y))
+    (desc, X, Wg, Wu, Wd, *_), = recorder.calls["agcn_gated_ffn_backward"]
+    (forward, *_), = recorder.calls["agcn_gated_ffn_forward"]
+    assert forward.ldx == F + 128
+    for name, p, cols, ld in (("X", X, F, desc.ldx), ("Wg", Wg, H, H), ("Wu", Wu, H, H), ("Wd", Wd, O, O)):
+        if p in hook.seen:
+            assert hook.seen[p].stride() == (ld, 1), name
+        else:
+            assert ld == cols, name
+        assert dtype == f32 or (p % 16 == 0 and ld % 8 == 0), name
+
+
+@pytest.mark.parametrize("back", [lambda t: t[:1], lambda t: t.double()])
+def test_ffn_refuses_a_saved_tensor_that_is_another(amd, recorder, back):
+    X = cut(5, 16, f32, 1).requires_grad_(True)
+    with Hook(back):
+        Y = amd.gated_ffn(X, torch.ones(16, 8), torch.ones(16, 8), torch.ones(8, 4))
+        with pytest.raises(ValueError, match="saved"):
+            Y.sum().backward()
+    assert "agcn_gated_ffn_backward" not in recorder.calls
+
+
+# (rows, H): few rows; A in two pieces; one piece / planes of fp32 pieces.  72: whole chunks of 16 bytes, 75: an image in the forward
+@pytest.mark.gpu
+@pytest.mark.parametrize("back", sorted(BACK) + ["save_on_cpu"])
+@pytest.mark.parametrize("dtype", [f32, bf16])
+@pytest.mark.parametrize("size", [(3, 72, 96, 40), (50, 72, 96, 40), (50, 75, 96, 41), (700, 200, 3000, 160), (700, 203, 3001, 161)])
+def test_ffn_gradients_under_saved_tensor_hooks(amd, size, back, dtype):
+    rows, F, H, O = size
+    ts = [cut(rows, F, dtype, 1, "cuda")] + [cut(a, b, dtype, 2 + i, "cuda", 0) / a ** 0.5 for i, (a, b) in enumerate(((F, H), (F, H), (H, O)))]
+    ts = [t.requires_grad_(True) for t in ts]
+    dY = cut(rows, O, dtype, 7, "cuda", 0)
+    want = torch.autograd.grad(amd.gated_ffn(*ts), ts, dY)
+    with torch.autograd.graph.save_on_cpu() if back == "save_on_cpu" else Hook(BACK[back]):
+        got = torch.autograd.grad(amd.gated_ffn(*ts), ts, dY)
+    for a, b in zip(want, got):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_ffn_gradients_when_some_weights_move(amd):
+    """Both projections are read in place or neither is: one that comes back at an odd address beside one that stayed, and an odd
+    one that comes back aligned."""
+    rows, F, H, O = 300, 72, 96, 40
+    X, dY = cut(rows, F, bf16, 1, "cuda"), cut(rows, O, bf16, 7, "cuda", 0)
+    W = [cut(a, b, bf16, 2 + i, "cuda", 0) / a ** 0.5 for i, (a, b) in enumerate(((F, H), (F, H), (H, O)))]
+    for start in (0, 1, 2, 4, 7):
+        ts = [X] + [odd(w) if start >> i & 1 else w for i, w in enumerate(W)]
+        ts = [t.detach().requires_grad_(True) for t in ts]
+        want = torch.autograd.grad(amd.gated_ffn(*ts), ts, dY)
+        for moved in range(8):
+            turn = iter(range(-1, 8))
+
+            def back(t):
+                i = next(turn)                               # saved in the order X, w_gate, w_up, w_down, reserve
+                return t if not 0 <= i < 3 or not moved >> i & 1 else (dense(t) if t.data_ptr() & 15 else odd(t))
+            with Hook(back):
+                got = torch.autograd.grad(amd.gated_ffn(*ts), ts, dY)
+            for a, b in zip(want, got):
+                assert torch.equal(a, b), (start, moved)
