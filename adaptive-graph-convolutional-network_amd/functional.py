@@ -6,6 +6,7 @@ import functools
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _ffi
 
@@ -782,7 +783,14 @@ def _vector(t, what, F, like):
     return t
 
 
+def _no_tangents(tensors):
+    """Refuses tensors that carry a forward-mode tangent: the kernels would drop it, which reads as a derivative of zero."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise _ffi.AgcnError("this operator has no forward-mode derivative")
+
+
 def _wants_grad(tensors):
+    _no_tangents(tensors)
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
@@ -874,6 +882,7 @@ class _NoSecondDerivative(torch.autograd.Function):
 def _first_order(backward):
     @functools.wraps(backward)
     def run(ctx, *grads):
+        _no_tangents(grads)
         if not torch.is_grad_enabled():                       # the usual case: no graph of the backward pass is wanted
             return backward(ctx, *grads)
         with torch.no_grad():

@@ -216,3 +216,51 @@ def test_ffn_gradients_when_some_weights_move(amd):
                 got = torch.autograd.grad(amd.gated_ffn(*ts), ts, dY)
             for a, b in zip(want, got):
                 assert torch.equal(a, b), (start, moved)
+
+
+def _operators(amd):
+    """name -> (call of a list of tensors, the tensors)"""
+    vec = torch.ones(8)
+    return {"norm": (lambda ts: amd.norm_gate_residual(ts[0], ts[1], gate=ts[2], post_weight=ts[3], pre_weight=vec),
+                     [cut(4, 8, f32, i) for i in range(3)] + [torch.ones(8)]),
+            "ffn": (lambda ts: amd.gated_ffn(*ts), [cut(4, 8, f32, 1), torch.ones(8, 6), torch.ones(8, 6), torch.ones(6, 3)])}
+
+
+@pytest.mark.parametrize("op", ["norm", "ffn"])
+@pytest.mark.parametrize("which", range(4))
+@pytest.mark.parametrize("mode", ["plain", "no_grad", "requires_grad", "jvp"])
+def test_forward_mode_is_refused(amd, recorder, op, which, mode):
+    """A tangent has no way through the kernels: dropped in silence it would be a derivative of zero."""
+    call, ts = _operators(amd)[op]
+    with pytest.raises(amd.AgcnError, match="forward-mode"):
+        if mode == "jvp":
+            torch.func.jvp(lambda t: call(ts[:which] + [t] + ts[which + 1:]), (ts[which],), (torch.ones_like(ts[which]),))
+        else:
+            with torch.autograd.forward_ad.dual_level(), torch.set_grad_enabled(mode != "no_grad"):
+                if mode == "requires_grad":
+                    ts = [t.requires_grad_(True) for t in ts]
+                ts[which] = torch.autograd.forward_ad.make_dual(ts[which], torch.ones_like(ts[which]))
+                call(ts)
+    assert not recorder.calls
+
+
+@pytest.mark.parametrize("op", ["norm", "ffn"])
+def test_calls_without_a_tangent_run_in_a_forward_mode_level(amd, recorder, op):
+    call, ts = _operators(amd)[op]
+    with torch.autograd.forward_ad.dual_level():
+        call(ts)
+    assert len(recorder.calls) == 1
+
+
+@pytest.mark.parametrize("op", ["norm", "ffn"])
+@pytest.mark.parametrize("create_graph", [False, True])
+def test_a_tangent_of_the_upstream_gradient_is_refused(amd, recorder, op, create_graph):
+    call, ts = _operators(amd)[op]
+    ts = [t.requires_grad_(True) for t in ts]
+    out = call(ts)
+    out = out[0] if isinstance(out, tuple) else out
+    with torch.autograd.forward_ad.dual_level():
+        up = torch.autograd.forward_ad.make_dual(torch.ones_like(out), torch.ones_like(out))
+        with pytest.raises(amd.AgcnError, match="forward-mode"):
+            torch.autograd.grad(out, ts, up, create_graph=create_graph)
+    assert len(recorder.calls) == 1
