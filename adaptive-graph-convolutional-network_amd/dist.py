@@ -15,6 +15,7 @@ import torch
 import torch.distributed as dist
 
 from . import _ffi
+from .functional import _no_tangents
 
 
 def graph_cost(n, Fin, Fout, K):
@@ -95,6 +96,13 @@ def _each(method, ts):
     return list(map(method, ts))
 
 
+def _no_graph(ts):
+    """Clipping has no derivative: a loss built on its results would lose these tensors' part in silence."""
+    if torch.is_grad_enabled() and True in map(_T.requires_grad.__get__, ts):
+        raise _ffi.AgcnError("the results of clipping carry no graph, but a tensor requires grad: call it under torch.no_grad()")
+    _no_tangents(ts)
+
+
 def _clip(ts, clip_norm, out):
     """(lists of a hundred tensors and more: every step below is one pass in C over the list)"""
     lib = _ffi.lib()
@@ -127,10 +135,12 @@ def _clip(ts, clip_norm, out):
 
 def global_norm(tensors):
     """sqrt of the sum of squares over every element of every tensor (float32 or bfloat16, one device; None entries are
-    skipped): a 0-dim device tensor, no synchronisation."""
+    skipped): a 0-dim device tensor, no synchronisation.  It has no derivative: tensors that require grad are refused outside
+    torch.no_grad()."""
     ts = [t.contiguous() for t in tensors if t is not None]
     if not ts:
         raise ValueError("no tensors")
+    _no_graph(ts)
     return _clip(ts, 1.0, None)
 
 
@@ -138,7 +148,8 @@ def clip_by_global_norm(tensors, clip_norm, out=None):
     """Scales a list of gradient tensors (float32 or bfloat16, one device) so that their global norm is at most `clip_norm`:
     out_t = t * clip_norm / max(norm, clip_norm).  Returns (list of clipped tensors, norm before clipping as a 0-dim device tensor);
     nothing synchronises.  None entries stay None.  A norm that is not finite makes every result NaN (the reference's framework
-    does the same: a broken step is seen, not applied).  out: contiguous tensors of the same sizes and types to write to;
+    does the same: a broken step is seen, not applied).  The results carry no graph: tensors that require grad are refused outside
+    torch.no_grad().  out: contiguous tensors of the same sizes and types to write to;
     `out=tensors` clips in place."""
     clip_norm = float(clip_norm)
     if not clip_norm > 0.0:
@@ -152,17 +163,20 @@ def clip_by_global_norm(tensors, clip_norm, out=None):
         raise ValueError("no tensors")
     whole = len(at) == len(tensors)
     ts = tensors if whole else [tensors[i] for i in at]
+    _no_graph(ts)
     if not all(map(_T.is_contiguous, ts)):
         ts = [t.contiguous() for t in ts]
     if out is None:
-        os_ = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in ts]
+        os_ = [torch.empty_like(t) for t in ts]
     else:
         os_ = out if whole else [out[i] for i in at]
         if any(o is None for o in os_):
             raise ValueError("out must hold a tensor for every gradient")
-        if (not all(map(_T.is_contiguous, os_)) or _each(_T.numel, os_) != _each(_T.numel, ts) or
-                [o.dtype for o in os_] != [t.dtype for t in ts] or _each(_T.get_device, os_) != _each(_T.get_device, ts)):
-            raise ValueError("out must hold contiguous tensors of the gradients' sizes, types and device")
+        if os_ is not ts:                                  # (in place: the tensors that were looked at above)
+            _no_graph(os_)
+            if (not all(map(_T.is_contiguous, os_)) or _each(_T.numel, os_) != _each(_T.numel, ts) or
+                    [o.dtype for o in os_] != [t.dtype for t in ts] or _each(_T.get_device, os_) != _each(_T.get_device, ts)):
+                raise ValueError("out must hold contiguous tensors of the gradients' sizes, types and device")
     norm = _clip(ts, clip_norm, os_)
     if out is None:
         if whole:

@@ -211,3 +211,41 @@ def test_refusals_of_tensors(amd):
         amd.clip_by_global_norm([a, a], 1.0, out=[a, a])
     with pytest.raises(ValueError):
         amd.clip_by_global_norm([a, torch.ones(3)], 1.0)
+
+
+def _calls(amd, ts, out):
+    yield lambda: amd.global_norm(ts)
+    yield lambda: amd.clip_by_global_norm(ts, 1.0)
+    yield lambda: amd.clip_by_global_norm(ts, 1.0, out=ts)
+    yield lambda: amd.clip_by_global_norm(ts, 1.0, out=out)
+
+
+def test_a_derivative_is_refused_not_lost(amd):
+    """Gradients that are themselves differentiable (create_graph=True), parameters, tangents: the results would carry no graph."""
+    a, b = torch.ones(4, requires_grad=True), torch.ones(4)
+    (g,) = torch.autograd.grad((a ** 3).sum(), [a], create_graph=True)
+    for first, ts, out in ((0, [b, g], [b, b]), (0, [a], [b]), (0, [None, a], [None, b]), (3, [b], [a])):
+        for call in list(_calls(amd, ts, out))[first:]:     # (the last: its input asks for nothing, its output does)
+            with pytest.raises(amd.AgcnError, match="no_grad"):
+                call()
+            with torch.no_grad(), pytest.raises(amd.AgcnError, match="GPU"):
+                call()                                      # (as far as the device check)
+    with torch.autograd.forward_ad.dual_level(), torch.no_grad():
+        d = torch.autograd.forward_ad.make_dual(b, b)
+        for call in _calls(amd, [b, d], [b, b]):
+            with pytest.raises(amd.AgcnError, match="forward-mode"):
+                call()
+
+
+@pytest.mark.gpu
+def test_clip_of_differentiable_gradients_without_a_graph(amd):
+    p = torch.nn.Parameter(torch.randn(500, device="cuda"))
+    (p ** 3).sum().backward(create_graph=True)
+    keep = [p.grad.detach().clone()]
+    with pytest.raises(amd.AgcnError, match="no_grad"):
+        amd.clip_by_global_norm([p.grad], 0.5)
+    with torch.no_grad():
+        out, norm = amd.clip_by_global_norm([p.grad], 0.5)
+    check(keep, out, norm, 0.5)
+    assert not out[0].requires_grad and not norm.requires_grad
+    p.grad = None                                           # (its graph holds p: a cycle)
