@@ -1,6 +1,6 @@
 // Global norm of many gradient tensors, and clipping by it (no counterpart in the reference's step, which clips per
 // Laplacian only; the semantics are those of its framework's clip-by-global-norm):
-//     n = sqrt(sum_t sum_i x_ti^2),   out_ti = x_ti * c / max(n, c);   n not finite -> every output is NaN.
+//     n = sqrt(sum_t sum_i x_ti^2),   out_ti = x_ti * c / max(n, c);   n, in fp32, not finite -> every output is NaN.
 // Two passes over the data, bound by memory: 3 transfers per element (read, read, write), of which the second read comes from
 // the caches as far as they reach.  The tensors are cut into chunks; a workgroup sums one chunk in 64 bits (a square of any fp32
 // value is finite there: neither a large nor a tiny gradient changes the answer's accuracy) and leaves one partial sum.  The
@@ -129,7 +129,13 @@ __global__ __launch_bounds__(1024) void clip_total_kernel(double* part, int tota
   }
 }
 
-__device__ __forceinline__ u32x4a scaled(u32x4a v, bool bf, float k) {
+__device__ __forceinline__ float times(float x, double f) { return (float)((double)x * f); }
+__device__ __forceinline__ u32x4a scaled(u32x4a v, bool bf, float k, bool tiny, double f) {
+  if (tiny) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = bf ? pack_bf(times(bf_lo(v[i]), f), times(bf_hi(v[i]), f)) : __float_as_uint(times(__uint_as_float(v[i]), f));
+    return v;
+  }
 #pragma unroll
   for (int i = 0; i < 4; ++i) v[i] = bf ? pack_bf(bf_lo(v[i]) * k, bf_hi(v[i]) * k) : __float_as_uint(__uint_as_float(v[i]) * k);
   return v;
@@ -146,8 +152,13 @@ __global__ __launch_bounds__(256) void clip_scale_kernel(ClipArgs a) {
     s = a.part[a.total];
   }
   const double n = sqrt(s), c = (double)a.clip;
-  // (a NaN or infinite sum fails both comparisons)
-  const float k = n <= c && n < INFINITY ? 1.f : (n < INFINITY ? (float)(c / n) : NAN);
+  // Finite or not is asked of the norm as it is handed back, in fp32: a caller that skips a step by it and the results agree.  (A
+  // NaN or infinite sum fails both comparisons.)
+  const bool finite = (float)n < INFINITY;
+  const double f = finite ? (n <= c ? 1.0 : c / n) : NAN;
+  const float k = (float)f;
+  // a factor below fp32's normal numbers has lost digits: those products are taken in 64 bits
+  const bool tiny = f < (double)__FLT_MIN__;
   const void* in = a.t.in[t];
   void* out = a.t.out[t];
   if (k == 1.f && in == out) return;
@@ -165,17 +176,19 @@ __global__ __launch_bounds__(256) void clip_scale_kernel(ClipArgs a) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const u32x4a*>(p + ((int64_t)(i + 256 * j) << 4));
 #pragma unroll
-    for (int j = 0; j < 4; ++j) *reinterpret_cast<u32x4a*>(q + ((int64_t)(i + 256 * j) << 4)) = scaled(v[j], bf, k);
+    for (int j = 0; j < 4; ++j) *reinterpret_cast<u32x4a*>(q + ((int64_t)(i + 256 * j) << 4)) = scaled(v[j], bf, k, tiny, f);
   }
   for (; i < full; i += 256)
-    *reinterpret_cast<u32x4a*>(q + ((int64_t)i << 4)) = scaled(*reinterpret_cast<const u32x4a*>(p + ((int64_t)i << 4)), bf, k);
+    *reinterpret_cast<u32x4a*>(q + ((int64_t)i << 4)) = scaled(*reinterpret_cast<const u32x4a*>(p + ((int64_t)i << 4)), bf, k, tiny, f);
   const int rest0 = full << 4, esz = bf ? 2 : 4;
   if (rest0 + tid * esz < len) {
     if (bf) {
       const uint16_t x = reinterpret_cast<const uint16_t*>(p + rest0)[tid];
-      reinterpret_cast<uint16_t*>(q + rest0)[tid] = (uint16_t)pack_bf(__uint_as_float((uint32_t)x << 16) * k, 0.f);
+      const float v = __uint_as_float((uint32_t)x << 16);
+      reinterpret_cast<uint16_t*>(q + rest0)[tid] = (uint16_t)pack_bf(tiny ? times(v, f) : v * k, 0.f);
     } else {
-      reinterpret_cast<float*>(q + rest0)[tid] = reinterpret_cast<const float*>(p + rest0)[tid] * k;
+      const float v = reinterpret_cast<const float*>(p + rest0)[tid];
+      reinterpret_cast<float*>(q + rest0)[tid] = tiny ? times(v, f) : v * k;
     }
   }
 }

@@ -147,8 +147,8 @@ def global_norm(tensors):
 def clip_by_global_norm(tensors, clip_norm, out=None):
     """Scales a list of gradient tensors (float32 or bfloat16, one device) so that their global norm is at most `clip_norm`:
     out_t = t * clip_norm / max(norm, clip_norm).  Returns (list of clipped tensors, norm before clipping as a 0-dim device tensor);
-    nothing synchronises.  None entries stay None.  A norm that is not finite makes every result NaN (the reference's framework
-    does the same: a broken step is seen, not applied).  The results carry no graph: tensors that require grad are refused outside
+    nothing synchronises.  None entries stay None.  A norm that is not finite, or that float32 does not hold, makes every
+    result NaN (the reference's framework does the same: a broken step is seen, not applied).  The results carry no graph: tensors that require grad are refused outside
     torch.no_grad().  out: contiguous tensors of the same sizes and types to write to;
     `out=tensors` clips in place."""
     clip_norm = float(clip_norm)

@@ -484,7 +484,7 @@ AGCN_API int agcn_norm_gate_residual_backward(const AgcnNormDesc* desc, const vo
 
 /* ---- clipping by the global norm of many gradient tensors --------------------------------------------
  * norm[0] = sqrt(sum over all tensors of the squares), out[t] = in[t] * clip_norm / max(norm, clip_norm); a norm that is not
- * finite makes every output NaN (the semantics of the reference's framework).  in / out / numel / dtype: HOST tables of
+ * finite, or that fp32 does not hold, makes every output NaN (the semantics of the reference's framework).  in / out / numel / dtype: HOST tables of
  * n_tensors entries (device pointers, element counts, AGCN_DTYPE_*); out[t] == in[t] clips in place, any other overlap of an
  * output with an input or an output is refused; out == NULL: the norm alone.  Squares are added in 64 bits, in a fixed order.
  * norm: DEVICE float.  workspace: agcn_clip_workspace_bytes of the same table. */

@@ -249,3 +249,42 @@ def test_clip_of_differentiable_gradients_without_a_graph(amd):
     check(keep, out, norm, 0.5)
     assert not out[0].requires_grad and not norm.requires_grad
     p.grad = None                                           # (its graph holds p: a cycle)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,t", [(100, f32), (100, bf16), (3000001, f32), (3000001, bf16)])
+def test_a_norm_beyond_fp32_is_one_that_is_not_finite(amd, n, t):
+    """Finite gradients whose norm no fp32 holds: the norm that is handed back is infinite, and the results agree with it.  Just
+    below, both are numbers."""
+    big = torch.finfo(t).max
+    below = [torch.zeros(n, device="cuda", dtype=t), torch.zeros(4, device="cuda", dtype=t)]
+    below[0][n // 2] = big / 2                              # norm = the largest number of the type
+    below[1][:3] = big / 2
+    out, norm = amd.clip_by_global_norm(below, 1.0)
+    check(below, out, norm, 1.0)
+    assert bool(torch.isfinite(norm))
+    below[1][3] = big
+    out, norm = amd.clip_by_global_norm(below, 1.0)         # sqrt 2 of it
+    assert float(norm) == float("inf") and all(bool(torch.isnan(o).all()) for o in out)
+    assert float(amd.global_norm(below)) == float("inf")
+    res, norm = amd.clip_by_global_norm(below, float("inf"), out=below)
+    assert float(norm) == float("inf") and all(bool(torch.isnan(o).all()) for o in res)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [50, 3000001])
+@pytest.mark.parametrize("clip", [1.0, 2.0 ** -20, 2.0 ** -100])
+def test_a_factor_below_the_normal_numbers(amd, n, clip):
+    """clip / norm down to 2^-226 is no normal fp32 number, the results are: within the bounds of check() (and half a step of the
+    smallest numbers, 2^-150; of bf16, 2^-134)."""
+    g = torch.Generator().manual_seed(n)
+    ts = [(torch.randn(k, generator=g) * 2.0 ** 110).to(t).cuda() for k, t in ((n, f32), (77, bf16), (3, f32))]
+    ts[0][1], ts[0][n // 2], ts[1][5] = 2.0 ** 126, 0.0, 1.0
+    for dst in (None, [t.clone() for t in ts]):
+        out, norm = amd.clip_by_global_norm(ts, clip, out=dst)
+        n64 = norm64(ts)
+        assert abs(float(norm) - n64) <= 2 * E * n64
+        for t, o in zip(ts, out):
+            want = t.double().cpu() * (clip / n64)
+            bound = (2 * E + (B8 if t.dtype == bf16 else E)) * want.abs() + 2.0 ** -150 + (2.0 ** -134 if t.dtype == bf16 else 0.0)
+            assert bool(((o.double().cpu() - want).abs() <= bound).all())
