@@ -807,12 +807,12 @@ def _saved(t, what, shape, dtype, index):
     """A saved tensor for a backward on GPU `index`.  Saved-tensor hooks (save_on_cpu, a pack hook that clones) give back the
     values, not the layout: sizes, type and device are held against the forward's, and leading dimensions are taken from the
     tensor that is returned here."""
-    if t.shape != shape or t.dtype is not dtype or t.get_device() != index:
-        raise ValueError("%s: saved as %s %s on GPU %d, but came back as %s %s on %s" %
-                         (what, tuple(shape), dtype, index, tuple(t.shape), t.dtype, t.device))
-    if t.is_contiguous() or (t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= shape[1]):
-        return t
-    return t.contiguous()
+    if t.dtype is dtype and t.get_device() == index and t.shape == shape:
+        if t.is_contiguous() or (len(shape) == 2 and t.stride(1) == 1 and t.stride(0) >= shape[1]):
+            return t
+        return t.contiguous()
+    raise ValueError("%s: saved as %s %s on GPU %d, but came back as %s %s on %s" %
+                     (what, tuple(shape), dtype, index, tuple(t.shape), t.dtype, t.device))
 
 
 def _norm_forward(z, x, gate, scale, post_weight, post_bias, pre_weight, pre_bias, plan, norm, eps, gate_activation, keep):
@@ -918,30 +918,36 @@ class NormGateResidualFunction(torch.autograd.Function):
         z, x, gate, scale, post_weight, post_bias, pre_weight, pre_bias, stats = saved
         rows, F = desc.rows, desc.F
         dev = (dh if dy is None else dy).device
-        at, xt, zt = (dh if dy is None else dy).get_device(), _TYPES[desc.x_dtype], _TYPES[desc.z_dtype]
-        x = _saved(x, "residual rows", (rows, F), xt, at)
-        z = None if z is None else _saved(z, "block output", (rows, F), zt, at)
-        gate = None if gate is None else _saved(gate, "gate", (plan.B if desc.gate == 2 else rows, F), zt, at)
-        stats = _saved(stats, "row statistics", (rows, 4), torch.float32, at).contiguous()
-        scale, post_weight, post_bias, pre_weight, pre_bias = [
-            None if p is None else _saved(p, "a vector", (F,), torch.float32, at)
-            for p in (scale, post_weight, post_bias, pre_weight, pre_bias)]
-        desc = _ffi.NormDesc(rows, F, desc.norm, desc.gate, desc.gate_activation, desc.x_dtype, desc.z_dtype, _ld(x),
-                             0 if z is None else _ld(z), 0 if gate is None else _ld(gate), desc.eps)
+        at, xt, zt, shape = (dh if dy is None else dy).get_device(), _TYPES[desc.x_dtype], _TYPES[desc.z_dtype], (rows, F)
+        x = _saved(x, "residual rows", shape, xt, at)
+        ldx, ldz, ldg = _ld(x), 0, 0
+        if z is not None:
+            z = _saved(z, "block output", shape, zt, at)
+            ldz = _ld(z)
+        if gate is not None:
+            gate = _saved(gate, "gate", shape if desc.gate == 1 else (plan.B, F), zt, at)
+            ldg = _ld(gate)
+        f32, where = torch.float32, []
+        stats = _saved(stats, "row statistics", (rows, 4), f32, at).contiguous()
+        vectors = [scale, post_weight, post_bias, pre_weight, pre_bias]
+        for i, p in enumerate(vectors):
+            if p is not None and not (p.dtype is f32 and p.is_contiguous() and p.numel() == F and p.get_device() == at):
+                p = vectors[i] = _saved(p, "a vector", (F,), f32, at)
+            where.append(0 if p is None else p.data_ptr())
+        if (ldx, ldz, ldg) != (desc.ldx, desc.ldz, desc.ldg):
+            desc = _ffi.NormDesc(rows, F, desc.norm, desc.gate, desc.gate_activation, desc.x_dtype, desc.z_dtype, ldx, ldz, ldg, desc.eps)
         dy = None if dy is None else dy.contiguous()
         dh = None if dh is None else dh.contiguous()
         dx = torch.empty((rows, F), dtype=x.dtype, device=dev)
         dz = None if z is None else torch.empty((rows, F), dtype=z.dtype, device=dev)
         dgate = None if gate is None else torch.empty(gate.shape, dtype=gate.dtype, device=dev)
         # (the vectors' gradients: rows of one small matrix)
-        vectors = (scale, post_weight, post_bias, pre_weight, pre_bias)
         given = [i for i, p in enumerate(vectors) if p is not None]
         params = [None] * 5
         for i, g in zip(given, torch.empty((len(given), F), dtype=torch.float32, device=dev).unbind(0)):
             params[i] = g
-        inputs = _ffi.NormInputs(_rows_ptr(z), _rows_ptr(x), _rows_ptr(gate), _ptr(scale), _ptr(post_weight), _ptr(post_bias),
-                                 _ptr(pre_weight), _ptr(pre_bias))
-        grads = _ffi.NormGrads(_rows_ptr(dz), _rows_ptr(dx), _rows_ptr(dgate), *[_ptr(p) for p in params])
+        inputs = _ffi.NormInputs(_rows_ptr(z), _rows_ptr(x), _rows_ptr(gate), *where)
+        grads = _ffi.NormGrads(_rows_ptr(dz), _rows_ptr(dx), _rows_ptr(dgate), *[0 if p is None else p.data_ptr() for p in params])
         host, devp = (None, None) if plan is None else (plan.host_ptr, plan.dev_ptr)
         wbytes = lib.agcn_norm_gate_residual_backward_workspace_bytes(C.byref(desc), host)
         ws = torch.empty(wbytes, dtype=torch.uint8, device=dev)
@@ -1006,14 +1012,6 @@ def _ffn_forward(X, Wg, Wu, Wd, activation, keep):
     return Y, (X, Wg, Wu, Wd, reserve), desc
 
 
-def _read_again(t, was):
-    """Where the forward could read a bf16 matrix in place it left no aligned copy of it.  One that has moved since (saved-tensor
-    hooks) and whose rows no longer start at 16 bytes is copied to where they do."""
-    if t.dtype is torch.bfloat16 and (t.data_ptr(), _ld(t)) != was and (t.data_ptr() & 15 or _ld(t) & 7):
-        return t.clone(memory_format=torch.contiguous_format)
-    return t
-
-
 class GatedFfnFunction(torch.autograd.Function):
     """Y = (act(X Wg) * (X Wu)) Wd; see gated_ffn."""
 
@@ -1021,7 +1019,7 @@ class GatedFfnFunction(torch.autograd.Function):
     def forward(ctx, X, Wg, Wu, Wd, activation):
         Y, saved, ctx.desc = _on_device_of(X, _ffn_forward, X, Wg, Wu, Wd, activation, True)
         ctx.save_for_backward(*saved)
-        ctx.read_at = [(t.data_ptr(), _ld(t)) for t in saved[:4]]
+        ctx.read_at = [t.data_ptr() for t in saved[:4]] if Y.dtype is torch.bfloat16 else None
         return Y
 
     @staticmethod
@@ -1032,17 +1030,27 @@ class GatedFfnFunction(torch.autograd.Function):
     @staticmethod
     def _backward(desc, saved, read_at, dY, need):
         lib = _ffi.lib()
-        dev, at, dtype = dY.device, dY.get_device(), _TYPES[desc.dtype]
-        sizes = (("node features", (desc.rows, desc.Fin)), ("w_gate", (desc.Fin, desc.H)), ("w_up", (desc.Fin, desc.H)),
-                 ("w_down", (desc.H, desc.Fout)))
-        X, Wg, Wu, Wd = [_read_again(_saved(t, what, shape, dtype, at), was) for t, (what, shape), was in zip(saved, sizes, read_at)]
-        Wg, Wu, Wd = Wg.contiguous(), Wu.contiguous(), Wd.contiguous()
-        reserve = saved[4]
+        X, Wg, Wu, Wd, reserve = saved
+        dev, dtype, rows, Fin, H, Fout = dY.device, dY.dtype, desc.rows, desc.Fin, desc.H, desc.Fout
+        at = dY.get_device()
+        X = _saved(X, "node features", (rows, Fin), dtype, at)
+        Wg, Wu = _saved(Wg, "w_gate", (Fin, H), dtype, at).contiguous(), _saved(Wu, "w_up", (Fin, H), dtype, at).contiguous()
+        Wd = _saved(Wd, "w_down", (H, Fout), dtype, at).contiguous()
+        ldx = _ld(X)
+        if read_at is not None:
+            # Where the forward could read a bf16 matrix in place it left no aligned copy of it.  One that has moved since and
+            # whose rows do not start at 16 bytes is copied to where they do.
+            now = [(X.data_ptr() | 2 * ldx) & 15, Wg.data_ptr() & 15, Wu.data_ptr() & 15, Wd.data_ptr() & 15]
+            if any(now):
+                X, Wg, Wu, Wd = [t.clone(memory_format=torch.contiguous_format) if odd and (t.data_ptr() != was or t is X and ldx != desc.ldx) else t
+                                 for t, odd, was in zip((X, Wg, Wu, Wd), now, read_at)]
+                ldx = _ld(X)
         if reserve.get_device() != at:
             raise ValueError("what the forward kept came back on %s" % reserve.device)
-        if not reserve.is_contiguous() or reserve.data_ptr() & 255:
+        if reserve.data_ptr() & 255 or not reserve.is_contiguous():
             reserve = reserve.clone(memory_format=torch.contiguous_format)
-        desc = _ffi.FfnDesc(desc.rows, desc.Fin, desc.H, desc.Fout, desc.activation, desc.dtype, _ld(X), desc.training, 0)
+        if ldx != desc.ldx:
+            desc = _ffi.FfnDesc(rows, Fin, H, Fout, desc.activation, desc.dtype, ldx, desc.training, 0)
         dY = dY.contiguous()
         dX = torch.empty((desc.rows, desc.Fin), dtype=X.dtype, device=dev) if need[0] else None
         dWg, dWu = (torch.empty_like(Wg), torch.empty_like(Wu)) if need[1] or need[2] else (None, None)
