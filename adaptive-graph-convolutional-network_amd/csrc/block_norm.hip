@@ -33,13 +33,13 @@ struct NormArgs {
   AgcnNormDesc d;
   // plan (nullable: no pad rows, no graphs)
   const int32_t *n, *row_off, *row_graph;
-  int32_t B, splits, graph_rows;        // per-graph gates: workgroups per graph, rows of a graph that one of them adds up
+  int32_t B, graph_log2;                // per-graph gates: log2 of the rows of a graph that one workgroup adds up
   const void *z, *x, *gate, *dy, *dh;
   const float *scale, *w, *b, *w2, *b2;
   void *y, *h, *dz, *dx, *dgate;
   float* stats;                         // [rows][4]: mean z, 1 / deviation of z, mean y, 1 / deviation of y
-  float* part;                          // [units][4][F]
-  int32_t units, stride, pads;          // partial sums; distance between those that the parameters' gradients are made of
+  float* part;                          // [units][4][F]; with a gate per graph the first B become the graphs' own
+  int32_t units, pads;                  // partial sums
 };
 
 typedef uint32_t u4f __attribute__((ext_vector_type(4), aligned(4)));
@@ -226,6 +226,21 @@ __device__ __forceinline__ bool is_pad(const NormArgs& a, int64_t row) {
   return (int)row - a.row_off[g] >= a.n[g];
 }
 
+// A gate per graph: the strips of S = 2^graph_log2 rows that the graphs are cut into, each from its first row on.  Place g: the first
+// strip of graph g.  Place B + e: the graph that holds row (e + 1) S - 1, its strip e - row_off / S + 1 (of those there are, or one
+// behind the graph's end: nothing).  That gives every further strip a place of its own -- a graph of n rows has at most as many as there
+// are such rows in it --, needs one load, and rows / S + B places, however the rows are spread over the graphs.
+__device__ __forceinline__ int strip_place(const NormArgs& a, int g, int strip) {
+  return strip ? a.B + (a.row_off[g] >> a.graph_log2) + strip - 1 : g;
+}
+__device__ __forceinline__ int strip_at(const NormArgs& a, int place, int& g) {
+  g = place;
+  if (place < a.B) return 0;
+  const int e = place - a.B;
+  g = a.row_graph[((e + 1) << a.graph_log2) - 1];
+  return e - (a.row_off[g] >> a.graph_log2) + 1;
+}
+
 template <typename TX, typename TZ, int L, int NV, bool LAYER>
 __global__ __launch_bounds__(threads_of<L>()) void norm_forward_kernel(NormArgs a) {
   constexpr int R = threads_of<L>() / L;                    // rows side by side
@@ -321,7 +336,7 @@ __global__ __launch_bounds__(threads_of<L>()) void norm_forward_kernel(NormArgs 
   }
 }
 
-// One workgroup walks a strip of rows (no gate per graph: rows block, block + grid, ..; with one: up to graph_rows rows of one
+// One workgroup walks a strip of rows (no gate per graph: rows block, block + grid, ..; with one: up to 2^graph_log2 rows of one
 // graph) and leaves the partial sums of its columns: q1, q2 (per graph: sum D zh, sum D), q3 = sum dh yh, q4 = sum dh (q2 and q4
 // for the biases of layer norms alone).
 // y is formed again from x, z and the gate, which have to be read anyway (x in y's place): the stored y may be rounded to
@@ -340,11 +355,12 @@ __global__ __launch_bounds__(threads_of<L>(), LAYER || GATED ? 3 : 4) void norm_
   const bool per_graph = GATED && a.d.gate == AGCN_GATE_GRAPH;
   int64_t row_begin, row_end, step;
   if (per_graph) {
-    const int g = blockIdx.x / a.splits, sp = blockIdx.x - g * a.splits;
-    const int lo = sp * a.graph_rows, all = a.row_off[g + 1] - a.row_off[g];   // pad rows too: their gradients are written (0)
-    if (lo >= all) return;
-    row_begin = a.row_off[g] + lo;
-    row_end = a.row_off[g] + (all < lo + a.graph_rows ? all : lo + a.graph_rows);
+    int g;
+    const int strip = strip_at(a, blockIdx.x, g), r1 = a.row_off[g + 1];   // pad rows too: their gradients are written (0)
+    row_begin = a.row_off[g] + ((int64_t)strip << a.graph_log2);
+    if (row_begin >= r1) return;
+    row_end = row_begin + (1 << a.graph_log2);
+    if (row_end > r1) row_end = r1;
     step = R;
   } else {
     row_begin = (int64_t)blockIdx.x * R;
@@ -540,7 +556,7 @@ __global__ __launch_bounds__(1024) void norm_params_kernel(ReduceArgs p) {
   const bool two = a.d.norm == AGCN_NORM_LAYER;
   float q[4] = {0.f, 0.f, 0.f, 0.f};
   if (c < F) {
-    const int64_t step = (int64_t)a.stride * 4 * F;
+    const int64_t step = (int64_t)4 * F;
     const float* t = a.part + c;
     if (a.z && a.dh && two) add_parts<true, true, true>(t, rl, a.units, step, F, q);
     else if (a.z && a.dh) add_parts<true, true, false>(t, rl, a.units, step, F, q);
@@ -575,17 +591,16 @@ __global__ __launch_bounds__(1024) void norm_params_kernel(ReduceArgs p) {
 }
 
 // A gate per graph: dg[graph] = a'(g) s (w sum D zh + b sum D), one thread per graph and column; and the graph's sums for the
-// parameters (those over z times a(g)), left in the place of its first partial.
+// parameters (those over z times a(g)), left in the place of its first strip.
 __global__ __launch_bounds__(64) void norm_graph_gate_kernel(NormArgs a) {
   const int F = a.d.F, g = blockIdx.x, c = blockIdx.y * 64 + threadIdx.x;
   if (c >= F) return;
-  const int n = (a.row_off[g + 1] - a.row_off[g] + a.graph_rows - 1) / a.graph_rows;
+  const int n = (int)(((int64_t)a.row_off[g + 1] - a.row_off[g] + (1 << a.graph_log2) - 1) >> a.graph_log2);
   const bool two = a.d.norm == AGCN_NORM_LAYER;
-  float* first = a.part + (int64_t)g * a.splits * 4 * F + c;
   float q[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
   for (int sp = 0; sp < n; ++sp) {
-    const float* t = first + (int64_t)sp * 4 * F;
+    const float* t = a.part + (int64_t)strip_place(a, g, sp) * 4 * F + c;
     q[0] += t[0];
     if (two) q[1] += t[F];
     if (a.dh) {
@@ -603,11 +618,12 @@ __global__ __launch_bounds__(64) void norm_graph_gate_kernel(NormArgs a) {
   const float o = da * sc * fmaf(w, q[0], b * q[1]);
   if (bf) reinterpret_cast<uint16_t*>(a.dgate)[(int64_t)g * F + c] = (uint16_t)pk_bf(o, 0.f);
   else static_cast<float*>(a.dgate)[(int64_t)g * F + c] = o;
-  first[0] = ga * q[0];
-  if (two) first[F] = ga * q[1];
+  float* sums = a.part + (int64_t)g * 4 * F + c;
+  sums[0] = ga * q[0];
+  if (two) sums[F] = ga * q[1];
   if (a.dh) {
-    first[2 * (int64_t)F] = q[2];
-    if (two) first[3 * (int64_t)F] = q[3];
+    sums[2 * (int64_t)F] = q[2];
+    if (two) sums[3 * (int64_t)F] = q[3];
   }
 }
 
@@ -655,10 +671,12 @@ void launch(bool back, const NormArgs& a, Shape sh, int grid, hipStream_t s) {
 }
 
 int rows_at_once(Shape sh) { return sh.L < 256 ? 256 / sh.L : 1; }
+int threads_for(Shape sh) { return sh.L < 256 ? 256 : sh.L; }
+// places for the partial sums of all graphs (a gate per graph)
+int64_t graph_units(const NormArgs& a) { return (a.d.rows >> a.graph_log2) + a.B; }
 // workgroups that walk the rows: as many as the rows ask for, up to what the chip holds (2048 threads per CU forward, 1024 backward)
 int row_grid(const AgcnNormDesc& d, Shape sh, bool back) {
-  const int T = sh.L < 256 ? 256 : sh.L;
-  const int64_t want = (d.rows + rows_at_once(sh) - 1) / rows_at_once(sh), cap = (int64_t)256 * (back ? 1024 : 2048) / T;
+  const int64_t want = (d.rows + rows_at_once(sh) - 1) / rows_at_once(sh), cap = (int64_t)256 * (back ? 1024 : 2048) / threads_for(sh);
   return (int)std::max<int64_t>(1, std::min(want, cap));
 }
 
@@ -686,14 +704,14 @@ int check_norm(const AgcnNormDesc* d, const void* plan_host, const void* plan_de
     a->n = dev.n; a->row_off = dev.row_off; a->row_graph = dev.row_graph;
     a->B = host.info.B;
     a->pads = host.info.rows != host.info.N1;
-    int32_t most = 0;                       // rows of the largest graph, its pad rows counted
-    if (d->gate == AGCN_GATE_GRAPH)
-      for (int32_t g = 0; g < host.info.B; ++g) most = std::max(most, host.row_off[g + 1] - host.row_off[g]);
-    // rows of a graph per workgroup: few enough for a thousand workgroups, up to 64 (each leaves four sums per column)
-    const int R = rows_at_once(shape_for(d->F));
-    a->graph_rows = R;
-    while (a->graph_rows < 64 && d->rows / a->graph_rows > 1024) a->graph_rows *= 2;
-    a->splits = (most + a->graph_rows - 1) / a->graph_rows;
+    if (d->gate == AGCN_GATE_GRAPH) {
+      // rows of a graph per workgroup: few enough for a thousand workgroups, up to 64 (each leaves four sums per column)
+      const Shape sh = shape_for(d->F);
+      for (int r = rows_at_once(sh); r > 1; r >>= 1) ++a->graph_log2;
+      while (a->graph_log2 < 6 && (d->rows >> a->graph_log2) > 1024) ++a->graph_log2;
+      if (graph_units(*a) > 0xffffffffll / threads_for(sh))
+        return fail(AGCN_EINVAL, "%s: %d graphs are more than one launch holds", who, host.info.B);
+    }
   } else if (d->gate == AGCN_GATE_GRAPH) {
     return fail(AGCN_EINVAL, "%s: a gate per graph needs a plan", who);
   }
@@ -716,7 +734,7 @@ int check_inputs(NormArgs* a, const AgcnNormInputs* in, const char* who) {
 }
 
 int back_units(const NormArgs& a) {
-  return a.d.gate == AGCN_GATE_GRAPH ? a.B * a.splits : row_grid(a.d, shape_for(a.d.F), true);
+  return a.d.gate == AGCN_GATE_GRAPH ? (int)graph_units(a) : row_grid(a.d, shape_for(a.d.F), true);
 }
 }  // namespace
 }  // namespace agcn
@@ -774,11 +792,9 @@ extern "C" int agcn_norm_gate_residual_backward(const AgcnNormDesc* desc, const 
   p.a = a;
   p.dscale = grads->dscale; p.dw = grads->dpost_weight; p.db = grads->dpost_bias;
   p.dw2 = grads->dpre_weight; p.db2 = grads->dpre_bias;
-  p.a.stride = 1;
   if (a.d.gate == AGCN_GATE_GRAPH) {
     hipLaunchKernelGGL(norm_graph_gate_kernel, dim3(a.B, (a.d.F + 63) / 64), dim3(64), 0, s, a);
     p.a.units = a.B;
-    p.a.stride = a.splits;
   }
   if (p.dscale || p.dw || p.db || p.dw2 || p.db2)
     hipLaunchKernelGGL(norm_params_kernel, dim3((a.d.F + 15) / 16), dim3(1024), 0, s, p);

@@ -465,3 +465,35 @@ def test_refusals_of_tensors(amd):
         kw = {**dict(z=z, x=x, pre_weight=w), **kw}
         with pytest.raises((bad, ValueError) if bad is amd.AgcnError else bad):
             amd.norm_gate_residual(kw.pop("z"), kw.pop("x"), **kw)
+
+
+def _skewed(big, small=20, count=4095):
+    """one large graph among thousands of small ones"""
+    return [small] * (count // 2) + [big] + [small] * (count - count // 2)
+
+
+def test_workspace_grows_with_the_rows_and_the_graphs_not_with_their_product(amd):
+    """A graph leaves one set of four sums per strip of its own rows (strips of eight rows or more at 256 features): at most
+    rows / 8 + B of them."""
+    lib = amd._ffi.lib()
+    F = 256
+    for ns in ([18] * 4096, _skewed(1024), _skewed(1600), [1600] * 3 + [1] * 30000, [1], [1600]):
+        plan = amd.Plan(ns)
+        d = amd._ffi.NormDesc(plan.rows, F, 0, 2, 2, 0, 0, F, F, F, 1e-6)
+        got = lib.agcn_norm_gate_residual_backward_workspace_bytes(C.byref(d), plan.host_ptr)
+        assert 0 < got <= (plan.rows // 8 + len(ns)) * 4 * F * 4 + 256, (len(ns), got)
+    many = amd.Plan(np.ones(4300000, dtype=np.int32))        # 1024 threads each: more than the 2^32 threads of a launch
+    d = amd._ffi.NormDesc(many.rows, 16384, 0, 2, 2, 0, 0, 16384, 16384, 16384, 1e-6)
+    assert lib.agcn_norm_gate_residual_backward_workspace_bytes(C.byref(d), many.host_ptr) == 0
+    assert b"graphs are more than one launch holds" in lib.agcn_last_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("F,kind,zt", [(64, "layer", "f32"), (300, "rms", "bf16"), (2050, "rms", "f32")])
+@pytest.mark.parametrize("ns", [_skewed(1600, 3, 900), [1] * 5000 + [700], [700] + [1] * 70, [2, 1, 1] * 700 + [33, 64, 65] * 40])
+def test_gate_per_graph_of_graphs_of_very_different_sizes(amd, ns, F, kind, zt):
+    plan = amd.Plan(ns, device="cuda")
+    gor = np.repeat(np.arange(len(ns)), ns)
+    d = make(len(ns) + F, sum(ns), F, "f32", zt, kind, "graph", ns)
+    ref, mag = reference(d, kind, 1e-6, "sigmoid", gor)
+    check(run(amd, d, kind, "sigmoid", plan), ref, mag, "f32", zt, sum(ns))
