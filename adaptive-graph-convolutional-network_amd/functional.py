@@ -752,14 +752,18 @@ def _rows_ptr(t):
     return None if t is None else (t.data_ptr() or 256)
 
 
-def _row_matrix(t, what, F=None):
-    """`t` as a [rows, F] matrix of f32 or bf16 whose rows are contiguous (any leading dimension)."""
+_I32 = 0x7fffffff               # descriptors hold 32 bits: a size beyond goes in as this, which every entry refuses
+_FFN_LD = 1 << 20               # agcn_gated_ffn_*: ldx
+
+
+def _row_matrix(t, what, F=None, most=_I32):
+    """`t` as a [rows, F] matrix of f32 or bf16 whose rows are contiguous, with a leading dimension of at most `most`."""
     _require_gpu(t, what)
     if t.dtype not in _DT:
         raise TypeError("%s must be float32 or bfloat16" % what)
     if t.dim() != 2 or t.shape[1] < 1 or (F is not None and t.shape[1] != F):
         raise ValueError("%s must be [rows, %s], got %s" % (what, "F" if F is None else F, tuple(t.shape)))
-    if t.stride(1) != 1 or t.stride(0) < t.shape[1]:
+    if t.stride(1) != 1 or not t.shape[1] <= t.stride(0) <= most:
         return t.contiguous()
     return t
 
@@ -803,12 +807,12 @@ def _on_device_of(t, fn, *args):
         return fn(*args)
 
 
-def _saved(t, what, shape, dtype, index):
+def _saved(t, what, shape, dtype, index, most=_I32):
     """A saved tensor for a backward on GPU `index`.  Saved-tensor hooks (save_on_cpu, a pack hook that clones) give back the
     values, not the layout: sizes, type and device are held against the forward's, and leading dimensions are taken from the
     tensor that is returned here."""
     if t.dtype is dtype and t.get_device() == index and t.shape == shape:
-        if t.is_contiguous() or (len(shape) == 2 and t.stride(1) == 1 and t.stride(0) >= shape[1]):
+        if t.is_contiguous() or (len(shape) == 2 and t.stride(1) == 1 and shape[1] <= t.stride(0) <= most):
             return t
         return t.contiguous()
     raise ValueError("%s: saved as %s %s on GPU %d, but came back as %s %s on %s" %
@@ -853,6 +857,8 @@ def _norm_forward(z, x, gate, scale, post_weight, post_bias, pre_weight, pre_bia
     post_weight, post_bias = _vector(post_weight, "post_weight", F, x), _vector(post_bias, "post_bias", F, x)
     pre_weight, pre_bias = _vector(pre_weight, "pre_weight", F, x), _vector(pre_bias, "pre_bias", F, x)
     zt = x.dtype if z is None else z.dtype
+    if F > _I32:
+        raise _ffi.AgcnError("F in 1..16384 (%d)" % F)
     desc = _ffi.NormDesc(rows, F, _ffi.NORM[norm], kind, _ffi.GATE_ACT[gate_activation], _DT[x.dtype], _DT[zt], _ld(x),
                          0 if z is None else _ld(z), 0 if gate is None else _ld(gate), eps)
     inputs = _ffi.NormInputs(_rows_ptr(z), _rows_ptr(x), _rows_ptr(gate), _ptr(scale), _ptr(post_weight), _ptr(post_bias),
@@ -984,7 +990,7 @@ def norm_gate_residual(z, x, post_weight=None, post_bias=None, gate=None, scale=
 def _ffn_forward(X, Wg, Wu, Wd, activation, keep):
     """-> (Y, what a backward needs: the tensors as the kernels read them and the reserve, the descriptor)"""
     lib = _ffi.lib()
-    X = _row_matrix(X, "node features")
+    X = _row_matrix(X, "node features", most=_FFN_LD)
     rows, Fin = X.shape
     dev = X.device
     Ws = []
@@ -1000,7 +1006,8 @@ def _ffn_forward(X, Wg, Wu, Wd, activation, keep):
     if Wg.shape[0] != Fin or Wu.shape != Wg.shape or Wd.shape[0] != H:
         raise ValueError("w_gate and w_up must be [%d, H] and w_down [H, F_out], got %s, %s, %s" %
                          (Fin, tuple(Wg.shape), tuple(Wu.shape), tuple(Wd.shape)))
-    desc = _ffi.FfnDesc(rows, Fin, H, Fout, _ffi.FFN_ACT[activation], _DT[X.dtype], _ld(X), 1 if keep else 0, 0)
+    desc = _ffi.FfnDesc(rows, min(Fin, _I32), min(H, _I32), min(Fout, _I32), _ffi.FFN_ACT[activation], _DT[X.dtype], min(_ld(X), _I32),
+                        1 if keep else 0, 0)
     rbytes, wbytes = lib.agcn_gated_ffn_reserve_bytes(C.byref(desc)), lib.agcn_gated_ffn_forward_workspace_bytes(C.byref(desc))
     if not rbytes:
         _ffi.check(-1)
@@ -1033,7 +1040,7 @@ class GatedFfnFunction(torch.autograd.Function):
         X, Wg, Wu, Wd, reserve = saved
         dev, dtype, rows, Fin, H, Fout = dY.device, dY.dtype, desc.rows, desc.Fin, desc.H, desc.Fout
         at = dY.get_device()
-        X = _saved(X, "node features", (rows, Fin), dtype, at)
+        X = _saved(X, "node features", (rows, Fin), dtype, at, _FFN_LD)
         Wg, Wu = _saved(Wg, "w_gate", (Fin, H), dtype, at).contiguous(), _saved(Wu, "w_up", (Fin, H), dtype, at).contiguous()
         Wd = _saved(Wd, "w_down", (H, Fout), dtype, at).contiguous()
         ldx = _ld(X)

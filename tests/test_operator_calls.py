@@ -264,3 +264,63 @@ def test_a_tangent_of_the_upstream_gradient_is_refused(amd, recorder, op, create
         with pytest.raises(amd.AgcnError, match="forward-mode"):
             torch.autograd.grad(out, ts, up, create_graph=create_graph)
     assert len(recorder.calls) == 1
+
+
+# (tensors without memory: the recorder reads nothing)
+def far(rows, cols, ld, dtype=f32):
+    return torch.empty_strided((rows, cols), (ld, 1), dtype=dtype, device="meta")
+
+
+@pytest.mark.parametrize("ld", [1 << 20, (1 << 20) + 8, (1 << 31) - 1, 1 << 31, (1 << 32) + 128])
+@pytest.mark.parametrize("grad", [False, True])
+def test_leading_dimensions_reach_the_library_whole(amd, recorder, ld, grad):
+    """The descriptors hold 32 bits, and gated_ffn takes up to 2^20: rows farther apart are copied together first."""
+    F = 64
+    t = {k: far(3, F, ld).requires_grad_(grad) for k in ("x", "z", "gate")}
+    out = amd.norm_gate_residual(**t, pre_weight=torch.ones(F, device="meta"))
+    X = far(3, F, ld).requires_grad_(grad)
+    W = [torch.ones(s, device="meta") for s in ((F, 32), (F, 32), (32, 8))]
+    Y = amd.gated_ffn(X, *W)
+    if grad:
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t):
+            out = amd.norm_gate_residual(**t, pre_weight=torch.ones(F, device="meta"))
+            Y = amd.gated_ffn(X, *W)
+        torch.autograd.grad(out, list(t.values()), [torch.ones_like(o) for o in out])
+        torch.autograd.grad(Y, X, torch.ones_like(Y))
+    for name, calls in recorder.calls.items():
+        for desc, *_ in calls:
+            if "ffn" in name:
+                assert desc.ldx == (ld if ld <= 1 << 20 else F), name
+            else:
+                assert (desc.ldx, desc.ldz, desc.ldg) == ((ld if ld < 1 << 31 else F),) * 3, name
+    assert len(recorder.calls) == (4 if grad else 2)
+
+
+def test_sizes_beyond_32_bits_are_refused(amd, monkeypatch):
+    """... and not taken for what their lower halves say."""
+    f = amd.functional
+    monkeypatch.setattr(f, "_require_gpu", lambda t, what: None)
+    monkeypatch.setattr(f, "_stream", lambda dev: 0)
+    monkeypatch.setattr(f, "_on_device_of", lambda t, fn, *args: fn(*args))
+    n = (1 << 32) + 64
+    x = far(2, n, n)
+    with pytest.raises(amd.AgcnError, match="F in 1..16384"):
+        amd.norm_gate_residual(None, x, pre_weight=torch.empty(n, device="meta"))
+    for F, H, O in ((n, 8, 8), (8, n, 8), (8, 8, n)):
+        with pytest.raises(amd.AgcnError, match="1..65536"):
+            amd.gated_ffn(far(2, F, F), far(F, H, H), far(F, H, H), far(H, O, O))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [f32, bf16])
+def test_rows_farther_apart_than_the_descriptors_hold(amd, dtype):
+    ld, F = (1 << 31) + 64, 40
+    buf = torch.empty(2 * ld + F, dtype=dtype, device="cuda")
+    x = buf.as_strided((3, F), (ld, 1))
+    near = cut(3, F, dtype, 1, "cuda")
+    x.copy_(near)
+    w = torch.ones(F, device="cuda")
+    W = [cut(a, b, dtype, 2 + i, "cuda", 0) for i, (a, b) in enumerate(((F, 32), (F, 32), (32, 8)))]
+    for a, b in zip(amd.norm_gate_residual(x, x, gate=x, pre_weight=w), amd.norm_gate_residual(near, near, gate=near, pre_weight=w)):
+        assert torch.equal(a, b)
+    assert torch.equal(amd.gated_ffn(x, *W), amd.gated_ffn(near, *W))
