@@ -497,3 +497,37 @@ def test_gate_per_graph_of_graphs_of_very_different_sizes(amd, ns, F, kind, zt):
     d = make(len(ns) + F, sum(ns), F, "f32", zt, kind, "graph", ns)
     ref, mag = reference(d, kind, 1e-6, "sigmoid", gor)
     check(run(amd, d, kind, "sigmoid", plan), ref, mag, "f32", zt, sum(ns))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("per_graph", [False, True])
+@pytest.mark.parametrize("act", ["tanh", "sigmoid"])
+def test_gates_by_value(amd, act, per_graph):
+    """The gate alone: x = 0, z = 1, no norms: y = a(g), dgate = a'(g) where the rows are alone in their graphs.  16 E of the value,
+    far gates and small ones included.  An e^-2|g| (e^-|g|) below 2^-126 may be flushed, and tanh's slope is 4 e / (1 + e)^2: 2^-124."""
+    g = torch.cat((torch.linspace(-100, 100, 401), torch.linspace(-6, 6, 173), torch.linspace(-0.3, 0.3, 121),
+                   torch.tensor([0.0, 1e-3, -1e-3, 1e-20, -1e-20, 1e4, -1e4, 1e30, -1e30])))
+    F = 8
+    rows = -(-len(g) // F)
+    gate = torch.cat((g, torch.zeros(rows * F - len(g)))).view(rows, F).cuda().requires_grad_(True)
+    plan = amd.Plan([1] * rows, device="cuda") if per_graph else None
+    x, z = torch.zeros(rows, F, device="cuda"), torch.ones(rows, F, device="cuda")
+    y, _ = amd.norm_gate_residual(z, x, gate=gate, gate_activation=act, plan=plan)
+    (dg,) = torch.autograd.grad(y, [gate], torch.ones_like(y))
+    v = gate.detach().double().cpu()
+    a = torch.tanh(v) if act == "tanh" else torch.sigmoid(v)
+    s, ns = torch.sigmoid(2 * v if act == "tanh" else v), torch.sigmoid(-2 * v if act == "tanh" else -v)
+    da = (4 if act == "tanh" else 1) * s * ns
+    for got, want in ((y.detach(), a), (dg, da)):
+        assert bool(((got.double().cpu() - want).abs() <= 16 * E * want.abs() + 2.0 ** -124).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("xt", ["f32", "bf16"])
+@pytest.mark.parametrize("kind,F", [("rms", 96), ("layer", 300), ("rms", 2049)])
+def test_gate_per_graph_in_bf16(amd, kind, F, xt):
+    ns = [18, 5, 48, 1, 70]
+    plan = amd.Plan(ns, device="cuda")
+    d = make(F, sum(ns), F, xt, "bf16", kind, "graph", ns)
+    ref, mag = reference(d, kind, 1e-6, "tanh", np.repeat(np.arange(len(ns)), ns))
+    check(run(amd, d, kind, "tanh", plan), ref, mag, xt, "bf16", sum(ns))

@@ -486,3 +486,48 @@ def test_refusals_of_tensors(amd):
                       (amd.AgcnError, (X, Wg.cpu(), Wu, Wd))):
         with pytest.raises(bad):
             amd.gated_ffn(*args)
+
+
+def _gate_values(act, g):
+    """act(g), act'(g) and the terms that they are made of, float64"""
+    if act == "sigmoid":
+        s, ns = torch.sigmoid(g), torch.sigmoid(-g)
+        return s, s * ns, s, s * ns
+    if act == "silu":
+        s, ns = torch.sigmoid(g), torch.sigmoid(-g)
+        return g * s, s * (1 + g * ns), (g * s).abs(), s * (1 + g.abs() * ns)
+    c = 0.5 * torch.special.erfc(-g / math.sqrt(2))
+    phi = torch.exp(-0.5 * g * g) / math.sqrt(2 * math.pi)
+    return g * c, c + g * phi, (g * c).abs(), c + g.abs() * phi
+
+
+# The gate alone: X = (v, 1), Wg picks v, Wu the one, so that G = v and U = 1 exactly, Y = act(v), dX = (act'(v), act(v)).
+# fp32: 16 E of the terms; gelu's functions of g^2 / 2 and g / sqrt 2 move by g^2 times the roundings of their arguments (3 in all).
+# bf16: e^-|g| from one rounded exponent, 2 |g| E; the fit of the normal distribution 2^-14 of its tail; the results 2^-8; with more
+# than 16384 elements of A it, dG and dU are rounded too (2^-8).  Below 2^-126 numbers, or pieces of them (2^-9 and 2^-18 of the whole),
+# may be flushed to zero: 2^-107 where the matrix pipe reads them.
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,dtype", [(1, f32), (1, bf16), (64, f32), (64, bf16)])
+@pytest.mark.parametrize("act", ["silu", "gelu", "sigmoid"])
+def test_gates_by_value(amd, act, H, dtype):
+    v = torch.cat((torch.linspace(-100, 100, 401), torch.linspace(-6, 6, 173), torch.tensor([0.0, -0.0, 1e-3, -1e-3, 1e-30, -1e-30]))).to(dtype)
+    X = torch.stack((v, torch.ones_like(v)), 1).cuda()
+    Wg, Wu, Wd = torch.zeros(2, H), torch.zeros(2, H), torch.zeros(H, 1)
+    Wg[0], Wu[1], Wd[0] = 1, 1, 1
+    Wg, Wu, Wd = (t.to(dtype).cuda() for t in (Wg, Wu, Wd))
+    g = v.double()
+    a, da, ta, tda = _gate_values(act, g)
+    rel = 16 * E + (3 * g * g * E if act == "gelu" else 0)
+    if dtype == bf16:
+        rel = rel + 2 * g.abs() * E + 2.0 ** -14 + (2 if H > 1 else 1) * B8 * 1.01
+    for rows in (len(v), 3):
+        for at in range(0, len(v), rows):
+            cut = slice(at, at + rows)
+            x, dY = X[cut], torch.ones(len(X[cut]), 1, dtype=dtype, device="cuda")
+            got = run(amd, x, Wg, Wu, Wd, dY, act)
+            for o, want, terms in ((got["Y"][:, 0], a, ta), (got["serving"][:, 0], a, ta), (got["dX"][:, 0], da, tda), (got["dX"][:, 1], a, ta)):
+                err = (o.double().cpu() - want[cut]).abs()
+                bound = (rel[cut] if torch.is_tensor(rel) else rel) * terms[cut] + 2.0 ** -107
+                assert bool((err <= bound).all()), (at, float((err / bound).max()))
+            if rows == 3 and at > 60:
+                break                                        # (the far ones; 20 calls)
