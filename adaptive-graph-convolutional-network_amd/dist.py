@@ -103,20 +103,24 @@ def _no_graph(ts):
     _no_tangents(ts)
 
 
-def _clip(ts, clip_norm, out):
-    """(lists of a hundred tensors and more: every step below is one pass in C over the list)"""
+def _looked_over(ts):
+    """devices, types, element counts (lists of a hundred tensors and more: each is one pass over the list, made once)"""
+    return _each(_T.get_device, ts), [t.dtype for t in ts], _each(_T.numel, ts)
+
+
+def _clip(ts, clip_norm, out, looked_over):
     lib = _ffi.lib()
-    where = _each(_T.get_device, ts)
-    if min(where) != max(where):
+    where, types, sizes = looked_over
+    if where.count(where[0]) != len(where):
         raise ValueError("all gradients must be on one device")
     if where[0] < 0:
         raise _ffi.AgcnError("gradients must live on the GPU: the clipping kernels have no CPU fallback")
     n = len(ts)
     try:
-        dtype = array("i", [_CLIP_DT[t.dtype] for t in ts])
+        dtype = array("i", [_CLIP_DT[t] for t in types])
     except KeyError:
         raise TypeError("gradients must be float32 or bfloat16")
-    numel = array("q", map(_T.numel, ts))
+    numel = array("q", sizes)
     ins = array("Q", map(_T.data_ptr, ts))
     outs = None
     if out is not None:
@@ -141,7 +145,7 @@ def global_norm(tensors):
     if not ts:
         raise ValueError("no tensors")
     _no_graph(ts)
-    return _clip(ts, 1.0, None)
+    return _clip(ts, 1.0, None, _looked_over(ts))
 
 
 def clip_by_global_norm(tensors, clip_norm, out=None):
@@ -158,14 +162,22 @@ def clip_by_global_norm(tensors, clip_norm, out=None):
     out = None if out is None else (tensors if out is given else list(out))
     if out is not None and len(out) != len(tensors):
         raise ValueError("out must hold one tensor per gradient (%d), got %d" % (len(tensors), len(out)))
-    at = [i for i, t in enumerate(tensors) if t is not None]
-    if not at:
-        raise ValueError("no tensors")
-    whole = len(at) == len(tensors)
-    ts = tensors if whole else [tensors[i] for i in at]
-    _no_graph(ts)
-    if not all(map(_T.is_contiguous, ts)):
+    try:
+        whole = bool(tensors) and all(map(_T.is_contiguous, tensors))
+    except TypeError:                                      # (a None entry)
+        whole = False
+    if whole:
+        ts = tensors
+        _no_graph(ts)
+    else:
+        at = [i for i, t in enumerate(tensors) if t is not None]
+        if not at:
+            raise ValueError("no tensors")
+        whole = len(at) == len(tensors)
+        ts = [tensors[i] for i in at]
+        _no_graph(ts)
         ts = [t.contiguous() for t in ts]
+    of_ts = _looked_over(ts)
     if out is None:
         os_ = [torch.empty_like(t) for t in ts]
     else:
@@ -174,10 +186,9 @@ def clip_by_global_norm(tensors, clip_norm, out=None):
             raise ValueError("out must hold a tensor for every gradient")
         if os_ is not ts:                                  # (in place: the tensors that were looked at above)
             _no_graph(os_)
-            if (not all(map(_T.is_contiguous, os_)) or _each(_T.numel, os_) != _each(_T.numel, ts) or
-                    [o.dtype for o in os_] != [t.dtype for t in ts] or _each(_T.get_device, os_) != _each(_T.get_device, ts)):
+            if not all(map(_T.is_contiguous, os_)) or _looked_over(os_) != of_ts:
                 raise ValueError("out must hold contiguous tensors of the gradients' sizes, types and device")
-    norm = _clip(ts, clip_norm, os_)
+    norm = _clip(ts, clip_norm, os_, of_ts)
     if out is None:
         if whole:
             return os_, norm
