@@ -13,9 +13,14 @@
 // memory's latency where a row after another would not.  Sums, means and column sums are fp32 (a column sum's partials, one per
 // workgroup, are added in a fixed order: no atomics); rounding happens where a result is stored, and h is taken from the unrounded
 // y.  Pad rows give zeros and take part in no sum.
-// Measured, forward / backward: 32916 x 4096 bf16 190 / 357 us (1074 MB: 5.6 TB/s; 1611 MB: 4.5 TB/s, registers leave half of the
-// forward's waves); 19202 x 1001, fp32 rows, bf16 z and a gate per element 66 / 120 us (4.1 and 3.5 TB/s: rows at odd addresses, sigmoids);
-// 4071 x 256 fp32 with a gate per graph 8 / 26 us in three launches.
+// Measured, forward / backward, a profile's averages: 32916 x 4096 bf16 203 / 381 us (1074 MB: 5.3 TB/s; 1611 MB: 4.2 TB/s, registers
+// leave half of the forward's waves); 19202 x 1001, fp32 rows, bf16 z and a gate per element 68 / 121 us (4.0 and 3.5 TB/s: rows at odd
+// addresses, sigmoids); 4071 x 256 fp32 with a gate per graph 8.6 / 23 us in three launches.
+// Wide rows spill.  The backwards of 1025 to 4096 features without gate and means spill 14 registers (60 bytes a lane) to the rows
+// fetched ahead, which pays all the same; fp32-row gated layer norms of 2049 to 4096 2 to 4; from 4097 on the layer norms' backwards
+// 20 to 65, beyond 8192, with two vectors a lane, every kernel 4 to 326.  134 M elements, forward / backward in TB/s: 4096 features bf16 rms
+// 4.8 / 4.4, layer 4.0 / 3.2, fp32 gated layer 5.0 / 5.0; 8192 4.7 / 4.3, 3.8 / 3.6, 5.2 / 3.8; 16384 4.9 / 2.7, 2.9 / 1.4, 3.3 / 1.9;
+// rows of odd widths beyond 4096 (5001) 2.2 / 1.9, 1.9 / 1.8, 3.3 / 2.5.
 #include <hip/hip_bf16.h>
 #include <hip/hip_runtime.h>
 
@@ -342,7 +347,7 @@ __global__ __launch_bounds__(threads_of<L>()) void norm_forward_kernel(NormArgs 
 // y is formed again from x, z and the gate, which have to be read anyway (x in y's place): the stored y may be rounded to
 // bf16, and a row whose features differ by less than that rounding would get a wrong yh.
 // AHEAD: the next row's operands are fetched while a row is worked on.  It pays where it costs few registers (bf16 rows, no gate, no
-// means: 32916 x 4096 463 -> 395 us); with more it spills.
+// means: 32916 x 4096 463 -> 395 us on average, although 14 registers are spilled for it); with more it costs more than it gives.
 template <typename TX, typename TZ, int L, int NV, bool LAYER, bool GATED>
 __global__ __launch_bounds__(threads_of<L>(), LAYER || GATED ? 3 : 4) void norm_backward_kernel(NormArgs a) {
   constexpr bool AHEAD = !LAYER && !GATED && NV == 1 && sizeof(TX) == 2;

@@ -6,8 +6,9 @@
 // value is finite there: neither a large nor a tiny gradient changes the answer's accuracy) and leaves one partial sum.  The
 // second pass walks the chunks BACKWARDS, so that it begins with what the first pass left in the 256 MB memory-side cache.
 // No atomics: the partial sums are added in a fixed order.
-// Measured: 571 M bf16 gradients in 96 tensors (1143 MB) 666 us: sums 215 us (5.3 TB/s), scaling 420 us (5.4 TB/s); a large copy on
-// this card reaches 4.9.  331 tensors of both types, 99 MB: 59 us on the GPU, 255 us with the host's table of tensors; 31 tensors 35 us.
+// Measured: 571 M bf16 gradients in 96 tensors (1143 MB) 667 us, on a profile's average sums 216 us (5.3 TB/s) and scaling 425 us (5.4
+// TB/s); a large copy on this card reaches 4.9.  331 tensors of both types, 99 MB: 60 us on the GPU, 226 us with the host's table of
+// tensors; 31 tensors 35 us.
 #include <hip/hip_bf16.h>
 #include <hip/hip_runtime.h>
 

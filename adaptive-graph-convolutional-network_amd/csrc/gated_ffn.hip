@@ -679,7 +679,8 @@ struct FusedArgs {
 // A chunk's gate is worked out among the next chunk's first products: the vector unit's work (as much as the matrix pipe's) is
 // hidden there (93 -> 75 us; two dependent products in a row in place of four accumulators in turn: 74 -> 70 us).  32768 x 128 x 512
 // fp32: the call 108 us as two products (80 + 31: the first has four k stages between filling and emptying its tiles, and A's planes
-// are 100 MB each way), 70 here: 1.2 PFLOP/s of bf16 products; bound by the matrix pipe and what is left of the vector unit.
+// are 100 MB each way), 70 here, the kernel 74 on a profile's average: 1.05 PFLOP/s of bf16 products; bound by the matrix pipe and what is
+// left of the vector unit.
 // bf16 calls give A to the second product in two pieces (851 x 16 x 5656, one piece: 1.5 times the error of an unrounded A; 32768 x 64 x 256
 // 12.8 -> 14.7 us, as two products 21.5).
 template <int P, int D, int WV, int ACT>
@@ -1117,9 +1118,12 @@ int op_of(const AgcnFfnDesc& d) {
   if (d.dtype == AGCN_DTYPE_BF16) return OP_BF16;
   return d.rows <= (d.training ? 160 : 320) || d.rows * (int64_t)d.H * (d.Fin + d.Fout) <= (int64_t)640 << 20 ? OP_FP32 : OP_PLANES;
 }
-// bf16 calls whose A has few elements: A, dG and dU go on in two bf16 pieces.  One rounding of each is as much error as the rounding of
-// the result on the average, but where few roundings meet in a result row the average does not hold (6 rows through 1617 x 270: 1.56
-// times the error of an unrounded A).  The second piece's products cost 0.3 to 1.2 us of a forward's 11 to 22 at that size.
+// bf16 calls whose A has few elements: A, dG and dU go on in two bf16 pieces.  Errors of a training pass's results, relative to rounding
+// them alone: two pieces 1.00 at every size; one piece 1.40 to 1.48 (a rounding of A, dG or dU is as much as one of the result), more where
+// few roundings make up a result or a tensor has few elements (6 rows through 1617 x 270 1.56, 18 through 64 x 64 1.60, 4000 through
+// 8 x 8 1.92).  The limit weighs that against time, a captured training pass with one piece / two: 64 x 64 x 256 24.1 / 26.8 us, 6 x 1617 x
+// 270 39.4 / 42.1, 1000 x 16 x 16 26.4 / 28.5; beyond the limit 260 x 64 x 256 27.2 / 33.4, 300 x 75 x 200 30.6 / 37.3, 16 x 2048 x 8192
+// 91.5 / 99.5, and where the matrix pipe is the bound fifteen products of M F H in place of nine.
 bool two_pieces(const AgcnFfnDesc& d) { return d.dtype == AGCN_DTYPE_BF16 && d.rows * d.H <= 16384; }
 bool whole_chunks(const AgcnFfnDesc& d, const void* p, int cols, int ld) {
   const int epc = d.dtype == AGCN_DTYPE_BF16 ? 8 : 4;
@@ -1175,7 +1179,7 @@ Config tile_of(int kind, int op, int nb, int splits) {
 }
 // The choice: the least time by a model of the chip's 256 CUs.  per_it[w - 1]: a k stage with w workgroups on the CU (the large tile's
 // 8 waves fill it; two middle or two to three small ones share it), fixed: a tile's first loads and its epilogue -- microseconds,
-// measured on 5003 x 1001 x 2731 (bf16) and 32768 x 128 x 512 (fp32) with every kind in turn: e.g. X^T dG, 344 middle tiles of 79
+// measured on 5003 x 1001 x 2731 (bf16) and 32768 x 128 x 512 (fp32, its training pass) with every kind in turn: e.g. X^T dG, 344 middle tiles of 79
 // stages 84 us, 172 large ones in two splits 82 + 17, small ones 105; A^T dY, 176 middle tiles 70 us, in two splits 54 + 9.
 // Splits cost their fp32 tiles' way to memory and back (4 MB a microsecond; half that through the gates' epilogues).
 Config choose(int64_t M, int64_t N, int nb, int op, int64_t iters, bool gates) {
