@@ -324,3 +324,30 @@ def test_rows_farther_apart_than_the_descriptors_hold(amd, dtype):
     for a, b in zip(amd.norm_gate_residual(x, x, gate=x, pre_weight=w), amd.norm_gate_residual(near, near, gate=near, pre_weight=w)):
         assert torch.equal(a, b)
     assert torch.equal(amd.gated_ffn(x, *W), amd.gated_ffn(near, *W))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("reentrant", [False, True])
+@pytest.mark.parametrize("dtype", [f32, bf16])
+def test_a_block_that_is_computed_again_in_the_backward(amd, dtype, reentrant):
+    """Checkpointing: the backward reads what a second forward kept, at other addresses."""
+    from torch.utils.checkpoint import checkpoint
+    rows, F, H = 90, 72, 96
+    X = cut(rows, F, dtype, 1, "cuda").requires_grad_(True)
+    W = [(cut(a, b, dtype, 2 + i, "cuda", 0) / a ** 0.5).requires_grad_(True) for i, (a, b) in enumerate(((F, H), (F, H), (H, 3 * F)))]
+    v = [(1 + 0.1 * cut(1, F, f32, 6 + i, "cuda")[0]).requires_grad_(True) for i in range(3)]
+
+    def block(x, *p):
+        wide = amd.gated_ffn(x, *p[:3])                      # z, gate: columns of one wide product
+        return amd.norm_gate_residual(wide[:, :F], x, gate=wide[:, 2 * F:], scale=p[3], post_weight=p[4], pre_weight=p[5], gate_activation="sigmoid")
+    ts = [X] + W + v
+    up = cut(rows, F, dtype, 9, "cuda"), cut(rows, F, dtype, 10, "cuda")
+
+    def grads(out):
+        for t in ts:
+            t.grad = None
+        torch.autograd.backward(out, up)
+        return [t.grad for t in ts]
+    want = grads(block(*ts))
+    for a, b in zip(want, grads(checkpoint(block, *ts, use_reentrant=reentrant))):
+        assert torch.equal(a, b)
