@@ -1421,6 +1421,29 @@ size_t carve_backward(const AgcnFfnDesc& d, void* mem, BackWs* w) {
                             std::max(product_part(d, d.Fin, d.H, 2, d.rows, pc, false), product_part(d, d.H, d.Fout, 1, d.rows, pc, false))));
   return c.off;
 }
+// A launch holds fewer than 2^32 threads.  The most that one of the call's own takes: of a product and of the sums of its parts.
+int64_t product_threads(const AgcnFfnDesc& d, int64_t M, int64_t N, int nb, int64_t K, int nseg, bool gates) {
+  const Config c = choose(M, N, nb, op_of(d), nseg * ktiles_of(d, K), gates);
+  const int64_t tiles = cdiv(M, c.bm) * cdiv(N, c.bn) * c.splits;
+  return std::max(cdiv(tiles, 8) * 8 * (c.kind == 0 ? 512 : 256), c.splits > 1 ? cdiv(M * (pad8((int)N) / 8), 32) * 256 : 0);
+}
+int check_threads(const AgcnFfnDesc& d, bool back, const char* who) {
+  const int64_t widest = std::max(std::max(d.Fin, d.H), d.Fout);
+  if (d.rows * (widest + 64) < (int64_t)1 << 26) return AGCN_OK;         // (2^15 of the smallest tiles, 256 threads each, in 64 parts: 2^29)
+  const int pc = pieces_of(d), Hp = pad8(d.H);
+  int64_t most = 0;
+  if (back) {
+    most = std::max(std::max(product_threads(d, d.rows, Hp, 1, d.Fout, 1, true), product_threads(d, d.rows, d.Fin, 1, d.H, 2 * pc, false)),
+                    std::max(product_threads(d, d.Fin, d.H, 2, d.rows, pc, false), product_threads(d, d.H, d.Fout, 1, d.rows, pc, false)));
+  } else if (fused(d)) {
+    const Fused c = fused_of(d);
+    most = std::max((int64_t)c.blocks * c.splits * 64 * c.waves, c.splits > 1 ? cdiv(d.rows * (c.ldp / 8), 32) * 256 : 0);
+  } else if (!few_rows(d)) {
+    most = std::max(product_threads(d, d.rows, Hp, 2, d.Fin, 1, true), product_threads(d, d.rows, d.Fout, 1, d.H, pc, false));
+  }
+  if (most > 0xffffffffll) return fail(AGCN_EINVAL, "%s: %lld rows at these widths are more than one launch holds", who, (long long)d.rows);
+  return AGCN_OK;
+}
 void zero(void* p, int64_t bytes, hipStream_t s) {
   hipLaunchKernelGGL(ffn_zero_kernel, dim3((unsigned)std::min<int64_t>(cdiv(bytes / 2, 256), 1 << 16)), dim3(256), 0, s, p, bytes);
 }
@@ -1453,6 +1476,7 @@ extern "C" int agcn_gated_ffn_forward(const AgcnFfnDesc* desc, const void* X, co
   if (rc != AGCN_OK) return rc;
   const AgcnFfnDesc& d = *desc;
   if (d.rows == 0) return AGCN_OK;
+  if ((rc = check_threads(d, false, who)) != AGCN_OK) return rc;
   if (!X || !Wg || !Wu || !Wd || !Y) return fail(AGCN_EINVAL, "%s: null tensor", who);
   Reserve r;
   const size_t need = carve_reserve(d, reserve, &r), wneed = forward_part(d);
@@ -1528,6 +1552,7 @@ extern "C" int agcn_gated_ffn_backward(const AgcnFfnDesc* desc, const void* X, c
     if (e != hipSuccess) return fail(AGCN_EDEVICE, "%s: %s", who, hipGetErrorString(e));
     return AGCN_OK;
   }
+  if ((rc = check_threads(d, true, who)) != AGCN_OK) return rc;
   if (!X || !Wg || !Wu || !Wd || !dY) return fail(AGCN_EINVAL, "%s: null tensor", who);
   Reserve r;
   BackWs w;

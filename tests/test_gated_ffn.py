@@ -531,3 +531,17 @@ def test_gates_by_value(amd, act, H, dtype):
                 assert bool((err <= bound).all()), (at, float((err / bound).max()))
             if rows == 3 and at > 60:
                 break                                        # (the far ones; 20 calls)
+
+
+def test_more_rows_than_a_launch_holds(amd):
+    """2^32 threads and more: refused before anything is launched (both products in one kernel; as two; the backward)."""
+    lib = amd._ffi.lib()
+    p, n = 4096, (1 << 63) - 1
+    for rows, F, H, O, dtype, training in ((1 << 30, 8, 8, 8, 1, 0), (1 << 30, 64, 32, 8, 0, 0), (1 << 30, 8, 8, 8, 1, 1),
+                                           ((1 << 31) - 257, 1, 1, 1, 1, 1)):
+        d = amd._ffi.FfnDesc(rows, F, H, O, 4, dtype, F, training, 0)
+        assert lib.agcn_gated_ffn_forward(C.byref(d), p, p, p, p, p, p, n, p, n, None) == -1
+        assert b"more than one launch holds" in lib.agcn_last_error()
+        if training:
+            assert lib.agcn_gated_ffn_backward(C.byref(d), p, p, p, p, p, p, p, p, p, p, n, p, n, None) == -1
+            assert b"more than one launch holds" in lib.agcn_last_error()
